@@ -255,6 +255,132 @@ sf_status sf_lif_multistep_events(const void* x, float* v_inout, void* spikes_ou
                                   void* stream);
 
 /* ------------------------------------------------------------------------ */
+/* Sequence operators: the learned, linear counterpart of the LIF recurrence */
+/* (a selective state space scan), the short causal convolution before it,  */
+/* and the norms around the block they form. No counterpart in the reference.*/
+/*                                                                           */
+/* Rows are tokens, channels are contiguous. Sequences come batched          */
+/* (seq_offsets NULL: sequence s is rows 0 .. length-1 of batch entry s) or  */
+/* packed (seq_offsets: n_seq + 1 int32 on the device, ascending from 0;     */
+/* sequence s is rows seq_offsets[s] .. seq_offsets[s+1]-1 of `length` rows  */
+/* in all; offsets are clamped to [0, length], so wrong ones read no other   */
+/* memory); rows of no sequence are not written. A sequence may be empty. Strides are in elements; inputs may be  */
+/* slices of wider rows, outputs are contiguous. Outputs must not overlap    */
+/* inputs. Sums and states are fp32 whatever the data type.                  */
+/* ------------------------------------------------------------------------ */
+typedef struct sf_causal_conv1d_desc {
+  int64_t length;                       /* rows per sequence; packed: rows in all */
+  int64_t x_batch_stride, x_row_stride; /* x_batch_stride is not used when packed */
+  int32_t n_seq, dim;
+  int32_t width;                        /* taps, 2 .. 8 */
+  int32_t silu;                         /* nonzero: y = silu(convolution) */
+  int32_t dtype;                        /* SF_DTYPE_* of x, y and the states */
+  int32_t w_dtype;                      /* SF_DTYPE_* of weight and bias */
+  int32_t packed;                       /* nonzero: seq_offsets is given */
+} sf_causal_conv1d_desc;
+
+/* y[t,d] = act(bias[d] + sum_k weight[d,k] x[t-(width-1)+k, d]), rows before a
+ * sequence's first from initial_state [n_seq, width-1, dim] (oldest first), or
+ * 0 where that is NULL. weight [dim, width]; bias may be NULL. final_state
+ * (same shape, may be NULL) receives the last width-1 rows of the state and
+ * the sequence together. */
+sf_status sf_causal_conv1d(const void* x, const void* weight, const void* bias, const void* initial_state,
+                           const int32_t* seq_offsets, void* y, void* final_state,
+                           const sf_causal_conv1d_desc* d, void* stream);
+/* Gradients from dy (contiguous rows) and d_final_state (may be NULL):
+ * dx (contiguous rows), dweight and dbias in w_dtype (dbias NULL without bias),
+ * d_initial_state (NULL if not wanted). No atomics: bit-identical run to run. */
+size_t sf_causal_conv1d_backward_workspace_size(const sf_causal_conv1d_desc* d);
+sf_status sf_causal_conv1d_backward(const void* x, const void* weight, const void* bias, const void* initial_state,
+                                    const int32_t* seq_offsets, const void* dy, const void* d_final_state, void* dx,
+                                    void* dweight, void* dbias, void* d_initial_state,
+                                    const sf_causal_conv1d_desc* d, void* workspace, size_t workspace_bytes,
+                                    void* stream);
+/* One token for each of n_seq rows: x [n_seq, dim] (row stride x_row_stride), y
+ * [n_seq, dim]; the states lie in a pool [n_slots, width-1, dim] and are
+ * shifted in place. state_indices (int32, distinct; NULL: row i uses slot i): a row whose
+ * index is outside [0, n_slots) is padding, its y is 0 and no state changes. */
+sf_status sf_causal_conv1d_update(const void* x, void* state_pool, const void* weight, const void* bias,
+                                  const int32_t* state_indices, void* y, int32_t n_slots,
+                                  const sf_causal_conv1d_desc* d, void* stream);
+
+typedef struct sf_selective_scan_desc {
+  int64_t length; /* rows per sequence; packed: rows in all */
+  int64_t x_batch_stride, x_row_stride, dt_batch_stride, dt_row_stride, z_batch_stride, z_row_stride;
+  int64_t b_batch_stride, b_row_stride, c_batch_stride, c_row_stride; /* a row of B or C is [groups, state] */
+  int32_t n_seq, dim;
+  int32_t state;       /* states per channel, 1 .. 128 */
+  int32_t groups;      /* divides dim: channel d reads group d / (dim / groups) of B and C */
+  int32_t dt_softplus; /* nonzero: dt = softplus(dt + dt_bias), else dt + dt_bias */
+  int32_t dtype;       /* SF_DTYPE_* of x, dt, z, B, C and y */
+  int32_t packed;      /* nonzero: seq_offsets is given */
+} sf_selective_scan_desc;
+
+/* h_t = exp(dt_t A) h_(t-1) + dt_t x_t B_t, y_t = (C_t . h_t + D x_t) silu(z_t),
+ * channel by channel: A [dim, state], D [dim] (may be NULL), dt_bias [dim] (may be
+ * NULL) fp32; z may be NULL (no gate); states [n_seq, dim, state] fp32,
+ * initial_state NULL means 0, final_state may be NULL. checkpoints (NULL
+ * unless the backward pass will run; sf_selective_scan_checkpoint_bytes, 16-byte
+ * aligned) receives the states that the backward pass starts from. */
+size_t sf_selective_scan_checkpoint_bytes(const sf_selective_scan_desc* d);
+size_t sf_selective_scan_workspace_size(const sf_selective_scan_desc* d);
+sf_status sf_selective_scan(const void* x, const void* dt, const float* A, const void* B, const void* C,
+                            const float* D, const void* z, const float* dt_bias, const float* initial_state,
+                            const int32_t* seq_offsets, void* y, float* final_state, void* checkpoints,
+                            const sf_selective_scan_desc* d, void* workspace, size_t workspace_bytes, void* stream);
+/* Gradients from dy (contiguous rows) and d_final_state (may be NULL). dx, ddt,
+ * dz (contiguous rows) and dB, dC (contiguous [rows, groups, state]) in dtype;
+ * dA, dD, d_dt_bias, d_initial_state fp32; dD, dz, d_dt_bias NULL where their
+ * input is, d_initial_state NULL if not wanted. No atomics. */
+size_t sf_selective_scan_backward_workspace_size(const sf_selective_scan_desc* d);
+sf_status sf_selective_scan_backward(const void* x, const void* dt, const float* A, const void* B, const void* C,
+                                     const float* D, const void* z, const float* dt_bias,
+                                     const int32_t* seq_offsets, const void* checkpoints, const void* dy,
+                                     const float* d_final_state, void* dx, void* ddt, float* dA, void* dB, void* dC,
+                                     float* dD, void* dz, float* d_dt_bias, float* d_initial_state,
+                                     const sf_selective_scan_desc* d, void* workspace, size_t workspace_bytes,
+                                     void* stream);
+/* One token for each of n_seq rows, states in a pool [n_slots, dim, state] fp32 updated
+ * in place; state_indices as in sf_causal_conv1d_update. */
+sf_status sf_selective_scan_update(const void* x, const void* dt, const float* A, const void* B, const void* C,
+                                   const float* D, const void* z, const float* dt_bias, float* state_pool,
+                                   const int32_t* state_indices, void* y, int32_t n_slots,
+                                   const sf_selective_scan_desc* d, void* stream);
+
+enum { SF_GATE_NONE = 0, SF_GATE_LINEAR = 1, SF_GATE_SILU = 2, SF_GATE_SIGMOID = 3 };
+typedef struct sf_block_norm_desc {
+  int64_t rows;
+  int64_t y_row_stride, residual_row_stride, gate_row_stride;
+  int64_t rows_per_gate; /* 1: a gate row for each row; > 1: one for so many rows (divides rows) */
+  int32_t dim;           /* 1 .. 16384 */
+  int32_t dtype;         /* SF_DTYPE_* of y, gate and normed */
+  int32_t res_dtype;     /* SF_DTYPE_* of the residual stream: dtype or fp32 */
+  int32_t w_dtype;       /* SF_DTYPE_* of post_weight, pre_weight and scale: dtype or fp32 */
+  int32_t gate_kind;     /* SF_GATE_* */
+  float residual_scale, eps;
+} sf_block_norm_desc;
+
+/* u = post_weight y / rms(y) (y itself where post_weight is NULL),
+ * residual_out = residual_scale residual + scale act(gate) u,
+ * normed = pre_weight residual_out / rms(residual_out), from the unrounded residual_out;
+ * rms(v) = sqrt(mean v^2 + eps). residual, scale and pre_weight may be NULL (then no
+ * normed), gate is NULL with SF_GATE_NONE. rstd (2 * rows floats, may be NULL)
+ * receives 1 / rms of both norms for the backward pass. */
+sf_status sf_block_norm(const void* y, const void* residual, const void* gate, const void* post_weight,
+                        const void* pre_weight, const void* scale, void* residual_out, void* normed, float* rstd,
+                        const sf_block_norm_desc* d, void* stream);
+/* Gradients from d_residual_out (res_dtype) and d_normed (dtype; either may be
+ * NULL: zero), contiguous rows; dy, d_residual (NULL without residual) contiguous
+ * rows, d_gate [rows / rows_per_gate, dim] (NULL without gate), d_post_weight,
+ * d_pre_weight, d_scale in w_dtype (NULL where their input is). No atomics. */
+size_t sf_block_norm_backward_workspace_size(const sf_block_norm_desc* d);
+sf_status sf_block_norm_backward(const void* y, const void* residual, const void* gate, const void* post_weight,
+                                 const void* pre_weight, const void* scale, const float* rstd,
+                                 const void* d_residual_out, const void* d_normed, void* dy, void* d_residual,
+                                 void* d_gate, void* d_post_weight, void* d_pre_weight, void* d_scale,
+                                 const sf_block_norm_desc* d, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ------------------------------------------------------------------------ */
 /* Path policy (process-wide; no counterpart in the reference, whose        */
 /* dispatch lives in Kernels/conv2d.py:1026-1178 as fixed Python rules).     */
 /* ------------------------------------------------------------------------ */

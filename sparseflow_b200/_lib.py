@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import contextlib
 import ctypes
+import functools
 import threading
 from pathlib import Path
 from typing import Optional
@@ -88,6 +89,40 @@ class LifMsDesc(ctypes.Structure):
     ]
 
 
+class CausalConv1dDesc(ctypes.Structure):
+    _fields_ = [
+        ("length", ctypes.c_int64), ("x_batch_stride", ctypes.c_int64), ("x_row_stride", ctypes.c_int64),
+        ("n_seq", ctypes.c_int32), ("dim", ctypes.c_int32), ("width", ctypes.c_int32), ("silu", ctypes.c_int32),
+        ("dtype", ctypes.c_int32), ("w_dtype", ctypes.c_int32), ("packed", ctypes.c_int32),
+    ]
+
+
+class SelectiveScanDesc(ctypes.Structure):
+    _fields_ = [
+        ("length", ctypes.c_int64),
+        ("x_batch_stride", ctypes.c_int64), ("x_row_stride", ctypes.c_int64),
+        ("dt_batch_stride", ctypes.c_int64), ("dt_row_stride", ctypes.c_int64),
+        ("z_batch_stride", ctypes.c_int64), ("z_row_stride", ctypes.c_int64),
+        ("b_batch_stride", ctypes.c_int64), ("b_row_stride", ctypes.c_int64),
+        ("c_batch_stride", ctypes.c_int64), ("c_row_stride", ctypes.c_int64),
+        ("n_seq", ctypes.c_int32), ("dim", ctypes.c_int32), ("state", ctypes.c_int32), ("groups", ctypes.c_int32),
+        ("dt_softplus", ctypes.c_int32), ("dtype", ctypes.c_int32), ("packed", ctypes.c_int32),
+    ]
+
+
+SF_GATE_NONE, SF_GATE_LINEAR, SF_GATE_SILU, SF_GATE_SIGMOID = 0, 1, 2, 3
+
+
+class BlockNormDesc(ctypes.Structure):
+    _fields_ = [
+        ("rows", ctypes.c_int64), ("y_row_stride", ctypes.c_int64), ("residual_row_stride", ctypes.c_int64),
+        ("gate_row_stride", ctypes.c_int64), ("rows_per_gate", ctypes.c_int64),
+        ("dim", ctypes.c_int32), ("dtype", ctypes.c_int32), ("res_dtype", ctypes.c_int32),
+        ("w_dtype", ctypes.c_int32), ("gate_kind", ctypes.c_int32),
+        ("residual_scale", ctypes.c_float), ("eps", ctypes.c_float),
+    ]
+
+
 # Every symbol declared in include/sparseflow_b200.h, with its ctypes signature.
 _VP = ctypes.c_void_p
 _SIGNATURES = {
@@ -119,6 +154,24 @@ _SIGNATURES = {
     "sf_sparse_conv2d_masks_or_x_workspace_size": (ctypes.c_size_t, []),
     "sf_sparse_conv2d_masks_or_x": (ctypes.c_int32, [_VP, _VP, _VP, _VP, _VP, ctypes.POINTER(ConvDesc), _VP,
                                                      ctypes.c_size_t, _VP]),
+    "sf_causal_conv1d": (ctypes.c_int32, [_VP] * 7 + [ctypes.POINTER(CausalConv1dDesc), _VP]),
+    "sf_causal_conv1d_backward_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(CausalConv1dDesc)]),
+    "sf_causal_conv1d_backward": (ctypes.c_int32, [_VP] * 11 + [ctypes.POINTER(CausalConv1dDesc), _VP,
+                                                                ctypes.c_size_t, _VP]),
+    "sf_causal_conv1d_update": (ctypes.c_int32, [_VP] * 6 + [ctypes.c_int32, ctypes.POINTER(CausalConv1dDesc), _VP]),
+    "sf_selective_scan_checkpoint_bytes": (ctypes.c_size_t, [ctypes.POINTER(SelectiveScanDesc)]),
+    "sf_selective_scan_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(SelectiveScanDesc)]),
+    "sf_selective_scan": (ctypes.c_int32, [_VP] * 13 + [ctypes.POINTER(SelectiveScanDesc), _VP, ctypes.c_size_t,
+                                                        _VP]),
+    "sf_selective_scan_backward_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(SelectiveScanDesc)]),
+    "sf_selective_scan_backward": (ctypes.c_int32, [_VP] * 21 + [ctypes.POINTER(SelectiveScanDesc), _VP,
+                                                                 ctypes.c_size_t, _VP]),
+    "sf_selective_scan_update": (ctypes.c_int32, [_VP] * 11 + [ctypes.c_int32, ctypes.POINTER(SelectiveScanDesc),
+                                                               _VP]),
+    "sf_block_norm": (ctypes.c_int32, [_VP] * 9 + [ctypes.POINTER(BlockNormDesc), _VP]),
+    "sf_block_norm_backward_workspace_size": (ctypes.c_size_t, [ctypes.POINTER(BlockNormDesc)]),
+    "sf_block_norm_backward": (ctypes.c_int32, [_VP] * 15 + [ctypes.POINTER(BlockNormDesc), _VP, ctypes.c_size_t,
+                                                             _VP]),
 }
 
 _lib = None
@@ -370,6 +423,48 @@ def lif_multistep_events(x: torch.Tensor, v: torch.Tensor, spikes: torch.Tensor,
     st = load().sf_lif_multistep_events(_ptr(x), _ptr(v), _ptr(spikes), _ptr(masks), ctypes.byref(desc), n, c, h, w,
                                         _stream(x.device))
     _check("sf_lif_multistep_events", st)
+
+
+# ----------------------------------------------------------------------------
+# Sequence operators
+# ----------------------------------------------------------------------------
+
+def call_on(device: torch.device, fn: str, *args) -> None:
+    """Calls an entry point whose last argument is the stream: the current one of `device`, whose
+    context is made current for the call where another device's is."""
+    idx = device.index if device.index is not None else torch.cuda.current_device()
+    if idx == torch.cuda.current_device():
+        st = getattr(load(), fn)(*args, raw_stream(idx))
+    else:
+        with torch.cuda.device(idx):
+            st = getattr(load(), fn)(*args, raw_stream(idx))
+    if st != SF_OK:
+        _check(fn, st)
+
+
+@functools.lru_cache(maxsize=512)
+def causal_conv1d_desc(length, x_batch_stride, x_row_stride, n_seq, dim, width, silu, dtype, w_dtype, packed):
+    """Descriptor of a convolution call, and a reference to it to pass; a decoding loop asks for the same one at
+    every step. `dtype` and `w_dtype` are torch types."""
+    desc = CausalConv1dDesc(length, x_batch_stride, x_row_stride, n_seq, dim, width, int(silu), sf_dtype(dtype),
+                            sf_dtype(w_dtype), int(packed))
+    return ctypes.byref(desc)
+
+
+@functools.lru_cache(maxsize=512)
+def selective_scan_desc(length, strides, n_seq, dim, state, groups, dt_softplus, dtype, packed):
+    """Descriptor of a scan call; `strides`: (batch, row) strides of x, dt, z, B and C, one after another."""
+    desc = SelectiveScanDesc(length, *strides, n_seq, dim, state, groups, int(dt_softplus), sf_dtype(dtype),
+                             int(packed))
+    return ctypes.byref(desc)
+
+
+@functools.lru_cache(maxsize=512)
+def block_norm_desc(rows, y_row_stride, residual_row_stride, gate_row_stride, rows_per_gate, dim, dtype, res_dtype,
+                    w_dtype, gate_kind, residual_scale, eps):
+    desc = BlockNormDesc(rows, y_row_stride, residual_row_stride, gate_row_stride, rows_per_gate, dim,
+                         sf_dtype(dtype), sf_dtype(res_dtype), sf_dtype(w_dtype), gate_kind, residual_scale, eps)
+    return ctypes.byref(desc)
 
 
 def set_path_policy(key: int, value: int) -> int:

@@ -1,0 +1,498 @@
+// The norms around a block, with its gate and residual scale, in one pass:
+//
+//   u = w_post y rstd1,  rstd1 = rsqrt(mean y^2 + eps)        (norm after the block)
+//   r' = alpha residual + scale act(gate) u                   (gate, residual scale, residual)
+//   x' = w_pre r' rstd2, rstd2 = rsqrt(mean r'^2 + eps)       (norm before the next block)
+//
+// Backward, from dr and dx (gradients of r' and x'), with yh = y rstd1, rh = r' rstd2, G = scale act(gate):
+//   dt   = dr + rstd2 (w_pre dx - rh c2),   c2 = mean(w_pre dx rh)
+//   dres = alpha dt;  dgate = dt scale u act'(gate);  dscale = sum dt act(gate) u
+//   du   = dt G;      dy = rstd1 (w_post du - yh c1),  c1 = mean(w_post du yh)
+//   dw_post = sum du yh;  dw_pre = sum dx rh
+// c1 depends on c2 through dt, but linearly: with e = w_post G yh, c1 = mean(e (dr + rstd2 w_pre dx))
+// - c2 rstd2 mean(e rh), so one reduction of three sums serves both.
+// r' is computed again from y, residual and gate: the stored one is rounded to the residual's type.
+//
+// About 14 operations an element forward and 36 backward against 4 to 7 tensors moved: HBM-bound. A block of
+// threads holds whole rows in registers, 8 neighbouring channels a thread and vector.
+#include "sequence.cuh"
+
+namespace sf {
+namespace {
+
+constexpr int kV = 8;             // channels per vector: 16 bytes of a 16-bit type
+constexpr int kMaxDim = 16384;    // 1024 threads, two vectors each
+
+struct NormArgs {
+  const void *y, *res, *gate, *w_post, *w_pre, *scale;
+  void *r_out, *x_out;
+  float* rstd;
+  const void *dr, *dx;
+  void *dy, *dres, *dgate;
+  float *part_w, *part_gate;  // backward partial sums: [blocks][3][dim], [blocks][dim]
+  long long rows, y_row, res_row, gate_row, rows_per_gate;
+  int dim, w_dtype, gate_kind;
+  float alpha, eps;
+  int vec;  // whether every row of every tensor takes vector accesses
+};
+
+// 8 channels from column c on as floats; past dim: 0.
+template <typename T>
+__device__ __forceinline__ void load8(float (&o)[kV], const T* p, int c, int dim, int vec) {
+  if (vec) {
+    if (c < dim) {
+      constexpr int W = 16 / sizeof(T);
+#pragma unroll
+      for (int h = 0; h < kV; h += W) {
+        float t[W];
+        seq::load_vec<T, W>(t, p + c + h);
+#pragma unroll
+        for (int i = 0; i < W; ++i) o[h + i] = t[i];
+      }
+      return;
+    }
+  } else if (c < dim) {
+#pragma unroll
+    for (int i = 0; i < kV; ++i) o[i] = c + i < dim ? DT<T>::to_f(p[c + i]) : 0.f;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < kV; ++i) o[i] = 0.f;
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* p, const float (&v)[kV], int c, int dim, int vec) {
+  if (c >= dim) return;
+  if (vec) {
+    constexpr int W = 16 / sizeof(T);
+#pragma unroll
+    for (int h = 0; h < kV; h += W) {
+      float t[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) t[i] = v[h + i];
+      seq::store_vec<T, W>(p + c + h, t);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < kV; ++i)
+      if (c + i < dim) p[c + i] = DT<T>::from_f(v[i]);
+  }
+}
+__device__ __forceinline__ void load_w8(float (&o)[kV], const void* p, int c, int dim, int vec, int dtype) {
+  if (!p) {
+#pragma unroll
+    for (int i = 0; i < kV; ++i) o[i] = 1.f;
+  } else if (dtype == SF_DTYPE_F32) {
+    load8<float>(o, static_cast<const float*>(p), c, dim, vec);
+  } else if (dtype == SF_DTYPE_F16) {
+    load8<__half>(o, static_cast<const __half*>(p), c, dim, vec);
+  } else {
+    load8<__nv_bfloat16>(o, static_cast<const __nv_bfloat16*>(p), c, dim, vec);
+  }
+}
+
+// act(gate) and its derivative.
+__device__ __forceinline__ float gate_act(float g, int kind) {
+  if (kind == SF_GATE_SILU) return seq::silu(g);
+  if (kind == SF_GATE_SIGMOID) return seq::sigmoid(g);
+  return g;
+}
+__device__ __forceinline__ float gate_dact(float g, int kind) {
+  if (kind == SF_GATE_SILU) return seq::dsilu(g);
+  if (kind == SF_GATE_SIGMOID) {
+    const float s = seq::sigmoid(g);
+    return s * (1.f - s);
+  }
+  return 1.f;
+}
+
+// Sums of N values over the block, in every thread; the order is fixed.
+template <int N>
+__device__ __forceinline__ void block_sum(float (&v)[N], float* buf) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+  const int warps = blockDim.x >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warps == 1) return;
+  __syncthreads();  // buf may still be read from the sum before
+  if (lane == 0)
+#pragma unroll
+    for (int n = 0; n < N; ++n) buf[w * N + n] = v[n];
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    float s = lane < warps ? buf[lane * N + n] : 0.f;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    v[n] = s;
+  }
+}
+
+template <typename T, typename R, int K>
+__global__ void __launch_bounds__(1024) norm_fwd_kernel(NormArgs a) {
+  __shared__ float buf[32];
+  const float inv = 1.f / (float)a.dim;
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const T* yp = static_cast<const T*>(a.y) + row * a.y_row;
+    float r[K][kV];
+    float s1[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * blockDim.x + threadIdx.x) * kV;
+      load8<T>(r[k], yp, c, a.dim, a.vec);
+#pragma unroll
+      for (int i = 0; i < kV; ++i) s1[0] = fmaf(r[k][i], r[k][i], s1[0]);
+    }
+    float rstd1 = 1.f;
+    if (a.w_post) {
+      block_sum<1>(s1, buf);
+      rstd1 = rsqrtf(s1[0] * inv + a.eps);
+    }
+    float s2[1] = {0.f};
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * blockDim.x + threadIdx.x) * kV;
+      float t[kV];
+      if (a.w_post) {
+        load_w8(t, a.w_post, c, a.dim, a.vec, a.w_dtype);
+#pragma unroll
+        for (int i = 0; i < kV; ++i) r[k][i] *= rstd1 * t[i];
+      }
+      if (a.scale) {
+        load_w8(t, a.scale, c, a.dim, a.vec, a.w_dtype);
+#pragma unroll
+        for (int i = 0; i < kV; ++i) r[k][i] *= t[i];
+      }
+      if (a.gate_kind != SF_GATE_NONE) {
+        load8<T>(t, static_cast<const T*>(a.gate) + row / a.rows_per_gate * a.gate_row, c, a.dim, a.vec);
+#pragma unroll
+        for (int i = 0; i < kV; ++i) r[k][i] *= gate_act(t[i], a.gate_kind);
+      }
+      if (a.res) {
+        load8<R>(t, static_cast<const R*>(a.res) + row * a.res_row, c, a.dim, a.vec);
+#pragma unroll
+        for (int i = 0; i < kV; ++i) r[k][i] = fmaf(a.alpha, t[i], r[k][i]);
+      }
+      if (a.r_out) store8<R>(static_cast<R*>(a.r_out) + row * a.dim, r[k], c, a.dim, a.vec);
+      if (c < a.dim)
+#pragma unroll
+        for (int i = 0; i < kV; ++i) s2[0] = fmaf(r[k][i], r[k][i], s2[0]);
+    }
+    float rstd2 = 1.f;
+    if (a.w_pre) {
+      block_sum<1>(s2, buf);
+      rstd2 = rsqrtf(s2[0] * inv + a.eps);
+#pragma unroll
+      for (int k = 0; k < K; ++k) {
+        const int c = (k * blockDim.x + threadIdx.x) * kV;
+        float t[kV];
+        load_w8(t, a.w_pre, c, a.dim, a.vec, a.w_dtype);
+#pragma unroll
+        for (int i = 0; i < kV; ++i) t[i] *= r[k][i] * rstd2;
+        store8<T>(static_cast<T*>(a.x_out) + row * a.dim, t, c, a.dim, a.vec);
+      }
+    }
+    if (a.rstd && threadIdx.x == 0) {
+      a.rstd[row] = rstd1;
+      a.rstd[a.rows + row] = rstd2;
+    }
+  }
+}
+
+// Block b of gate group g: rows g * group_rows + [b * per, (b + 1) * per) of the group. The sums over rows of the
+// weights' gradients (and, where one gate row serves many rows, of the gate's) stay in registers.
+template <typename T, typename R, int K, int MAXT>
+__global__ void __launch_bounds__(MAXT) norm_bwd_kernel(NormArgs a, long long group_rows, long long per) {
+  __shared__ float buf[96];
+  const float inv = 1.f / (float)a.dim;
+  const long long first = (long long)blockIdx.y * group_rows;
+  const long long begin = first + blockIdx.x * per, end = min(begin + per, first + group_rows);
+  const bool shared_gate = a.part_gate != nullptr;
+  float gpost[K][kV] = {}, gpre[K][kV] = {}, gscale[K][kV] = {}, ggate[K][kV] = {};
+  for (long long row = begin; row < end; ++row) {
+    const float rstd1 = a.w_post ? a.rstd[row] : 1.f, rstd2 = a.w_pre ? a.rstd[a.rows + row] : 0.f;
+    float yh[K][kV], rh[K][kV], dt[K][kV], dx[K][kV];
+    float s[3] = {0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * blockDim.x + threadIdx.x) * kV;
+      float wpost[kV], g[kV], t[kV];
+      load8<T>(yh[k], static_cast<const T*>(a.y) + row * a.y_row, c, a.dim, a.vec);
+      load_w8(wpost, a.w_post, c, a.dim, a.vec, a.w_dtype);
+      load_w8(g, a.scale, c, a.dim, a.vec, a.w_dtype);
+      if (a.gate_kind != SF_GATE_NONE) {
+        load8<T>(t, static_cast<const T*>(a.gate) + row / a.rows_per_gate * a.gate_row, c, a.dim, a.vec);
+#pragma unroll
+        for (int i = 0; i < kV; ++i) g[i] *= gate_act(t[i], a.gate_kind);
+      }
+#pragma unroll
+      for (int i = 0; i < kV; ++i) {
+        yh[k][i] *= rstd1;
+        rh[k][i] = g[i] * wpost[i] * yh[k][i];  // scale act(gate) u
+      }
+      if (a.res) {
+        load8<R>(t, static_cast<const R*>(a.res) + row * a.res_row, c, a.dim, a.vec);
+#pragma unroll
+        for (int i = 0; i < kV; ++i) t[i] = fmaf(a.alpha, t[i], rh[k][i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < kV; ++i) t[i] = rh[k][i];
+      }
+#pragma unroll
+      for (int i = 0; i < kV; ++i) {
+        dt[k][i] = 0.f;
+        dx[k][i] = 0.f;
+      }
+      if (a.dr) load8<R>(dt[k], static_cast<const R*>(a.dr) + row * a.dim, c, a.dim, a.vec);
+      float wpre[kV];
+      load_w8(wpre, a.w_pre, c, a.dim, a.vec, a.w_dtype);
+      if (a.dx && a.w_pre) load8<T>(dx[k], static_cast<const T*>(a.dx) + row * a.dim, c, a.dim, a.vec);
+#pragma unroll
+      for (int i = 0; i < kV; ++i) {
+        const float e = rh[k][i];  // w_post G yh
+        rh[k][i] = t[i] * rstd2;
+        gpre[k][i] = fmaf(dx[k][i], rh[k][i], gpre[k][i]);
+        const float q = wpre[i] * dx[k][i];
+        s[0] = fmaf(q, rh[k][i], s[0]);
+        dt[k][i] = fmaf(rstd2, q, dt[k][i]);
+        s[1] = fmaf(e, dt[k][i], s[1]);
+        s[2] = fmaf(e, rh[k][i], s[2]);
+      }
+    }
+    block_sum<3>(s, buf);
+    const float c2 = s[0] * inv * rstd2, c1 = a.w_post ? (s[1] - c2 * s[2]) * inv : 0.f;
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      const int c = (k * blockDim.x + threadIdx.x) * kV;
+      float wpost[kV], sc[kV], z[kV], o[kV], act[kV];
+      load_w8(wpost, a.w_post, c, a.dim, a.vec, a.w_dtype);
+      load_w8(sc, a.scale, c, a.dim, a.vec, a.w_dtype);
+#pragma unroll
+      for (int i = 0; i < kV; ++i) {
+        act[i] = 1.f;
+        dt[k][i] = fmaf(-c2, rh[k][i], dt[k][i]);
+      }
+      if (a.gate_kind != SF_GATE_NONE) {
+        load8<T>(z, static_cast<const T*>(a.gate) + row / a.rows_per_gate * a.gate_row, c, a.dim, a.vec);
+#pragma unroll
+        for (int i = 0; i < kV; ++i) {
+          act[i] = gate_act(z[i], a.gate_kind);
+          o[i] = dt[k][i] * sc[i] * wpost[i] * yh[k][i] * gate_dact(z[i], a.gate_kind);
+          ggate[k][i] += o[i];
+        }
+        if (a.dgate && !shared_gate) store8<T>(static_cast<T*>(a.dgate) + row * a.dim, o, c, a.dim, a.vec);
+      }
+#pragma unroll
+      for (int i = 0; i < kV; ++i) {
+        const float da = dt[k][i] * act[i];
+        gscale[k][i] = fmaf(da, wpost[i] * yh[k][i], gscale[k][i]);
+        const float du = da * sc[i];
+        gpost[k][i] = fmaf(du, yh[k][i], gpost[k][i]);
+        o[i] = rstd1 * fmaf(wpost[i], du, -yh[k][i] * c1);
+      }
+      store8<T>(static_cast<T*>(a.dy) + row * a.dim, o, c, a.dim, a.vec);
+      if (a.dres) {
+#pragma unroll
+        for (int i = 0; i < kV; ++i) o[i] = a.alpha * dt[k][i];
+        store8<R>(static_cast<R*>(a.dres) + row * a.dim, o, c, a.dim, a.vec);
+      }
+    }
+  }
+  const long long block = (long long)blockIdx.y * gridDim.x + blockIdx.x;
+  float* pw = a.part_w + block * 3 * a.dim;
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    const int c = (k * blockDim.x + threadIdx.x) * kV;
+#pragma unroll
+    for (int i = 0; i < kV; ++i)
+      if (c + i < a.dim) {
+        pw[c + i] = gpost[k][i];
+        pw[a.dim + c + i] = gpre[k][i];
+        pw[2 * a.dim + c + i] = gscale[k][i];
+        if (shared_gate) a.part_gate[block * a.dim + c + i] = ggate[k][i];
+      }
+  }
+}
+
+// out[g][i] = sum over j < blocks of part[g][j][stride] at i, in order.
+__global__ void norm_reduce_kernel(const float* part, long long blocks, long long stride, int n, int dtype,
+                                   void* out) {
+  const int i = blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= n) return;
+  const float* p = part + (long long)blockIdx.y * blocks * stride + i;
+  float s = 0.f;
+  for (long long j = 0; j < blocks; ++j) s += p[j * stride];
+  seq::store_param(out, (long long)blockIdx.y * n + i, dtype, s);
+}
+
+bool valid(const sf_block_norm_desc* d) {
+  if (!d || d->rows < 0 || d->dim < 1 || d->rows_per_gate < 1) return false;
+  if (dtype_size(d->dtype) == 0 || dtype_size(d->res_dtype) == 0 || dtype_size(d->w_dtype) == 0) return false;
+  if (d->res_dtype != d->dtype && d->res_dtype != SF_DTYPE_F32) return false;
+  if (d->w_dtype != d->dtype && d->w_dtype != SF_DTYPE_F32) return false;
+  if (d->gate_kind < SF_GATE_NONE || d->gate_kind > SF_GATE_SIGMOID) return false;
+  return d->rows % d->rows_per_gate == 0;
+}
+
+bool vectors_fit(const sf_block_norm_desc* d, std::initializer_list<const void*> ptrs) {
+  if (d->dim % kV || d->y_row_stride % kV || d->residual_row_stride % kV || d->gate_row_stride % kV) return false;
+  for (const void* p : ptrs)
+    if (!aligned16(p)) return false;
+  return true;
+}
+
+// Threads for a row, and vectors per thread.
+int vectors_per_thread(int dim) { return dim > 1024 * kV ? 2 : 1; }
+int threads_for(int dim, int K) {
+  const int t = (dim + kV * K - 1) / (kV * K);
+  return (t + 31) / 32 * 32;
+}
+
+struct BwdPlan {
+  long long groups, group_rows, blocks, per;
+  bool shared_gate;
+};
+BwdPlan bwd_plan(const sf_block_norm_desc* d) {
+  BwdPlan p;
+  p.shared_gate = d->gate_kind != SF_GATE_NONE && d->rows_per_gate > 1;
+  p.groups = p.shared_gate ? d->rows / d->rows_per_gate : 1;
+  p.group_rows = p.shared_gate ? d->rows_per_gate : d->rows;
+  const long long want = 592;  // blocks in all: 148 SMs, a few blocks each
+  long long blocks = (want + p.groups - 1) / p.groups;
+  if (blocks > p.group_rows) blocks = p.group_rows;
+  if (blocks < 1) blocks = 1;
+  p.per = (p.group_rows + blocks - 1) / blocks;
+  p.blocks = p.per > 0 ? (p.group_rows + p.per - 1) / p.per : 1;
+  return p;
+}
+
+NormArgs base_args(const void* y, const void* residual, const void* gate, const void* w_post, const void* w_pre,
+                   const void* scale, const sf_block_norm_desc* d) {
+  NormArgs a = {};
+  a.y = y;
+  a.res = residual;
+  a.gate = gate;
+  a.w_post = w_post;
+  a.w_pre = w_pre;
+  a.scale = scale;
+  a.rows = d->rows;
+  a.y_row = d->y_row_stride;
+  a.res_row = d->residual_row_stride;
+  a.gate_row = d->gate_row_stride;
+  a.rows_per_gate = d->rows_per_gate;
+  a.dim = d->dim;
+  a.w_dtype = d->w_dtype;
+  a.gate_kind = d->gate_kind;
+  a.alpha = d->residual_scale;
+  a.eps = d->eps;
+  return a;
+}
+
+template <typename T, typename R>
+sf_status run_fwd(const NormArgs& a, cudaStream_t st) {
+  const int K = vectors_per_thread(a.dim), threads = threads_for(a.dim, K);
+  const unsigned grid = (unsigned)(a.rows < INT32_MAX ? a.rows : INT32_MAX);
+  if (K == 1) norm_fwd_kernel<T, R, 1><<<grid, threads, 0, st>>>(a);
+  else norm_fwd_kernel<T, R, 2><<<grid, threads, 0, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
+}
+template <typename T, typename R>
+sf_status run_bwd(const NormArgs& a, const BwdPlan& p, cudaStream_t st) {
+  // The kernel wants about 90 registers with one vector a thread and 160 with two.
+  const int K = a.dim > 512 * kV ? 2 : 1, threads = threads_for(a.dim, K);
+  const dim3 grid((unsigned)p.blocks, (unsigned)p.groups);
+  if (K == 1) norm_bwd_kernel<T, R, 1, 512><<<grid, threads, 0, st>>>(a, p.group_rows, p.per);
+  else if (threads <= 512) norm_bwd_kernel<T, R, 2, 512><<<grid, threads, 0, st>>>(a, p.group_rows, p.per);
+  else norm_bwd_kernel<T, R, 2, 1024><<<grid, threads, 0, st>>>(a, p.group_rows, p.per);
+  return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
+}
+
+}  // namespace
+}  // namespace sf
+
+using namespace sf;
+
+#define SF_NORM_DISPATCH(D, CALL)                                                          \
+  do {                                                                                     \
+    if ((D)->dtype == SF_DTYPE_F32) { using T = float; using R = float; status = CALL; }   \
+    else if ((D)->dtype == SF_DTYPE_F16) {                                                 \
+      using T = __half;                                                                    \
+      if ((D)->res_dtype == SF_DTYPE_F32) { using R = float; status = CALL; }              \
+      else { using R = __half; status = CALL; }                                            \
+    } else {                                                                               \
+      using T = __nv_bfloat16;                                                             \
+      if ((D)->res_dtype == SF_DTYPE_F32) { using R = float; status = CALL; }              \
+      else { using R = __nv_bfloat16; status = CALL; }                                     \
+    }                                                                                      \
+  } while (0)
+
+extern "C" sf_status sf_block_norm(const void* y, const void* residual, const void* gate, const void* post_weight,
+                                   const void* pre_weight, const void* scale, void* residual_out, void* normed,
+                                   float* rstd, const sf_block_norm_desc* d, void* stream) {
+  if (!valid(d)) return SF_ERR_INVALID_ARG;
+  if (d->dim > kMaxDim) return SF_ERR_UNSUPPORTED;
+  if (d->rows == 0) return SF_OK;
+  if (!y || (!residual_out && !normed) || (normed && !pre_weight)) return SF_ERR_INVALID_ARG;
+  if ((d->gate_kind != SF_GATE_NONE) != (gate != nullptr)) return SF_ERR_INVALID_ARG;
+  NormArgs a = base_args(y, residual, gate, post_weight, normed ? pre_weight : nullptr, scale, d);
+  a.r_out = residual_out;
+  a.x_out = normed;
+  a.rstd = rstd;
+  a.vec = vectors_fit(d, {y, residual, gate, post_weight, pre_weight, scale, residual_out, normed});
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  sf_status status;
+  SF_NORM_DISPATCH(d, (run_fwd<T, R>(a, st)));
+  return status;
+}
+
+extern "C" size_t sf_block_norm_backward_workspace_size(const sf_block_norm_desc* d) {
+  if (!valid(d)) return 0;
+  const BwdPlan p = bwd_plan(d);
+  return (size_t)(p.blocks * p.groups) * d->dim * (p.shared_gate ? 4 : 3) * sizeof(float);
+}
+
+extern "C" sf_status sf_block_norm_backward(const void* y, const void* residual, const void* gate,
+                                            const void* post_weight, const void* pre_weight, const void* scale,
+                                            const float* rstd, const void* d_residual_out, const void* d_normed,
+                                            void* dy, void* d_residual, void* d_gate, void* d_post_weight,
+                                            void* d_pre_weight, void* d_scale, const sf_block_norm_desc* d,
+                                            void* workspace, size_t workspace_bytes, void* stream) {
+  if (!valid(d)) return SF_ERR_INVALID_ARG;
+  if (d->dim > kMaxDim) return SF_ERR_UNSUPPORTED;
+  if (d->rows > 0 && (!y || !rstd || !dy)) return SF_ERR_INVALID_ARG;
+  if ((d->gate_kind != SF_GATE_NONE) != (gate != nullptr) && d->rows > 0) return SF_ERR_INVALID_ARG;
+  if (d->rows > 0 && (!workspace || workspace_bytes < sf_block_norm_backward_workspace_size(d)))
+    return SF_ERR_WORKSPACE;
+  if (d->rows > 0 && !aligned16(workspace)) return SF_ERR_ALIGNMENT;
+  const BwdPlan p = bwd_plan(d);
+  if (p.groups > 65535) return SF_ERR_UNSUPPORTED;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const long long blocks = d->rows > 0 ? p.blocks * p.groups : 0;
+  float* part = static_cast<float*>(workspace);
+  NormArgs a = base_args(y, residual, gate, post_weight, pre_weight, scale, d);
+  a.rstd = const_cast<float*>(rstd);
+  a.dr = d_residual_out;
+  a.dx = d_normed;
+  a.dy = dy;
+  a.dres = d_residual;
+  a.dgate = d_gate;
+  a.part_w = part;
+  a.part_gate = p.shared_gate ? part + blocks * 3 * d->dim : nullptr;
+  a.vec = vectors_fit(d, {y, residual, gate, post_weight, pre_weight, scale, d_residual_out, d_normed, dy, d_residual,
+                          p.shared_gate ? nullptr : d_gate});
+  if (d->rows > 0) {
+    sf_status status;
+    SF_NORM_DISPATCH(d, (run_bwd<T, R>(a, p, st)));
+    if (status != SF_OK) return status;
+  }
+  const unsigned grid = (d->dim + 127) / 128;
+  void* outs[3] = {d_post_weight, d_pre_weight, d_scale};
+  for (int i = 0; i < 3; ++i)
+    if (outs[i])
+      norm_reduce_kernel<<<grid, 128, 0, st>>>(part + (long long)i * d->dim, blocks, 3ll * d->dim, d->dim, d->w_dtype,
+                                               outs[i]);
+  if (p.shared_gate && d_gate && d->rows > 0)
+    norm_reduce_kernel<<<dim3(grid, (unsigned)p.groups), 128, 0, st>>>(a.part_gate, p.blocks, d->dim, d->dim, d->dtype,
+                                                                       d_gate);
+  return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
+}
