@@ -8,8 +8,21 @@
 //   gx = dt S + D gp;  q = gh h_(t-1) a_t;  gdt = x S + sum_n q A;  gA = sum_t q dt;  gD = sum gp x
 //   gz = dy p silu'(z);  gdt_raw = gdt softplus'(dt_raw + bias);  gbias = sum gdt_raw;  gh0 = a_1 gh_1
 //
-// A thread owns 4 states of one channel; the LPC = ceil(state / 4) (a power of two) lanes of a channel lie next to
-// each other and add up C . h by shuffles. States past `state` have A = B = C = 0 and stay 0.
+// What bounds it: one exponential a state and row (16 a cycle and SM: 4.5e12/s) against 8 bytes a channel and row,
+// so with 16 states the exponentials take three times as long as the bytes. Next come issue slots: fp32 pairs
+// (mul/fma .f32x2) halve the multiply-adds, and everything that is per channel and row, not per state (softplus,
+// the gate, D x), is done once, by the thread that loads the element, and handed on through shared memory.
+//
+// Layout: a lane owns 4 states of one channel; the LPC = ceil(state / 4) (a power of two) lanes of a channel lie
+// next to each other. A block takes CH = 64 channels of one group (fewer above 16 states) through a segment of the
+// rows, 16 rows a tile; tile t+1 is on its way to registers while tile t is worked on. Sums over the states end in
+// a reduce-scatter over four rows and the lanes of a channel, so each lane finishes other rows.
+// States past `state` have A = B = C = 0 and stay 0; rows past the end have dt = x = 0 and change nothing.
+//
+// Few channels and long sequences leave most of the GPU idle, so sequences are cut into segments: a first kernel
+// finds what each segment adds to a state of 0 and how much it decays one (exp(A sum dt)), and the second starts
+// each segment from the sum of those before it. The exponentials are then taken twice, so one segment is kept
+// where the channels alone fill the GPU (segment_rows).
 #include "sequence.cuh"
 
 namespace sf {
@@ -17,11 +30,13 @@ namespace {
 
 using seq::Rows;
 using seq::Span;
+typedef unsigned long long u64;
 
-constexpr int kThreads = 128;
-constexpr int kS = 4;       // states per lane
+constexpr int kThreads = 128;  // of the single-token kernel
+constexpr int kS = 4;          // states per lane
 constexpr int kMaxState = 128;
-constexpr int kChunk = 16;  // rows per checkpoint, and per staged tile
+constexpr int kRows = 16;      // rows per tile, and per checkpoint
+constexpr int kHalf = 8;       // rows whose states the backward pass keeps in registers
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct ScanArgs {
@@ -30,15 +45,52 @@ struct ScanArgs {
   void *y, *dx, *ddt, *dz;
   float *final_state, *ck_out, *dinit;
   float *part_bc, *part_a, *part_d;  // backward partial sums
+  float *seg_state, *seg_dt;         // what segments add to a state [slots][dim][state], and their sum of dt [slots][dim]
   Rows rows;
+  long long seg_rows;                // rows per segment, a multiple of kRows
   long long x_batch, x_row, dt_batch, dt_row, z_batch, z_row, b_batch, b_row, c_batch, c_row;
   int dim, state, groups, softplus;
+  int vec;                           // four channels as one word: rows and pointers are aligned for it
 };
 
 __device__ __forceinline__ float ex2(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
+}
+// Pairs of fp32: each half is rounded like the scalar operation.
+__device__ __forceinline__ u64 pack2(float lo, float hi) {
+  u64 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack2(float& lo, float& hi, u64 v) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
+  u64 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
+  u64 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ u64 add2(u64 a, u64 b) {
+  u64 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float sum2(u64 a) {
+  float lo, hi;
+  unpack2(lo, hi, a);
+  return lo + hi;
+}
+__device__ __forceinline__ u64 ex2x2(u64 v) {
+  float lo, hi;
+  unpack2(lo, hi, v);
+  return pack2(ex2(lo), ex2(hi));
 }
 
 template <typename T>
@@ -52,13 +104,38 @@ __device__ __forceinline__ long long row0(const ScanArgs& a, const Span& s) {
 
 // Four values of a [.., state] row of floats from state n on, 0 past the end.
 __device__ __forceinline__ void load4(float (&o)[kS], const float* p, int n, int state) {
+  if ((state & 3) == 0) {
+    if (n < state) {
+      const float4 v = *reinterpret_cast<const float4*>(p + n);
+      o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w;
+    } else {
+      o[0] = o[1] = o[2] = o[3] = 0.f;
+    }
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < kS; ++i) o[i] = n + i < state ? p[n + i] : 0.f;
 }
 __device__ __forceinline__ void store4(float* p, const float (&v)[kS], int n, int state) {
+  if ((state & 3) == 0) {
+    if (n < state) *reinterpret_cast<float4*>(p + n) = make_float4(v[0], v[1], v[2], v[3]);
+    return;
+  }
 #pragma unroll
   for (int i = 0; i < kS; ++i)
     if (n + i < state) p[n + i] = v[i];
+}
+__device__ __forceinline__ void load4(u64 (&o)[2], const float* p, int n, int state) {
+  float v[kS];
+  load4(v, p, n, state);
+  o[0] = pack2(v[0], v[1]);
+  o[1] = pack2(v[2], v[3]);
+}
+__device__ __forceinline__ void store4(float* p, const u64 (&v)[2], int n, int state) {
+  float f[kS];
+  unpack2(f[0], f[1], v[0]);
+  unpack2(f[2], f[3], v[1]);
+  store4(p, f, n, state);
 }
 
 template <int LPC>
@@ -68,238 +145,607 @@ __device__ __forceinline__ float lanes_sum(float v) {
   return v;
 }
 
-// One block: one sequence and kThreads / LPC channels of one group.
-template <typename T, int LPC>
-__global__ void __launch_bounds__(kThreads) scan_fwd_kernel(ScanArgs a) {
-  constexpr int CH = kThreads / LPC, NP = LPC * kS;
-  __shared__ float sB[kChunk][NP], sC[kChunk][NP];
-  __shared__ float sx[kChunk][CH], sdt[kChunk][CH], sz[kChunk][CH];
-  const int per = a.dim / a.groups, tiles = (per + CH - 1) / CH;
-  const int g = blockIdx.x / tiles, d0 = g * per + (blockIdx.x % tiles) * CH, dend = (g + 1) * per;
-  const Span p = seq::seq_span(a.rows, blockIdx.y, kChunk);
-  const int q = threadIdx.x % LPC, c = threadIdx.x / LPC, d = d0 + c, n = q * kS;
-  const bool own = d < dend;
-  const T* xs = at<T>(a.x, a, p, a.x_batch, a.x_row);
-  const T* dts = at<T>(a.dt, a, p, a.dt_batch, a.dt_row);
-  const T* zs = a.z ? at<T>(a.z, a, p, a.z_batch, a.z_row) : nullptr;
-  const T* Bs = at<T>(a.B, a, p, a.b_batch, a.b_row) + (long long)g * a.state;
-  const T* Cs = at<T>(a.C, a, p, a.c_batch, a.c_row) + (long long)g * a.state;
-  T* ys = static_cast<T*>(a.y) + row0(a, p) * a.dim;
-
-  float A2[kS] = {}, h[kS] = {};
-  float D = 0.f;
-  if (own) {
-    load4(A2, a.A + (long long)d * a.state, n, a.state);
+// Sums of four rows' values over the lanes of a channel: lane q gets row q % 4 (two lanes: rows 2q and 2q + 1, one
+// lane: all four). Three shuffles where four whole reductions would take eight.
+template <int LPC>
+constexpr int kRowsPerLane = LPC >= 4 ? 1 : 4 / LPC;
+template <int LPC>
+__device__ __forceinline__ void scatter4(float (&o)[kRowsPerLane<LPC>], const float (&v)[4], int q) {
+  if constexpr (LPC == 1) {
 #pragma unroll
-    for (int i = 0; i < kS; ++i) A2[i] *= kLog2e;
-    if (a.init) load4(h, a.init + ((long long)p.s * a.dim + d) * a.state, n, a.state);
-    if (a.D) D = a.D[d];
-  }
-  for (long long t0 = 0; t0 < p.len; t0 += kChunk) {
-    const int rows = (int)min((long long)kChunk, p.len - t0);
-    if (a.ck_out && own)
-      store4(a.ck_out + ((p.slot0 + t0 / kChunk) * a.dim + d) * a.state, h, n, a.state);
-    __syncthreads();
-    for (int i = threadIdx.x; i < rows * NP; i += kThreads) {
-      const int r = i / NP, m = i % NP;
-      sB[r][m] = m < a.state ? DT<T>::to_f(Bs[(t0 + r) * a.b_row + m]) : 0.f;
-      sC[r][m] = m < a.state ? DT<T>::to_f(Cs[(t0 + r) * a.c_row + m]) : 0.f;
-    }
-    for (int i = threadIdx.x; i < rows * CH; i += kThreads) {
-      const int r = i / CH, m = i % CH;
-      if (d0 + m < dend) {
-        sx[r][m] = DT<T>::to_f(xs[(t0 + r) * a.x_row + d0 + m]);
-        float v = DT<T>::to_f(dts[(t0 + r) * a.dt_row + d0 + m]);
-        if (a.dt_bias) v += a.dt_bias[d0 + m];
-        sdt[r][m] = a.softplus ? seq::softplus(v) : v;
-        sz[r][m] = zs ? DT<T>::to_f(zs[(t0 + r) * a.z_row + d0 + m]) : 0.f;
-      } else {
-        sx[r][m] = sdt[r][m] = sz[r][m] = 0.f;
-      }
-    }
-    __syncthreads();
-    for (int r = 0; r < rows; ++r) {
-      const float dt = sdt[r][c], x = sx[r][c], u = dt * x;
-      float y = 0.f;
+    for (int i = 0; i < 4; ++i) o[i] = v[i];
+  } else if constexpr (LPC == 2) {
+    const bool b = q & 1;
+    o[0] = (b ? v[2] : v[0]) + __shfl_xor_sync(0xffffffffu, b ? v[0] : v[2], 1);
+    o[1] = (b ? v[3] : v[1]) + __shfl_xor_sync(0xffffffffu, b ? v[1] : v[3], 1);
+  } else {
+    const bool b1 = q & 2, b0 = q & 1;
+    const float k0 = (b1 ? v[2] : v[0]) + __shfl_xor_sync(0xffffffffu, b1 ? v[0] : v[2], 2);
+    const float k1 = (b1 ? v[3] : v[1]) + __shfl_xor_sync(0xffffffffu, b1 ? v[1] : v[3], 2);
+    o[0] = (b0 ? k1 : k0) + __shfl_xor_sync(0xffffffffu, b0 ? k0 : k1, 1);
 #pragma unroll
-      for (int i = 0; i < kS; ++i) {
-        h[i] = fmaf(ex2(dt * A2[i]), h[i], u * sB[r][n + i]);
-        y = fmaf(sC[r][n + i], h[i], y);
-      }
-      y = lanes_sum<LPC>(y);
-      if (q == 0 && own) {
-        y = fmaf(D, x, y);
-        if (zs) y *= seq::silu(sz[r][c]);
-        ys[(t0 + r) * a.dim + d] = DT<T>::from_f(y);
-      }
-    }
+    for (int s = 4; s < LPC; s <<= 1) o[0] += __shfl_xor_sync(0xffffffffu, o[0], s);
   }
-  if (a.final_state && own) store4(a.final_state + ((long long)p.s * a.dim + d) * a.state, h, n, a.state);
+}
+template <int LPC>
+__device__ __forceinline__ int scatter_row(int q) {  // the first row that lane q gets
+  return LPC >= 4 ? (q & 3) : q * kRowsPerLane<LPC>;
 }
 
-// Chunks of kChunk rows from the last to the first: the states of a chunk from its checkpoint, then its rows
-// backwards. Sums over channels of a chunk's gB and gC go to part_bc[tile][row][2][group, NP] and are added over the tiles by
-// scan_bc_reduce_kernel; sums over a sequence of gA, gD and gbias to part_a / part_d, added over the sequences.
-template <typename T, int LPC>
-__global__ void __launch_bounds__(kThreads) scan_bwd_kernel(ScanArgs a) {
-  constexpr int CH = kThreads / LPC, NP = LPC * kS, CW = 32 / LPC, WARPS = kThreads / 32;
-  __shared__ float sB[kChunk][NP], sC[kChunk][NP];
-  __shared__ float sx[kChunk][CH], sdt[kChunk][CH], sz[kChunk][CH], sg[kChunk][CH], sraw[kChunk][CH];
-  __shared__ float sgbc[WARPS][2][NP];
-  const int per = a.dim / a.groups, tiles = (per + CH - 1) / CH;
-  const int g = blockIdx.x / tiles, tile = blockIdx.x % tiles, d0 = g * per + tile * CH, dend = (g + 1) * per;
-  const Span p = seq::seq_span(a.rows, blockIdx.y, kChunk);
-  const int q = threadIdx.x % LPC, c = threadIdx.x / LPC, d = d0 + c, n = q * kS;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const bool own = d < dend;
-  const T* xs = at<T>(a.x, a, p, a.x_batch, a.x_row);
-  const T* dts = at<T>(a.dt, a, p, a.dt_batch, a.dt_row);
-  const T* zs = a.z ? at<T>(a.z, a, p, a.z_batch, a.z_row) : nullptr;
-  const T* Bs = at<T>(a.B, a, p, a.b_batch, a.b_row) + (long long)g * a.state;
-  const T* Cs = at<T>(a.C, a, p, a.c_batch, a.c_row) + (long long)g * a.state;
-  const long long r00 = row0(a, p);
-  const T* dys = static_cast<const T*>(a.dy) + r00 * a.dim;
-  T* dxs = static_cast<T*>(a.dx) + r00 * a.dim;
-  T* ddts = static_cast<T*>(a.ddt) + r00 * a.dim;
-  T* dzs = a.dz ? static_cast<T*>(a.dz) + r00 * a.dim : nullptr;
-  const long long total_rows = a.rows.offsets ? a.rows.length : a.rows.length * a.rows.n_seq;
+template <int LPC>
+struct Cfg {
+  static constexpr int CH = LPC <= 4 ? 64 : 256 / LPC;  // channels per block
+  static constexpr int NP = LPC * kS;
+  static constexpr int THREADS = CH * LPC;
+  static constexpr int WARPS = THREADS / 32;
+  static constexpr int UNITS = kRows * CH / 4;  // four channels of a row each
+  static constexpr int UPT = (UNITS + THREADS - 1) / THREADS;
+  static constexpr int BPT = kRows * NP / THREADS;  // elements of B (and of C) per thread
+  static constexpr int PAD = CH + 8;                // row pitch of arrays that are read four rows at a time
+};
 
-  float A[kS] = {}, gh[kS] = {}, gA[kS] = {};
-  float D = 0.f, gD = 0.f, gbias = 0.f;
-  if (own) {
-    load4(A, a.A + (long long)d * a.state, n, a.state);
-    if (a.dfinal) load4(gh, a.dfinal + ((long long)p.s * a.dim + d) * a.state, n, a.state);
-    if (a.D) D = a.D[d];
+// Which 16-byte entry of a row holds channel c: threads write channels 4l + j (j fixed), lanes read eight
+// neighbouring channels; with this exchange within groups of eight neither conflicts.
+__device__ __forceinline__ int entry(int c) { return c ^ ((c >> 3) & 3); }
+
+template <typename T>
+__device__ __forceinline__ void load_unit(seq::Vec<T, 4>& o, const T* p, int valid, int vec) {
+  if (vec && valid >= 4) {
+    o = *reinterpret_cast<const seq::Vec<T, 4>*>(p);
+    return;
   }
-  const long long chunks = (p.len + kChunk - 1) / kChunk;
-  for (long long ch = chunks - 1; ch >= 0; --ch) {
-    const long long t0 = ch * kChunk;
-    const int rows = (int)min((long long)kChunk, p.len - t0);
-    __syncthreads();
-    for (int i = threadIdx.x; i < kChunk * NP; i += kThreads) {
-      const int r = i / NP, m = i % NP;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o.v[i] = i < valid ? p[i] : DT<T>::from_f(0.f);
+}
+template <typename T>
+__device__ __forceinline__ void store_unit(T* p, const seq::Vec<T, 4>& v, int valid, int vec) {
+  if (vec && valid >= 4) {
+    *reinterpret_cast<seq::Vec<T, 4>*>(p) = v;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < valid) p[i] = v.v[i];
+}
+
+// The block's place: its group and channels, its segment of a sequence.
+template <int LPC>
+struct Place {
+  int g, tile, d0, ch;  // group, channel tile of the group, first channel, channels of the tile
+  int c, q, n, d;       // this lane's channel (in the tile and in all), lane of the channel, first state
+  bool own;
+  __device__ __forceinline__ Place(const ScanArgs& a) {
+    const int per = a.dim / a.groups, tiles = (per + Cfg<LPC>::CH - 1) / Cfg<LPC>::CH;
+    g = blockIdx.x / tiles;
+    tile = blockIdx.x % tiles;
+    d0 = g * per + tile * Cfg<LPC>::CH;
+    ch = min(Cfg<LPC>::CH, (g + 1) * per - d0);
+    c = threadIdx.x / LPC;
+    q = threadIdx.x % LPC;
+    n = q * kS;
+    d = d0 + c;
+    own = c < ch;
+  }
+};
+
+// A tile's elements on their way to shared memory: x, dt, z and dy of four channels and one row, some of B and C.
+template <typename T, int LPC, bool X, bool Z, bool GY, bool BB, bool CC>
+struct Fetch {
+  using F = Cfg<LPC>;
+  seq::Vec<T, 4> x[F::UPT], dt[F::UPT], z[F::UPT], gy[F::UPT];
+  T b[F::BPT], c[F::BPT];
+  __device__ __forceinline__ void load(const ScanArgs& a, const Place<LPC>& k, const T* xs, const T* dts,
+                                       const T* zs, const T* gys, const T* Bs, const T* Cs, long long t0, int rows) {
+#pragma unroll
+    for (int i = 0; i < F::UPT; ++i) {
+      const int u = threadIdx.x + i * F::THREADS, r = u / (F::CH / 4), m = u % (F::CH / 4) * 4;
+      const int valid = (F::UNITS % F::THREADS == 0 || u < F::UNITS) && r < rows ? k.ch - m : 0;
+      const long long t = t0 + r;
+      if (X) load_unit(x[i], xs + t * a.x_row + m, valid, a.vec);
+      load_unit(dt[i], dts + t * a.dt_row + m, valid, a.vec);
+      if (Z && zs) load_unit(z[i], zs + t * a.z_row + m, valid, a.vec);
+      if (GY) load_unit(gy[i], gys + t * a.dim + m, valid, a.vec);
+    }
+#pragma unroll
+    for (int i = 0; i < F::BPT; ++i) {
+      const int u = threadIdx.x + i * F::THREADS, r = u / F::NP, m = u % F::NP;
       const bool in = r < rows && m < a.state;
-      sB[r][m] = in ? DT<T>::to_f(Bs[(t0 + r) * a.b_row + m]) : 0.f;
-      sC[r][m] = in ? DT<T>::to_f(Cs[(t0 + r) * a.c_row + m]) : 0.f;
-    }
-    // Rows past the end have dt = x = dy = 0: they change nothing.
-    for (int i = threadIdx.x; i < kChunk * CH; i += kThreads) {
-      const int r = i / CH, m = i % CH;
-      float x = 0.f, dt = 0.f, raw = 0.f, z = 0.f, gy = 0.f;
-      if (r < rows && d0 + m < dend) {
-        x = DT<T>::to_f(xs[(t0 + r) * a.x_row + d0 + m]);
-        raw = DT<T>::to_f(dts[(t0 + r) * a.dt_row + d0 + m]);
-        if (a.dt_bias) raw += a.dt_bias[d0 + m];
-        dt = a.softplus ? seq::softplus(raw) : raw;
-        if (zs) z = DT<T>::to_f(zs[(t0 + r) * a.z_row + d0 + m]);
-        gy = DT<T>::to_f(dys[(t0 + r) * a.dim + d0 + m]);
-      }
-      sx[r][m] = x;
-      sdt[r][m] = dt;
-      sraw[r][m] = raw;
-      sz[r][m] = z;
-      sg[r][m] = gy;
-    }
-    __syncthreads();
-    float hs[kChunk + 1][kS] = {};
-    if (own) load4(hs[0], a.ck + ((p.slot0 + ch) * a.dim + d) * a.state, n, a.state);
-#pragma unroll
-    for (int r = 0; r < kChunk; ++r) {
-      const float dt = sdt[r][c], u = dt * sx[r][c];
-#pragma unroll
-      for (int i = 0; i < kS; ++i) hs[r + 1][i] = fmaf(ex2(dt * (A[i] * kLog2e)), hs[r][i], u * sB[r][n + i]);
-    }
-#pragma unroll
-    for (int r = kChunk - 1; r >= 0; --r) {
-      if (r >= rows) continue;
-      const float dt = sdt[r][c], x = sx[r][c], u = dt * x, gy = sg[r][c];
-      float pre = 0.f;
-#pragma unroll
-      for (int i = 0; i < kS; ++i) pre = fmaf(sC[r][n + i], hs[r + 1][i], pre);
-      pre = fmaf(D, x, lanes_sum<LPC>(pre));
-      float gp = gy, gz = 0.f;
-      if (zs) {
-        gp *= seq::silu(sz[r][c]);
-        gz = gy * pre * seq::dsilu(sz[r][c]);
-      }
-      float S = 0.f, qa = 0.f, vb[kS], vc[kS];
-#pragma unroll
-      for (int i = 0; i < kS; ++i) {
-        gh[i] = fmaf(gp, sC[r][n + i], gh[i]);
-        vc[i] = gp * hs[r + 1][i];
-        vb[i] = gh[i] * u;
-        S = fmaf(gh[i], sB[r][n + i], S);
-        gh[i] *= ex2(dt * (A[i] * kLog2e));
-        const float k = gh[i] * hs[r][i];
-        qa = fmaf(k, A[i], qa);
-        gA[i] = fmaf(k, dt, gA[i]);
-      }
-      S = lanes_sum<LPC>(S);
-      qa = lanes_sum<LPC>(qa);
-      float gdt = fmaf(x, S, qa);
-      if (a.softplus) gdt *= seq::sigmoid(sraw[r][c]);
-      gD = fmaf(gp, x, gD);
-      gbias += gdt;
-      if (q == 0 && own) {
-        const long long o = (t0 + r) * a.dim + d;
-        dxs[o] = DT<T>::from_f(fmaf(dt, S, D * gp));
-        ddts[o] = DT<T>::from_f(gdt);
-        if (dzs) dzs[o] = DT<T>::from_f(gz);
-      }
-#pragma unroll
-      for (int i = 0; i < kS; ++i)
-#pragma unroll
-        for (int o = 16; o >= LPC; o >>= 1) {
-          vb[i] += __shfl_xor_sync(0xffffffffu, vb[i], o);
-          vc[i] += __shfl_xor_sync(0xffffffffu, vc[i], o);
-        }
-      __syncthreads();
-      if (lane < LPC)
-#pragma unroll
-        for (int i = 0; i < kS; ++i) {
-          sgbc[warp][0][n + i] = vb[i];
-          sgbc[warp][1][n + i] = vc[i];
-        }
-      __syncthreads();
-      for (int i = threadIdx.x; i < 2 * NP; i += kThreads) {
-        float s = 0.f;
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) s += sgbc[w][i / NP][i % NP];
-        a.part_bc[(((long long)tile * total_rows + r00 + t0 + r) * 2 * a.groups + (i / NP) * a.groups + g) * NP + i % NP] = s;
-      }
+      if (BB) b[i] = in ? Bs[(t0 + r) * a.b_row + m] : DT<T>::from_f(0.f);
+      if (CC) c[i] = in ? Cs[(t0 + r) * a.c_row + m] : DT<T>::from_f(0.f);
     }
   }
-  if (!own) return;
-  const long long sd = (long long)p.s * a.dim + d;
-  if (a.dinit) store4(a.dinit + sd * a.state, gh, n, a.state);
-  store4(a.part_a + sd * a.state, gA, n, a.state);
-  if (q == 0) {
-    a.part_d[sd] = gD;
-    a.part_d[(long long)a.rows.n_seq * a.dim + sd] = gbias;
+  // dt of element j of unit i as the recurrence uses it (0 where there is no element), and its argument before softplus
+  __device__ __forceinline__ float step(const ScanArgs& a, const Place<LPC>& k, int i, int j, int rows,
+                                        float& raw) const {
+    const int u = threadIdx.x + i * F::THREADS, r = u / (F::CH / 4), m = u % (F::CH / 4) * 4 + j;
+    raw = DT<T>::to_f(dt[i].v[j]);
+    if (r >= rows || m >= k.ch) return 0.f;
+    if (a.dt_bias) raw += __ldg(a.dt_bias + k.d0 + m);
+    return a.softplus ? seq::softplus(raw) : raw;
   }
-  (void)CW;
+};
+
+// State at the start of segment j (of segment n_slots - 1 - j, going backwards): what the segments before it leave.
+template <bool REV>
+__device__ __forceinline__ void segment_start(u64 (&h)[2], const ScanArgs& a, const Span& p, const u64 (&A2)[2], int j,
+                                              int d, int n) {
+  for (int i = 0; i < j; ++i) {
+    const long long slot = p.slot0 + (REV ? p.n_slots - 1 - i : i);
+    u64 e[2];
+    load4(e, a.seg_state + (slot * a.dim + d) * a.state, n, a.state);
+    const float s = a.seg_dt[slot * a.dim + d];
+    const u64 s2 = pack2(s, s);
+    h[0] = fma2(ex2x2(mul2(s2, A2[0])), h[0], e[0]);
+    h[1] = fma2(ex2x2(mul2(s2, A2[1])), h[1], e[1]);
+  }
 }
 
-// dB, dC [rows, groups, state] from part_bc[tiles][rows][2][groups][NP].
+template <int LPC>
+__device__ __forceinline__ void load_decay(u64 (&A2)[2], const ScanArgs& a, const Place<LPC>& k) {
+  float v[kS] = {};
+  if (k.own) load4(v, a.A + (long long)k.d * a.state, k.n, a.state);
+  A2[0] = pack2(v[0] * kLog2e, v[1] * kLog2e);
+  A2[1] = pack2(v[2] * kLog2e, v[3] * kLog2e);
+}
+
+// What a segment adds to a state of 0, forwards (h = a h + dt x B) or backwards (gh = a (gh + gp C)), and its sum of
+// dt. The last segment's (backwards: the first's) is not needed.
+template <typename T, int LPC, bool REV>
+__global__ void __launch_bounds__(Cfg<LPC>::THREADS) scan_carry_kernel(ScanArgs a) {
+  using F = Cfg<LPC>;
+  __shared__ __align__(16) float4 sdu[kRows][F::CH];
+  __shared__ __align__(16) float sB[kRows][F::NP];
+  const Place<LPC> k(a);
+  const Span p = seq::slot_span(a.rows, blockIdx.y, a.seg_rows);
+  if (p.len < 0) return;
+  const int seg = (int)(blockIdx.y - p.slot0);
+  if (REV ? seg == 0 : seg == p.n_slots - 1) return;
+  const T* xs = at<T>(a.x, a, p, a.x_batch, a.x_row) + k.d0;
+  const T* dts = at<T>(a.dt, a, p, a.dt_batch, a.dt_row) + k.d0;
+  const T* zs = a.z ? at<T>(a.z, a, p, a.z_batch, a.z_row) + k.d0 : nullptr;
+  const T* gys = REV ? static_cast<const T*>(a.dy) + row0(a, p) * a.dim + k.d0 : nullptr;
+  const T* Bs = at<T>(a.B, a, p, a.b_batch, a.b_row) + (long long)k.g * a.state;
+  const T* Cs = at<T>(a.C, a, p, a.c_batch, a.c_row) + (long long)k.g * a.state;
+  u64 A2[2], h[2] = {0, 0};
+  load_decay(A2, a, k);
+  float sum = 0.f;
+  const long long r1 = min(p.r0 + a.seg_rows, p.len);
+  const int tiles = (int)((r1 - p.r0 + kRows - 1) / kRows);
+  Fetch<T, LPC, !REV, REV, REV, !REV, REV> f;
+  auto fetch = [&](int i) {
+    const long long t0 = p.r0 + (long long)(REV ? tiles - 1 - i : i) * kRows;
+    f.load(a, k, xs, dts, zs, gys, Bs, Cs, t0, (int)min((long long)kRows, r1 - t0));
+  };
+  fetch(0);
+  for (int i = 0; i < tiles; ++i) {
+    const long long t0 = p.r0 + (long long)(REV ? tiles - 1 - i : i) * kRows;
+    const int rows = (int)min((long long)kRows, r1 - t0);
+    __syncthreads();
+#pragma unroll
+    for (int v = 0; v < F::UPT; ++v) {
+      const int u = threadIdx.x + v * F::THREADS, r = u / (F::CH / 4), m = u % (F::CH / 4) * 4;
+      if (F::UNITS % F::THREADS == 0 || u < F::UNITS)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float raw, w;
+          const float dt = f.step(a, k, v, j, rows, raw);
+          if (REV) {
+            w = DT<T>::to_f(f.gy[v].v[j]);
+            if (zs) w *= seq::silu(DT<T>::to_f(f.z[v].v[j]));
+          } else {
+            w = dt * DT<T>::to_f(f.x[v].v[j]);
+          }
+          sdu[r][entry(m + j)] = make_float4(dt, dt, w, w);
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < F::BPT; ++v) {
+      const int u = threadIdx.x + v * F::THREADS;
+      sB[u / F::NP][u % F::NP] = DT<T>::to_f(REV ? f.c[v] : f.b[v]);
+    }
+    if (i + 1 < tiles) fetch(i + 1);
+    __syncthreads();
+    const int e = entry(k.c);
+#pragma unroll
+    for (int rr = 0; rr < kRows; ++rr) {
+      const int r = REV ? kRows - 1 - rr : rr;
+      const ulonglong2 du = *reinterpret_cast<const ulonglong2*>(&sdu[r][e]);
+      const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&sB[r][k.n]);
+      const u64 a0 = ex2x2(mul2(du.x, A2[0])), a1 = ex2x2(mul2(du.x, A2[1]));
+      if (REV) {
+        h[0] = mul2(a0, fma2(du.y, b.x, h[0]));
+        h[1] = mul2(a1, fma2(du.y, b.y, h[1]));
+      } else {
+        h[0] = fma2(a0, h[0], mul2(du.y, b.x));
+        h[1] = fma2(a1, h[1], mul2(du.y, b.y));
+      }
+      sum += __uint_as_float((unsigned)du.x);
+    }
+  }
+  if (!k.own) return;
+  const long long o = (long long)blockIdx.y * a.dim + k.d;
+  store4(a.seg_state + o * a.state, h, k.n, a.state);
+  if (k.q == 0) a.seg_dt[o] = sum;
+}
+
+template <typename T, int LPC>
+struct FwdSmem {
+  using F = Cfg<LPC>;
+  float4 du[kRows][F::CH];  // dt, dt, dt x, dt x
+  float2 gx[kRows][F::PAD]; // D x, gate
+  float B[kRows][F::NP], C[kRows][F::NP];
+  T out[kRows][F::PAD];
+};
+
+// One block: one segment of a sequence and CH channels of one group.
+template <typename T, int LPC>
+__global__ void __launch_bounds__(Cfg<LPC>::THREADS, 3) scan_fwd_kernel(ScanArgs a) {
+  using F = Cfg<LPC>;
+  extern __shared__ __align__(16) char smem[];
+  FwdSmem<T, LPC>& s = *reinterpret_cast<FwdSmem<T, LPC>*>(smem);
+  const Place<LPC> k(a);
+  const Span p = seq::slot_span(a.rows, blockIdx.y, a.seg_rows);
+  if (p.len < 0) return;
+  const int seg = (int)(blockIdx.y - p.slot0);
+  const T* xs = at<T>(a.x, a, p, a.x_batch, a.x_row) + k.d0;
+  const T* dts = at<T>(a.dt, a, p, a.dt_batch, a.dt_row) + k.d0;
+  const T* zs = a.z ? at<T>(a.z, a, p, a.z_batch, a.z_row) + k.d0 : nullptr;
+  const T* Bs = at<T>(a.B, a, p, a.b_batch, a.b_row) + (long long)k.g * a.state;
+  const T* Cs = at<T>(a.C, a, p, a.c_batch, a.c_row) + (long long)k.g * a.state;
+  T* ys = static_cast<T*>(a.y) + row0(a, p) * a.dim + k.d0;
+  const long long r1 = min(p.r0 + a.seg_rows, p.len);
+  const int tiles = (int)((r1 - p.r0 + kRows - 1) / kRows);
+  Fetch<T, LPC, true, true, false, true, true> f;
+  auto tile_rows = [&](int i) { return (int)min((long long)kRows, r1 - (p.r0 + (long long)i * kRows)); };
+  auto fetch = [&](int i) {
+    f.load(a, k, xs, dts, zs, nullptr, Bs, Cs, p.r0 + (long long)i * kRows, tile_rows(i));
+  };
+  auto put = [&](int i) {  // tile i's results, each row's channels together
+    const int rows = tile_rows(i);
+#pragma unroll
+    for (int v = 0; v < F::UPT; ++v) {
+      const int u = threadIdx.x + v * F::THREADS, r = u / (F::CH / 4), m = u % (F::CH / 4) * 4;
+      if ((F::UNITS % F::THREADS == 0 || u < F::UNITS) && r < rows)
+        store_unit(ys + (p.r0 + (long long)i * kRows + r) * a.dim + m,
+                   *reinterpret_cast<const seq::Vec<T, 4>*>(&s.out[r][m]), k.ch - m, a.vec);
+    }
+  };
+  if (tiles > 0) fetch(0);
+  u64 A2[2], h[2] = {0, 0};
+  load_decay(A2, a, k);
+  if (k.own) {
+    if (a.init) load4(h, a.init + ((long long)p.s * a.dim + k.d) * a.state, k.n, a.state);
+    if (seg > 0) segment_start<false>(h, a, p, A2, seg, k.d, k.n);
+  }
+  const long long ck0 = a.ck_out ? seq::seq_slot0(a.rows, p.s, kRows) + p.r0 / kRows : 0;
+  const int e = entry(k.c);
+  for (int i = 0; i < tiles; ++i) {
+    const int rows = tile_rows(i);
+    if (a.ck_out && k.own) store4(a.ck_out + ((ck0 + i) * a.dim + k.d) * a.state, h, k.n, a.state);
+    __syncthreads();
+    if (i > 0) put(i - 1);
+#pragma unroll
+    for (int v = 0; v < F::UPT; ++v) {
+      const int u = threadIdx.x + v * F::THREADS, r = u / (F::CH / 4), m = u % (F::CH / 4) * 4;
+      if (F::UNITS % F::THREADS == 0 || u < F::UNITS)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float raw;
+          const float dt = f.step(a, k, v, j, rows, raw), x = DT<T>::to_f(f.x[v].v[j]), w = dt * x;
+          const float D = a.D && m + j < k.ch ? __ldg(a.D + k.d0 + m + j) : 0.f;
+          s.du[r][entry(m + j)] = make_float4(dt, dt, w, w);
+          s.gx[r][m + j] = make_float2(D * x, zs ? seq::silu(DT<T>::to_f(f.z[v].v[j])) : 1.f);
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < F::BPT; ++v) {
+      const int u = threadIdx.x + v * F::THREADS;
+      s.B[u / F::NP][u % F::NP] = DT<T>::to_f(f.b[v]);
+      s.C[u / F::NP][u % F::NP] = DT<T>::to_f(f.c[v]);
+    }
+    if (i + 1 < tiles) fetch(i + 1);
+    __syncthreads();
+#pragma unroll
+    for (int r0 = 0; r0 < kRows; r0 += 4) {
+      float y[4], o[kRowsPerLane<LPC>];
+#pragma unroll
+      for (int rr = 0; rr < 4; ++rr) {
+        const int r = r0 + rr;
+        const ulonglong2 du = *reinterpret_cast<const ulonglong2*>(&s.du[r][e]);
+        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&s.B[r][k.n]);
+        const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(&s.C[r][k.n]);
+        h[0] = fma2(ex2x2(mul2(du.x, A2[0])), h[0], mul2(du.y, b.x));
+        h[1] = fma2(ex2x2(mul2(du.x, A2[1])), h[1], mul2(du.y, b.y));
+        y[rr] = sum2(fma2(c.x, h[0], mul2(c.y, h[1])));
+      }
+      scatter4<LPC>(o, y, k.q);
+      if (LPC <= 4 || k.q < 4)
+#pragma unroll
+        for (int j = 0; j < kRowsPerLane<LPC>; ++j) {
+          const int r = r0 + scatter_row<LPC>(k.q) + j;
+          const float2 g = s.gx[r][k.c];
+          s.out[r][k.c] = DT<T>::from_f((o[j] + g.x) * g.y);
+        }
+    }
+  }
+  if (tiles > 0) {
+    __syncthreads();
+    put(tiles - 1);
+  }
+  if (a.final_state && k.own && seg == p.n_slots - 1)
+    store4(a.final_state + ((long long)p.s * a.dim + k.d) * a.state, h, k.n, a.state);
+}
+
+template <typename T, int LPC>
+struct BwdSmem {
+  using F = Cfg<LPC>;
+  float4 du[kRows][F::CH];   // dt, dt, dt x, dt x
+  float4 gp[kRows][F::CH];   // gp, gp, D gp, x
+  float2 sg[kRows][F::PAD];  // softplus'(raw), dy silu'(z)
+  float px[kRows][F::PAD];   // D x
+  float B[kRows][F::NP], C[kRows][F::NP];
+  float bc[2][F::WARPS][kHalf][2 * F::NP];  // sums over a warp's channels, one half tile after the other
+  T dx[kRows][F::PAD], ddt[kRows][F::PAD], dz[kRows][F::PAD];
+};
+
+// Sums of 8 values over the channels of a warp: scattered over the lanes as far as they go. Returns how many values
+// this lane has in v[0..], the first of them number `first`.
+template <int LPC>
+__device__ __forceinline__ void channels_sum(float (&v)[8], int lane) {
+  int cnt = 8;
+#pragma unroll
+  for (int o = 16; o >= LPC; o >>= 1) {
+    if (cnt > 1) {
+      cnt >>= 1;
+      const bool up = lane & o;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < cnt) {
+          const float keep = up ? v[cnt + i] : v[i], send = up ? v[i] : v[cnt + i];
+          v[i] = keep + __shfl_xor_sync(0xffffffffu, send, o);
+        }
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+    }
+  }
+}
+template <int LPC>
+constexpr int kSumsPerLane = LPC <= 4 ? 1 : LPC / 4;
+template <int LPC>
+__device__ __forceinline__ int sums_first(int lane) {
+  int cnt = 8, first = 0;
+#pragma unroll
+  for (int o = 16; o >= LPC; o >>= 1)
+    if (cnt > 1) {
+      cnt >>= 1;
+      if (lane & o) first += cnt;
+    }
+  return first;
+}
+
+// Tiles from the last to the first: a tile's states again from its checkpoint, half a tile at a time in registers,
+// then its rows backwards. Sums over a block's channels of gB and gC go to part_bc[tile][row][group][2][NP], added
+// over the tiles by scan_bc_reduce_kernel; sums over a segment of gA, gD and gbias to part_a / part_d, added over
+// the segments by scan_sum_kernel. No atomics: the order of every sum is fixed.
+template <typename T, int LPC>
+__global__ void __launch_bounds__(Cfg<LPC>::THREADS, 2) scan_bwd_kernel(ScanArgs a) {
+  using F = Cfg<LPC>;
+  extern __shared__ __align__(16) char smem[];
+  BwdSmem<T, LPC>& s = *reinterpret_cast<BwdSmem<T, LPC>*>(smem);
+  const Place<LPC> k(a);
+  const Span p = seq::slot_span(a.rows, blockIdx.y, a.seg_rows);
+  const long long sd = (long long)blockIdx.y * a.dim + k.d;
+  if (p.len < 0) {  // a slot of no sequence still has a place in the sums
+    if (k.own) {
+      const u64 zero[2] = {0, 0};
+      store4(a.part_a + sd * a.state, zero, k.n, a.state);
+      if (k.q == 0) a.part_d[sd] = a.part_d[(long long)gridDim.y * a.dim + sd] = 0.f;
+    }
+    return;
+  }
+  const int seg = (int)(blockIdx.y - p.slot0), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const T* xs = at<T>(a.x, a, p, a.x_batch, a.x_row) + k.d0;
+  const T* dts = at<T>(a.dt, a, p, a.dt_batch, a.dt_row) + k.d0;
+  const T* zs = a.z ? at<T>(a.z, a, p, a.z_batch, a.z_row) + k.d0 : nullptr;
+  const T* Bs = at<T>(a.B, a, p, a.b_batch, a.b_row) + (long long)k.g * a.state;
+  const T* Cs = at<T>(a.C, a, p, a.c_batch, a.c_row) + (long long)k.g * a.state;
+  const long long r00 = row0(a, p);
+  const T* gys = static_cast<const T*>(a.dy) + r00 * a.dim + k.d0;
+  const long long total_rows = a.rows.offsets ? a.rows.length : a.rows.length * a.rows.n_seq;
+  float* bc_out = a.part_bc + ((k.tile * total_rows + r00) * a.groups + k.g) * 2 * F::NP;
+  const long long r1 = min(p.r0 + a.seg_rows, p.len);
+  const int tiles = (int)((r1 - p.r0 + kRows - 1) / kRows);
+  const long long ck0 = seq::seq_slot0(a.rows, p.s, kRows) + p.r0 / kRows;
+
+  Fetch<T, LPC, true, true, true, true, true> f;
+  auto tile_row0 = [&](int i) { return p.r0 + (long long)i * kRows; };
+  auto tile_rows = [&](int i) { return (int)min((long long)kRows, r1 - tile_row0(i)); };
+  auto put = [&](int i) {
+    const int rows = tile_rows(i);
+#pragma unroll
+    for (int v = 0; v < F::UPT; ++v) {
+      const int u = threadIdx.x + v * F::THREADS, r = u / (F::CH / 4), m = u % (F::CH / 4) * 4;
+      if ((F::UNITS % F::THREADS == 0 || u < F::UNITS) && r < rows) {
+        const long long o = (r00 + tile_row0(i) + r) * a.dim + k.d0 + m;
+        using V4 = seq::Vec<T, 4>;
+        store_unit(static_cast<T*>(a.dx) + o, *reinterpret_cast<const V4*>(&s.dx[r][m]), k.ch - m, a.vec);
+        store_unit(static_cast<T*>(a.ddt) + o, *reinterpret_cast<const V4*>(&s.ddt[r][m]), k.ch - m, a.vec);
+        if (a.dz) store_unit(static_cast<T*>(a.dz) + o, *reinterpret_cast<const V4*>(&s.dz[r][m]), k.ch - m, a.vec);
+      }
+    }
+  };
+  if (tiles > 0) f.load(a, k, xs, dts, zs, gys, Bs, Cs, tile_row0(tiles - 1), tile_rows(tiles - 1));
+  u64 A2[2], gh[2] = {0, 0}, gA[2] = {0, 0};
+  load_decay(A2, a, k);
+  if (k.own) {
+    if (a.dfinal) load4(gh, a.dfinal + ((long long)p.s * a.dim + k.d) * a.state, k.n, a.state);
+    if (seg < p.n_slots - 1) segment_start<true>(gh, a, p, A2, p.n_slots - 1 - seg, k.d, k.n);
+  }
+  float gD = 0.f, gbias = 0.f;
+  const int e = entry(k.c), first = sums_first<LPC>(lane);
+  int buf = 0;
+  for (int i = tiles - 1; i >= 0; --i) {
+    const int rows = tile_rows(i);
+    u64 h0[2] = {0, 0};
+    if (k.own) load4(h0, a.ck + ((ck0 + i) * a.dim + k.d) * a.state, k.n, a.state);
+    __syncthreads();
+    if (i + 1 < tiles) put(i + 1);
+#pragma unroll
+    for (int v = 0; v < F::UPT; ++v) {
+      const int u = threadIdx.x + v * F::THREADS, r = u / (F::CH / 4), m = u % (F::CH / 4) * 4;
+      if (F::UNITS % F::THREADS == 0 || u < F::UNITS)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          float raw;
+          const float dt = f.step(a, k, v, j, rows, raw), x = DT<T>::to_f(f.x[v].v[j]), w = dt * x;
+          const float D = a.D && m + j < k.ch ? __ldg(a.D + k.d0 + m + j) : 0.f;
+          const float gy = DT<T>::to_f(f.gy[v].v[j]);
+          float gp = gy, gz = 0.f;
+          if (zs) {
+            const float z = DT<T>::to_f(f.z[v].v[j]);
+            gp *= seq::silu(z);
+            gz = gy * seq::dsilu(z);
+          }
+          s.du[r][entry(m + j)] = make_float4(dt, dt, w, w);
+          s.gp[r][entry(m + j)] = make_float4(gp, gp, D * gp, x);
+          s.sg[r][m + j] = make_float2(a.softplus ? seq::sigmoid(raw) : 1.f, gz);
+          s.px[r][m + j] = D * x;
+        }
+    }
+#pragma unroll
+    for (int v = 0; v < F::BPT; ++v) {
+      const int u = threadIdx.x + v * F::THREADS;
+      s.B[u / F::NP][u % F::NP] = DT<T>::to_f(f.b[v]);
+      s.C[u / F::NP][u % F::NP] = DT<T>::to_f(f.c[v]);
+    }
+    if (i > 0) f.load(a, k, xs, dts, zs, gys, Bs, Cs, tile_row0(i - 1), kRows);
+    __syncthreads();
+    u64 h8[2] = {h0[0], h0[1]};
+    if (rows > kHalf) {
+#pragma unroll
+      for (int r = 0; r < kHalf; ++r) {
+        const ulonglong2 du = *reinterpret_cast<const ulonglong2*>(&s.du[r][e]);
+        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&s.B[r][k.n]);
+        h8[0] = fma2(ex2x2(mul2(du.x, A2[0])), h8[0], mul2(du.y, b.x));
+        h8[1] = fma2(ex2x2(mul2(du.x, A2[1])), h8[1], mul2(du.y, b.y));
+      }
+    }
+    u64 tA[2] = {0, 0};  // this tile's share of gA: sums of sums keep more digits than one long one
+#pragma unroll 1
+    for (int half = rows > kHalf ? 1 : 0; half >= 0; --half) {
+      const int t = half * kHalf;
+      u64 hs[kHalf + 1][2], as[kHalf][2];
+      hs[0][0] = half ? h8[0] : h0[0];
+      hs[0][1] = half ? h8[1] : h0[1];
+#pragma unroll
+      for (int r = 0; r < kHalf; ++r) {
+        const ulonglong2 du = *reinterpret_cast<const ulonglong2*>(&s.du[t + r][e]);
+        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&s.B[t + r][k.n]);
+        as[r][0] = ex2x2(mul2(du.x, A2[0]));
+        as[r][1] = ex2x2(mul2(du.x, A2[1]));
+        hs[r + 1][0] = fma2(as[r][0], hs[r][0], mul2(du.y, b.x));
+        hs[r + 1][1] = fma2(as[r][1], hs[r][1], mul2(du.y, b.y));
+      }
+#pragma unroll
+      for (int r4 = kHalf - 4; r4 >= 0; r4 -= 4) {
+        float pre[4], S[4], qa[4];
+#pragma unroll
+        for (int rr = 3; rr >= 0; --rr) {
+          const int r = r4 + rr;
+          const ulonglong2 du = *reinterpret_cast<const ulonglong2*>(&s.du[t + r][e]);
+          const u64 gp = *reinterpret_cast<const u64*>(&s.gp[t + r][e]);
+          const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&s.B[t + r][k.n]);
+          const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(&s.C[t + r][k.n]);
+          pre[rr] = sum2(fma2(c.x, hs[r + 1][0], mul2(c.y, hs[r + 1][1])));
+          gh[0] = fma2(gp, c.x, gh[0]);
+          gh[1] = fma2(gp, c.y, gh[1]);
+          S[rr] = sum2(fma2(gh[0], b.x, mul2(gh[1], b.y)));
+          float v[8];
+          unpack2(v[0], v[1], mul2(gh[0], du.y));
+          unpack2(v[2], v[3], mul2(gh[1], du.y));
+          unpack2(v[4], v[5], mul2(gp, hs[r + 1][0]));
+          unpack2(v[6], v[7], mul2(gp, hs[r + 1][1]));
+          gh[0] = mul2(gh[0], as[r][0]);
+          gh[1] = mul2(gh[1], as[r][1]);
+          const u64 q0 = mul2(gh[0], hs[r][0]), q1 = mul2(gh[1], hs[r][1]);
+          qa[rr] = sum2(fma2(q0, A2[0], mul2(q1, A2[1])));
+          tA[0] = fma2(q0, du.x, tA[0]);
+          tA[1] = fma2(q1, du.x, tA[1]);
+          channels_sum<LPC>(v, lane);
+          // value i < 4: state n + i of gB, else of gC
+          if (LPC >= 4 || (lane & 3 & ~(LPC - 1)) == 0)
+#pragma unroll
+            for (int j = 0; j < kSumsPerLane<LPC>; ++j)
+              s.bc[buf][warp][r][((first + j) >> 2) * F::NP + k.n + ((first + j) & 3)] = v[j];
+        }
+        float po[kRowsPerLane<LPC>], So[kRowsPerLane<LPC>], qo[kRowsPerLane<LPC>];
+        scatter4<LPC>(po, pre, k.q);
+        scatter4<LPC>(So, S, k.q);
+        scatter4<LPC>(qo, qa, k.q);
+        if (LPC <= 4 || k.q < 4)
+#pragma unroll
+          for (int j = 0; j < kRowsPerLane<LPC>; ++j) {
+            const int r = t + r4 + scatter_row<LPC>(k.q) + j;
+            const float4 g = s.gp[r][e];
+            const float2 sg = s.sg[r][k.c];
+            const float dt = s.du[r][e].x;
+            const float gdt = fmaf(g.w, So[j], qo[j] * (1.f / kLog2e)) * sg.x;
+            s.dx[r][k.c] = DT<T>::from_f(fmaf(dt, So[j], g.z));
+            s.ddt[r][k.c] = DT<T>::from_f(gdt);
+            s.dz[r][k.c] = DT<T>::from_f((po[j] + s.px[r][k.c]) * sg.y);
+            gD = fmaf(g.x, g.w, gD);
+            gbias += t + r4 + scatter_row<LPC>(k.q) + j < rows ? gdt : 0.f;
+          }
+      }
+      __syncthreads();
+      for (int u = threadIdx.x; u < kHalf * 2 * F::NP; u += F::THREADS) {
+        const int r = u / (2 * F::NP), m = u % (2 * F::NP);
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < F::WARPS; ++w) v += s.bc[buf][w][r][m];
+        if (t + r < rows) bc_out[(tile_row0(i) + t + r) * a.groups * 2 * F::NP + m] = v;
+      }
+      buf ^= 1;
+    }
+    gA[0] = add2(gA[0], tA[0]);
+    gA[1] = add2(gA[1], tA[1]);
+  }
+  if (tiles > 0) {
+    __syncthreads();
+    put(0);
+  }
+  gD = lanes_sum<(LPC < 4 ? LPC : 4)>(gD);
+  gbias = lanes_sum<(LPC < 4 ? LPC : 4)>(gbias);
+  if (!k.own) return;
+  if (a.dinit && seg == 0) store4(a.dinit + ((long long)p.s * a.dim + k.d) * a.state, gh, k.n, a.state);
+  store4(a.part_a + sd * a.state, gA, k.n, a.state);
+  if (k.q == 0) {
+    a.part_d[sd] = gD;
+    a.part_d[(long long)gridDim.y * a.dim + sd] = gbias;
+  }
+}
+
+// dB, dC [rows, groups, state] from part_bc[tiles][rows][groups][2][NP].
 template <typename T>
 __global__ void scan_bc_reduce_kernel(const float* part, long long rows, int tiles, int groups, int NP, int state,
                                       T* dB, T* dC) {
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  const long long per_row = 2ll * groups * NP;
-  if (i >= rows * per_row) return;
-  float s = 0.f;
-  for (int j = 0; j < tiles; ++j) s += part[j * rows * per_row + i];
-  const int m = (int)(i % NP), which = (int)(i / ((long long)groups * NP) % 2), g = (int)(i / NP % groups);
-  if (m < state) (which ? dC : dB)[(i / per_row * groups + g) * state + m] = DT<T>::from_f(s);
+  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x, n = rows * groups * 2 * NP;
+  if (i >= n) return;
+  float v = 0.f;
+#pragma unroll 8
+  for (int j = 0; j < tiles; ++j) v += part[j * n + i];
+  const int m = (int)(i % NP);
+  if (m < state) (i / NP % 2 ? dC : dB)[i / (2 * NP) * state + m] = DT<T>::from_f(v);
 }
 
 // out[i] = sum over j < count of part[j * n + i], in order.
-__global__ void scan_sum_kernel(const float* part, int count, long long n, float* out) {
+__global__ void scan_sum_kernel(const float* part, long long count, long long n, float* out) {
   const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= n) return;
-  float s = 0.f;
-  for (int j = 0; j < count; ++j) s += part[j * n + i];
-  out[i] = s;
+  float v = 0.f;
+#pragma unroll 8
+  for (long long j = 0; j < count; ++j) v += part[j * n + i];
+  out[i] = v;
 }
 
 template <typename T, int LPC>
@@ -350,9 +796,33 @@ int lanes(int state) {
   while (l * kS < state) l *= 2;
   return l;
 }
-int tiles_of(const sf_selective_scan_desc* d) {
-  const int ch = kThreads / lanes(d->state), per = d->dim / d->groups;
+int channels_per_block(int state) { return lanes(state) <= 4 ? 64 : 256 / lanes(state); }
+int tiles_of(const sf_selective_scan_desc* d) {  // blocks for the channels of a group
+  const int ch = channels_per_block(d->state), per = d->dim / d->groups;
   return (per + ch - 1) / ch;
+}
+constexpr long long kWhole = 1ll << 40;  // rows of a segment that takes any sequence whole
+
+// Rows per segment: sequences whole where their channels alone give `want` blocks; else cut so that they do, but
+// not below 128 rows, nor into more than 32 segments.
+long long segment_rows(const sf_selective_scan_desc* d, long long want) {
+  const long long blocks = (long long)tiles_of(d) * d->groups * d->n_seq;
+  if (blocks >= want || d->length <= 256) return kWhole;
+  const long long total = d->packed ? d->length : d->length * d->n_seq;
+  const long long cuts = (want + (long long)tiles_of(d) * d->groups - 1) / ((long long)tiles_of(d) * d->groups);
+  long long rows = (total + cuts - 1) / cuts;
+  if (rows < 128) rows = 128;
+  if (rows < (d->length + 31) / 32) rows = (d->length + 31) / 32;
+  rows = (rows + kRows - 1) / kRows * kRows;
+  return rows >= d->length ? kWhole : rows;
+}
+constexpr long long kFwdBlocks = 444, kBwdBlocks = 296;  // three, two blocks for each SM
+long long slots_of(const sf_selective_scan_desc* d, long long seg) {
+  return seq::total_slots(d->length, d->n_seq, d->packed, seg);
+}
+// Floats of seg_state and seg_dt.
+long long carry_floats(const sf_selective_scan_desc* d, long long seg) {
+  return seg == kWhole ? 0 : (slots_of(d, seg) * d->dim * (d->state + 1ll) + 3) / 4 * 4;
 }
 long long rows_of(const sf_selective_scan_desc* d) {
   return d->n_seq == 0 ? 0 : (d->packed ? d->length : d->length * d->n_seq);
@@ -387,17 +857,55 @@ ScanArgs base_args(const void* x, const void* dt, const float* A, const void* B,
   return a;
 }
 
-struct BwdLayout {  // floats
-  long long bc, a, d, total;
+struct BwdLayout {  // floats from the start of the workspace
+  long long carry, bc, a, d, total;
 };
-BwdLayout bwd_layout(const sf_selective_scan_desc* d, long long rows) {
+BwdLayout bwd_layout(const sf_selective_scan_desc* d, long long seg) {
   BwdLayout l;
-  const long long np = (long long)lanes(d->state) * kS;
-  l.bc = 0;
-  l.a = (tiles_of(d) * rows * 2 * d->groups * np + 3) / 4 * 4;
-  l.d = l.a + (long long)d->n_seq * d->dim * d->state;
-  l.total = l.d + 2ll * d->n_seq * d->dim;
+  const long long np = (long long)lanes(d->state) * kS, slots = slots_of(d, seg);
+  l.carry = 0;
+  l.bc = carry_floats(d, seg);
+  l.a = l.bc + (tiles_of(d) * rows_of(d) * 2 * d->groups * np + 3) / 4 * 4;
+  l.d = l.a + (slots * d->dim * d->state + 3) / 4 * 4;
+  l.total = l.d + 2 * slots * d->dim;
   return l;
+}
+
+// Whether four channels can be read and written as one word: every row of every group begins at a multiple.
+bool vectors_fit(const sf_selective_scan_desc* d, std::initializer_list<const void*> ptrs) {
+  if ((d->dim / d->groups) % 4) return false;
+  for (long long v : {d->x_row_stride, d->dt_row_stride, d->z_row_stride})
+    if (v % 4) return false;
+  if (!d->packed && d->n_seq > 1)
+    for (long long v : {d->x_batch_stride, d->dt_batch_stride, d->z_batch_stride})
+      if (v % 4) return false;
+  for (const void* p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) % (4 * dtype_size(d->dtype))) return false;
+  return true;
+}
+
+template <typename K>
+bool prepare_smem(K kernel, size_t bytes) {
+  return bytes <= 48 * 1024 || allow_max_smem(reinterpret_cast<const void*>(kernel));
+}
+
+template <typename T, int LPC>
+sf_status run_fwd(const ScanArgs& a, dim3 grid, cudaStream_t st) {
+  constexpr int threads = Cfg<LPC>::THREADS;
+  if (a.seg_rows != kWhole) scan_carry_kernel<T, LPC, false><<<grid, threads, 0, st>>>(a);
+  constexpr size_t smem = sizeof(FwdSmem<T, LPC>);
+  if (!prepare_smem(scan_fwd_kernel<T, LPC>, smem)) return SF_ERR_CUDA;
+  scan_fwd_kernel<T, LPC><<<grid, threads, smem, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
+}
+template <typename T, int LPC>
+sf_status run_bwd(const ScanArgs& a, dim3 grid, cudaStream_t st) {
+  constexpr int threads = Cfg<LPC>::THREADS;
+  if (a.seg_rows != kWhole) scan_carry_kernel<T, LPC, true><<<grid, threads, 0, st>>>(a);
+  constexpr size_t smem = sizeof(BwdSmem<T, LPC>);
+  if (!prepare_smem(scan_bwd_kernel<T, LPC>, smem)) return SF_ERR_CUDA;
+  scan_bwd_kernel<T, LPC><<<grid, threads, smem, st>>>(a);
+  return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
 }
 
 }  // namespace
@@ -423,18 +931,19 @@ using namespace sf;
 
 extern "C" size_t sf_selective_scan_checkpoint_bytes(const sf_selective_scan_desc* d) {
   if (!valid(d)) return 0;
-  return (size_t)seq::total_slots(d->length, d->n_seq, d->packed, kChunk) * d->dim * d->state * sizeof(float);
+  return (size_t)seq::total_slots(d->length, d->n_seq, d->packed, kRows) * d->dim * d->state * sizeof(float);
 }
 
-extern "C" size_t sf_selective_scan_workspace_size(const sf_selective_scan_desc*) { return 0; }
+extern "C" size_t sf_selective_scan_workspace_size(const sf_selective_scan_desc* d) {
+  if (!valid(d) || d->n_seq == 0) return 0;
+  return (size_t)carry_floats(d, segment_rows(d, kFwdBlocks)) * sizeof(float);
+}
 
 extern "C" sf_status sf_selective_scan(const void* x, const void* dt, const float* A, const void* B, const void* C,
                                        const float* D, const void* z, const float* dt_bias,
                                        const float* initial_state, const int32_t* seq_offsets, void* y,
                                        float* final_state, void* checkpoints, const sf_selective_scan_desc* d,
                                        void* workspace, size_t workspace_bytes, void* stream) {
-  (void)workspace;
-  (void)workspace_bytes;
   if (!valid(d) || !A || (seq_offsets != nullptr) != (d->packed != 0)) return SF_ERR_INVALID_ARG;
   if (d->state > kMaxState || d->n_seq > 65535) return SF_ERR_UNSUPPORTED;
   if (d->n_seq == 0 || d->dim == 0) return SF_OK;
@@ -444,15 +953,27 @@ extern "C" sf_status sf_selective_scan(const void* x, const void* dt, const floa
   a.y = y;
   a.final_state = final_state;
   a.ck_out = static_cast<float*>(checkpoints);
-  const dim3 grid(tiles_of(d) * d->groups, d->n_seq);
+  a.vec = vectors_fit(d, {x, dt, z, y});
+  a.seg_rows = segment_rows(d, kFwdBlocks);
+  const long long carry = carry_floats(d, a.seg_rows), slots = slots_of(d, a.seg_rows);
+  if (carry && (!workspace || workspace_bytes < (size_t)carry * sizeof(float))) return SF_ERR_WORKSPACE;
+  for (const void* p : {static_cast<const void*>(A), static_cast<const void*>(initial_state),
+                        static_cast<const void*>(final_state), static_cast<const void*>(checkpoints),
+                        static_cast<const void*>(carry ? workspace : nullptr)})
+    if (!aligned16(p)) return SF_ERR_ALIGNMENT;
+  if (slots > 65535) return SF_ERR_UNSUPPORTED;
+  a.seg_state = static_cast<float*>(workspace);
+  a.seg_dt = a.seg_state + slots * d->dim * d->state;
+  const dim3 grid(tiles_of(d) * d->groups, (unsigned)slots);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  SF_SCAN_TYPES(d->dtype, SF_SCAN_LANES(d->state, (scan_fwd_kernel<T, L><<<grid, kThreads, 0, st>>>(a))))
-  return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
+  sf_status status = SF_OK;
+  SF_SCAN_TYPES(d->dtype, SF_SCAN_LANES(d->state, status = (run_fwd<T, L>(a, grid, st))))
+  return status;
 }
 
 extern "C" size_t sf_selective_scan_backward_workspace_size(const sf_selective_scan_desc* d) {
   if (!valid(d)) return 0;
-  return (size_t)bwd_layout(d, rows_of(d)).total * sizeof(float);
+  return (size_t)bwd_layout(d, segment_rows(d, kBwdBlocks)).total * sizeof(float);
 }
 
 extern "C" sf_status sf_selective_scan_backward(const void* x, const void* dt, const float* A, const void* B,
@@ -471,9 +992,14 @@ extern "C" sf_status sf_selective_scan_backward(const void* x, const void* dt, c
   if (rows > 0 && (!x || !dt || !B || !C || !checkpoints || !dy || !dx || !ddt || !dB || !dC))
     return SF_ERR_INVALID_ARG;
   if ((z && rows > 0 && !dz) || (D && !dD) || (dt_bias && !d_dt_bias)) return SF_ERR_INVALID_ARG;
-  const BwdLayout l = bwd_layout(d, rows);
+  const long long seg = segment_rows(d, kBwdBlocks), slots = slots_of(d, seg);
+  const BwdLayout l = bwd_layout(d, seg);
   if (some && (!workspace || workspace_bytes < (size_t)l.total * sizeof(float))) return SF_ERR_WORKSPACE;
   if (some && !aligned16(workspace)) return SF_ERR_ALIGNMENT;
+  for (const void* p : {static_cast<const void*>(A), checkpoints, static_cast<const void*>(d_final_state),
+                        static_cast<const void*>(d_initial_state)})
+    if (!aligned16(p)) return SF_ERR_ALIGNMENT;
+  if (slots > 65535) return SF_ERR_UNSUPPORTED;
   float* ws = static_cast<float*>(workspace);
   ScanArgs a = base_args(x, dt, A, B, C, D, z, dt_bias, seq_offsets, d);
   a.ck = static_cast<const float*>(checkpoints);
@@ -488,8 +1014,14 @@ extern "C" sf_status sf_selective_scan_backward(const void* x, const void* dt, c
     a.part_bc = ws + l.bc;
     a.part_a = ws + l.a;
     a.part_d = ws + l.d;
-    const dim3 grid(tiles_of(d) * d->groups, d->n_seq);
-    SF_SCAN_TYPES(d->dtype, SF_SCAN_LANES(d->state, (scan_bwd_kernel<T, L><<<grid, kThreads, 0, st>>>(a))))
+    a.seg_rows = seg;
+    a.seg_state = ws + l.carry;
+    a.seg_dt = a.seg_state + slots * d->dim * d->state;
+    a.vec = vectors_fit(d, {x, dt, z, dy, dx, ddt, dz});
+    const dim3 grid(tiles_of(d) * d->groups, (unsigned)slots);
+    sf_status status = SF_OK;
+    SF_SCAN_TYPES(d->dtype, SF_SCAN_LANES(d->state, status = (run_bwd<T, L>(a, grid, st))))
+    if (status != SF_OK) return status;
     if (rows > 0) {
       const int np = lanes(d->state) * kS;
       const long long n = rows * 2 * d->groups * np;
@@ -498,12 +1030,11 @@ extern "C" sf_status sf_selective_scan_backward(const void* x, const void* dt, c
                                   static_cast<T*>(dC))))
     }
   }
-  const long long na = (long long)d->dim * d->state, nd = d->dim;
-  scan_sum_kernel<<<(unsigned)((na + 255) / 256), 256, 0, st>>>(a.part_a, d->n_seq, na, dA);
-  const unsigned gd = (unsigned)((nd + 255) / 256);
-  if (dD) scan_sum_kernel<<<gd, 256, 0, st>>>(a.part_d, d->n_seq, nd, dD);
-  if (d_dt_bias)
-    scan_sum_kernel<<<gd, 256, 0, st>>>(some ? a.part_d + (long long)d->n_seq * nd : nullptr, d->n_seq, nd, d_dt_bias);
+  const long long na = (long long)d->dim * d->state, nd = d->dim, count = some ? slots : 0;
+  scan_sum_kernel<<<(unsigned)((na + 127) / 128), 128, 0, st>>>(a.part_a, count, na, dA);
+  const unsigned gd = (unsigned)((nd + 127) / 128);
+  if (dD) scan_sum_kernel<<<gd, 128, 0, st>>>(a.part_d, count, nd, dD);
+  if (d_dt_bias) scan_sum_kernel<<<gd, 128, 0, st>>>(some ? a.part_d + slots * nd : nullptr, count, nd, d_dt_bias);
   return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
 }
 
@@ -517,6 +1048,7 @@ extern "C" sf_status sf_selective_scan_update(const void* x, const void* dt, con
   if (!x || !dt || !B || !C || !y || !state_pool) return SF_ERR_INVALID_ARG;
   ScanArgs a = base_args(x, dt, A, B, C, D, z, dt_bias, nullptr, d);
   a.y = y;
+  if (!aligned16(A) || !aligned16(state_pool)) return SF_ERR_ALIGNMENT;
   const int ch = kThreads / lanes(d->state);
   const dim3 grid(d->n_seq, (d->dim + ch - 1) / ch);
   if (grid.y > 65535) return SF_ERR_UNSUPPORTED;
