@@ -50,7 +50,7 @@ struct ScanArgs {
   long long seg_rows;                // rows per segment, a multiple of kRows
   long long x_batch, x_row, dt_batch, dt_row, z_batch, z_row, b_batch, b_row, c_batch, c_row;
   int dim, state, groups, softplus;
-  int vec;                           // four channels as one word: rows and pointers are aligned for it
+  int vec, words;  // four channels, 4 bytes of a row of B and C as one access: rows and pointers are aligned for it
 };
 
 __device__ __forceinline__ float ex2(float v) {
@@ -87,11 +87,33 @@ __device__ __forceinline__ float sum2(u64 a) {
   unpack2(lo, hi, a);
   return lo + hi;
 }
+__device__ __forceinline__ float rcp(float v) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+  return r;
+}
 __device__ __forceinline__ u64 ex2x2(u64 v) {
   float lo, hi;
   unpack2(lo, hi, v);
   return pack2(ex2(lo), ex2(hi));
 }
+
+// softplus(v) = max(v, 0) + log(1 + e) with e = exp(-|v|), which is returned too. log(1 + e) = 2 atanh(s), s = e / (2 + e)
+// <= 1/3, is odd in s: s times a polynomial of degree 4 in s^2, fitted by weighted least squares to a relative error
+// of 8e-9 (of fp32 coefficients) over [0, 1/9]. Small e keep all their digits (a time step of 1e-3 is e = 1e-3), which
+// log(1 + e) from a logarithm would not. (Scalar: pairs would need a move for every coefficient.)
+__device__ __forceinline__ float softplus(float v, float& e) {
+  e = ex2(-kLog2e * fabsf(v));
+  const float s = e * rcp(2.f + e), q = s * s;
+  float c = 0.28178343176841736f;
+  c = fmaf(c, q, 0.27960601449012756f);
+  c = fmaf(c, q, 0.40024909377098083f);
+  c = fmaf(c, q, 0.6666631698608398f);
+  c = fmaf(c, q, 2.f);
+  return fmaf(s, c, fmaxf(v, 0.f));
+}
+// 1 / (1 + exp(-v))
+__device__ __forceinline__ float logistic(float v) { return rcp(1.f + ex2(-kLog2e * v)); }
 
 template <typename T>
 __device__ __forceinline__ const T* at(const void* p, const ScanArgs& a, const Span& s, long long batch,
@@ -228,40 +250,155 @@ struct Place {
   }
 };
 
-// A tile's elements on their way to shared memory: x, dt, z and dy of four channels and one row, some of B and C.
-template <typename T, int LPC, bool X, bool Z, bool GY, bool BB, bool CC>
+__device__ __forceinline__ void cp_async(void* dst, const void* src, int bytes, bool in) {
+  const uint32_t d = smem_u32(dst);
+  const int n = in ? bytes : 0;  // bytes past n are filled with 0
+  if (bytes == 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
+  if (bytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
+  if (bytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+// Tiles' elements on their way: x, dt, z and dy of four channels and one row, and words of B and C, copied
+// asynchronously to a ring of STAGES tiles in shared memory. A thread copies what it will convert itself, so no barrier
+// guards the ring, and it has the same channels in every tile. (In registers the tile ahead was spilled, which waits
+// for the loads; one tile ahead is also less than the latency of memory.) Rows of 16-bit data that no word fits are
+// loaded and stored by the thread, which waits for them.
+template <typename T, int LPC, bool X, bool Z, bool GY, bool BB, bool CC, int STAGES>
+struct Ring {
+  using F = Cfg<LPC>;
+  static constexpr int ARRAYS = X + 1 + Z + GY;
+  static constexpr int EPW = 4 / (int)sizeof(T);  // elements per word of B and C
+  static constexpr int WORDS = kRows * F::NP / EPW, WPT = (WORDS + F::THREADS - 1) / F::THREADS;
+  seq::Vec<T, 4> v[STAGES][ARRAYS][F::UPT][F::THREADS];
+  seq::Vec<T, EPW> bc[STAGES][BB + CC][WPT][F::THREADS];
+  float bias[F::CH], D[F::CH];
+};
+
+template <typename T, int LPC, bool X, bool Z, bool GY, bool BB, bool CC, int STAGES>
 struct Fetch {
   using F = Cfg<LPC>;
-  seq::Vec<T, 4> x[F::UPT], dt[F::UPT], z[F::UPT], gy[F::UPT];
-  T b[F::BPT], c[F::BPT];
-  __device__ __forceinline__ void load(const ScanArgs& a, const Place<LPC>& k, const T* xs, const T* dts,
-                                       const T* zs, const T* gys, const T* Bs, const T* Cs, long long t0, int rows) {
-#pragma unroll
-    for (int i = 0; i < F::UPT; ++i) {
-      const int u = threadIdx.x + i * F::THREADS, r = u / (F::CH / 4), m = u % (F::CH / 4) * 4;
-      const int valid = (F::UNITS % F::THREADS == 0 || u < F::UNITS) && r < rows ? k.ch - m : 0;
-      const long long t = t0 + r;
-      if (X) load_unit(x[i], xs + t * a.x_row + m, valid, a.vec);
-      load_unit(dt[i], dts + t * a.dt_row + m, valid, a.vec);
-      if (Z && zs) load_unit(z[i], zs + t * a.z_row + m, valid, a.vec);
-      if (GY) load_unit(gy[i], gys + t * a.dim + m, valid, a.vec);
-    }
-#pragma unroll
-    for (int i = 0; i < F::BPT; ++i) {
-      const int u = threadIdx.x + i * F::THREADS, r = u / F::NP, m = u % F::NP;
-      const bool in = r < rows && m < a.state;
-      if (BB) b[i] = in ? Bs[(t0 + r) * a.b_row + m] : DT<T>::from_f(0.f);
-      if (CC) c[i] = in ? Cs[(t0 + r) * a.c_row + m] : DT<T>::from_f(0.f);
+  using R = Ring<T, LPC, X, Z, GY, BB, CC, STAGES>;
+  static constexpr int RSTEP = F::THREADS / (F::CH / 4);  // rows between a thread's units
+  static constexpr int WROW = F::NP / R::EPW;             // words per row of B
+  static constexpr int AX = 0, AT = X, AZ = X + 1, AG = X + 1 + Z;
+  R& ring;
+  const T *px, *pdt, *pz, *pgy, *pb, *pc;
+  int r, m, valid;
+  int put, get;  // stages
+
+  // The first tile's rows start at t0 (of the sequence). Ends with the block's bias and D in shared memory, for the
+  // barrier that follows.
+  __device__ __forceinline__ Fetch(R& ring_, const ScanArgs& a, const Place<LPC>& k, const Span& p, long long t0)
+      : ring(ring_) {
+    r = threadIdx.x / (F::CH / 4);
+    m = threadIdx.x % (F::CH / 4) * 4;
+    valid = F::THREADS <= F::UNITS || threadIdx.x < F::UNITS ? max(0, min(4, k.ch - m)) : 0;
+    put = get = 0;
+    const long long t = t0 + r;
+    const int wr = threadIdx.x / WROW, wm = threadIdx.x % WROW * R::EPW;
+    if (X) px = at<T>(a.x, a, p, a.x_batch, a.x_row) + k.d0 + t * a.x_row + m;
+    pdt = at<T>(a.dt, a, p, a.dt_batch, a.dt_row) + k.d0 + t * a.dt_row + m;
+    if (Z) pz = a.z ? at<T>(a.z, a, p, a.z_batch, a.z_row) + k.d0 + t * a.z_row + m : nullptr;
+    if (GY) pgy = static_cast<const T*>(a.dy) + (row0(a, p) + t) * a.dim + k.d0 + m;
+    if (BB) pb = at<T>(a.B, a, p, a.b_batch, a.b_row) + (long long)k.g * a.state + (t0 + wr) * a.b_row + wm;
+    if (CC) pc = at<T>(a.C, a, p, a.c_batch, a.c_row) + (long long)k.g * a.state + (t0 + wr) * a.c_row + wm;
+    for (int i = threadIdx.x; i < F::CH; i += F::THREADS) {
+      ring.bias[i] = a.dt_bias && i < k.ch ? a.dt_bias[k.d0 + i] : 0.f;
+      ring.D[i] = a.D && i < k.ch ? a.D[k.d0 + i] : 0.f;
     }
   }
-  // dt of element j of unit i as the recurrence uses it (0 where there is no element), and its argument before softplus
-  __device__ __forceinline__ float step(const ScanArgs& a, const Place<LPC>& k, int i, int j, int rows,
-                                        float& raw) const {
-    const int u = threadIdx.x + i * F::THREADS, r = u / (F::CH / 4), m = u % (F::CH / 4) * 4 + j;
-    raw = DT<T>::to_f(dt[i].v[j]);
-    if (r >= rows || m >= k.ch) return 0.f;
-    if (a.dt_bias) raw += __ldg(a.dt_bias + k.d0 + m);
-    return a.softplus ? seq::softplus(raw) : raw;
+  __device__ __forceinline__ void unit_in(seq::Vec<T, 4>& dst, const T* src, int ok, int vec) {
+    if (vec) {
+      cp_async(&dst, src, 4 * sizeof(T), ok > 0);
+    } else if (sizeof(T) == 4) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) cp_async(&dst.v[i], src + (i < ok ? i : 0), 4, i < ok);
+    } else {
+      load_unit(dst, src, ok, 0);
+    }
+  }
+  __device__ __forceinline__ void word_in(seq::Vec<T, R::EPW>& dst, const T* src, int ok, int words) {
+    if (sizeof(T) == 4 || words) {
+      cp_async(&dst, src, 4, ok > 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < R::EPW; ++i) dst.v[i] = i < ok ? src[i] : DT<T>::from_f(0.f);
+    }
+  }
+  // Starts a tile of `rows` rows at the pointers, which then move on by `next` rows. Rows below 1: nothing to copy.
+  __device__ __forceinline__ void load(const ScanArgs& a, int rows, int next) {
+    if (rows > 0) {
+#pragma unroll
+      for (int i = 0; i < F::UPT; ++i) {
+        const int rr = i * RSTEP, ok = r + rr < rows ? valid : 0;
+        if (X) unit_in(ring.v[put][AX][i][threadIdx.x], px + (ok ? rr * a.x_row : 0), ok, a.vec);
+        unit_in(ring.v[put][AT][i][threadIdx.x], pdt + (ok ? rr * a.dt_row : 0), ok, a.vec);
+        if (Z && a.z) unit_in(ring.v[put][AZ][i][threadIdx.x], pz + (ok ? rr * a.z_row : 0), ok, a.vec);
+        if (GY) unit_in(ring.v[put][AG][i][threadIdx.x], pgy + (ok ? (long long)rr * a.dim : 0), ok, a.vec);
+      }
+      const int wr = threadIdx.x / WROW, wm = threadIdx.x % WROW * R::EPW;
+#pragma unroll
+      for (int i = 0; i < R::WPT; ++i) {
+        const int rr = i * (F::THREADS / WROW), ok = wr + rr < rows ? a.state - wm : 0;
+        if (R::WORDS % F::THREADS == 0 || threadIdx.x + i * F::THREADS < R::WORDS) {
+          if (BB) word_in(ring.bc[put][0][i][threadIdx.x], pb + (ok > 0 ? rr * a.b_row : 0), ok, a.words);
+          if (CC) word_in(ring.bc[put][BB][i][threadIdx.x], pc + (ok > 0 ? rr * a.c_row : 0), ok, a.words);
+        }
+      }
+      if (X) px += next * a.x_row;
+      pdt += next * a.dt_row;
+      if (Z && a.z) pz += next * a.z_row;
+      if (GY) pgy += (long long)next * a.dim;
+      if (BB) pb += next * a.b_row;
+      if (CC) pc += next * a.c_row;
+    }
+    cp_async_commit();
+    put = put + 1 == STAGES ? 0 : put + 1;
+  }
+  // Waits for the oldest tile of STAGES - 1 in flight.
+  __device__ __forceinline__ void wait() { cp_async_wait<STAGES - 2>(); }
+  __device__ __forceinline__ void done() { get = get + 1 == STAGES ? 0 : get + 1; }
+  __device__ __forceinline__ seq::Vec<T, 4> unit(int array, int i) const { return ring.v[get][array][i][threadIdx.x]; }
+  __device__ __forceinline__ bool has_unit(int i) const {
+    return F::UNITS % F::THREADS == 0 || threadIdx.x + i * F::THREADS < F::UNITS;
+  }
+  // B and C as floats, in [kRows][NP] arrays.
+  __device__ __forceinline__ void convert_bc(float (*B)[F::NP], float (*C)[F::NP]) const {
+    const int wr = threadIdx.x / WROW, wm = threadIdx.x % WROW * R::EPW;
+#pragma unroll
+    for (int i = 0; i < R::WPT; ++i)
+      if (R::WORDS % F::THREADS == 0 || threadIdx.x + i * F::THREADS < R::WORDS) {
+        const int rr = wr + i * (F::THREADS / WROW);
+        float f[R::EPW];
+        if (BB) {
+          seq::load_vec<T, R::EPW>(f, ring.bc[get][0][i][threadIdx.x].v);
+          *reinterpret_cast<seq::Vec<float, R::EPW>*>(&B[rr][wm]) = *reinterpret_cast<seq::Vec<float, R::EPW>*>(f);
+        }
+        if (CC) {
+          seq::load_vec<T, R::EPW>(f, ring.bc[get][BB][i][threadIdx.x].v);
+          *reinterpret_cast<seq::Vec<float, R::EPW>*>(&C[rr][wm]) = *reinterpret_cast<seq::Vec<float, R::EPW>*>(f);
+        }
+      }
+  }
+  // dt of element j of unit i as the recurrence uses it, 0 where there is no element (rows past the tile's, channels
+  // past the block's); SLOPE: and its derivative by dt_raw.
+  template <bool SLOPE>
+  __device__ __forceinline__ float step(const ScanArgs& a, float raw, int i, int j, int rows, float& slope) const {
+    float v = raw + ring.bias[m + j];
+    slope = 1.f;
+    if (a.softplus) {
+      float e;
+      const float u = v;
+      v = softplus(u, e);
+      if (SLOPE) slope = (u >= 0.f ? 1.f : e) * rcp(1.f + e);  // the logistic function of u
+    }
+    return r + i * RSTEP < rows && j < valid ? v : 0.f;
   }
 };
 
@@ -291,66 +428,68 @@ __device__ __forceinline__ void load_decay(u64 (&A2)[2], const ScanArgs& a, cons
 // What a segment adds to a state of 0, forwards (h = a h + dt x B) or backwards (gh = a (gh + gp C)), and its sum of
 // dt. The last segment's (backwards: the first's) is not needed.
 template <typename T, int LPC, bool REV>
-__global__ void __launch_bounds__(Cfg<LPC>::THREADS) scan_carry_kernel(ScanArgs a) {
+struct CarrySmem {
   using F = Cfg<LPC>;
-  __shared__ __align__(16) float4 sdu[kRows][F::CH];
-  __shared__ __align__(16) float sB[kRows][F::NP];
+  static constexpr int STAGES = sizeof(T) == 2 ? 4 : 3;
+  float4 du[kRows][F::CH];  // dt, dt, dt x, dt x (backwards gp)
+  float B[kRows][F::NP];
+  Ring<T, LPC, !REV, REV, REV, !REV, REV, STAGES> ring;
+};
+template <typename T, int LPC, bool REV>
+__global__ void __launch_bounds__(Cfg<LPC>::THREADS, 3) scan_carry_kernel(ScanArgs a) {
+  using F = Cfg<LPC>;
+  using S = CarrySmem<T, LPC, REV>;
+  extern __shared__ __align__(16) char smem[];
+  S& sm = *reinterpret_cast<S*>(smem);
   const Place<LPC> k(a);
   const Span p = seq::slot_span(a.rows, blockIdx.y, a.seg_rows);
   if (p.len < 0) return;
   const int seg = (int)(blockIdx.y - p.slot0);
   if (REV ? seg == 0 : seg == p.n_slots - 1) return;
-  const T* xs = at<T>(a.x, a, p, a.x_batch, a.x_row) + k.d0;
-  const T* dts = at<T>(a.dt, a, p, a.dt_batch, a.dt_row) + k.d0;
-  const T* zs = a.z ? at<T>(a.z, a, p, a.z_batch, a.z_row) + k.d0 : nullptr;
-  const T* gys = REV ? static_cast<const T*>(a.dy) + row0(a, p) * a.dim + k.d0 : nullptr;
-  const T* Bs = at<T>(a.B, a, p, a.b_batch, a.b_row) + (long long)k.g * a.state;
-  const T* Cs = at<T>(a.C, a, p, a.c_batch, a.c_row) + (long long)k.g * a.state;
+  const long long r1 = min(p.r0 + a.seg_rows, p.len);
+  const int tiles = (int)((r1 - p.r0 + kRows - 1) / kRows);
+  Fetch<T, LPC, !REV, REV, REV, !REV, REV, S::STAGES> f(sm.ring, a, k, p, p.r0 + (REV ? (tiles - 1ll) * kRows : 0));
+  auto tile_rows = [&](int i) {
+    return i < tiles ? (int)min((long long)kRows, r1 - p.r0 - (long long)(REV ? tiles - 1 - i : i) * kRows) : 0;
+  };
+  for (int i = 0; i < S::STAGES - 1; ++i) f.load(a, tile_rows(i), REV ? -kRows : kRows);
   u64 A2[2], h[2] = {0, 0};
   load_decay(A2, a, k);
   float sum = 0.f;
-  const long long r1 = min(p.r0 + a.seg_rows, p.len);
-  const int tiles = (int)((r1 - p.r0 + kRows - 1) / kRows);
-  Fetch<T, LPC, !REV, REV, REV, !REV, REV> f;
-  auto fetch = [&](int i) {
-    const long long t0 = p.r0 + (long long)(REV ? tiles - 1 - i : i) * kRows;
-    f.load(a, k, xs, dts, zs, gys, Bs, Cs, t0, (int)min((long long)kRows, r1 - t0));
-  };
-  fetch(0);
   for (int i = 0; i < tiles; ++i) {
-    const long long t0 = p.r0 + (long long)(REV ? tiles - 1 - i : i) * kRows;
-    const int rows = (int)min((long long)kRows, r1 - t0);
+    const int rows = tile_rows(i);
+    f.wait();
     __syncthreads();
 #pragma unroll
-    for (int v = 0; v < F::UPT; ++v) {
-      const int u = threadIdx.x + v * F::THREADS, r = u / (F::CH / 4), m = u % (F::CH / 4) * 4;
-      if (F::UNITS % F::THREADS == 0 || u < F::UNITS)
+    for (int v = 0; v < F::UPT; ++v)
+      if (f.has_unit(v)) {
+        const auto tdt = f.unit(f.AT, v), tx = f.unit(REV ? f.AG : f.AX, v);
+        seq::Vec<T, 4> tz;
+        if (REV && a.z) tz = f.unit(f.AZ, v);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float raw, w;
-          const float dt = f.step(a, k, v, j, rows, raw);
-          if (REV) {
-            w = DT<T>::to_f(f.gy[v].v[j]);
-            if (zs) w *= seq::silu(DT<T>::to_f(f.z[v].v[j]));
-          } else {
-            w = dt * DT<T>::to_f(f.x[v].v[j]);
+          float slope;
+          const float dt = f.template step<false>(a, DT<T>::to_f(tdt.v[j]), v, j, rows, slope);
+          float w = DT<T>::to_f(tx.v[j]);
+          if (!REV) {
+            w *= dt;
+          } else if (a.z) {
+            const float z = DT<T>::to_f(tz.v[j]);
+            w *= z * logistic(z);
           }
-          sdu[r][entry(m + j)] = make_float4(dt, dt, w, w);
+          sm.du[f.r + v * f.RSTEP][entry(f.m + j)] = make_float4(dt, dt, w, w);
         }
-    }
-#pragma unroll
-    for (int v = 0; v < F::BPT; ++v) {
-      const int u = threadIdx.x + v * F::THREADS;
-      sB[u / F::NP][u % F::NP] = DT<T>::to_f(REV ? f.c[v] : f.b[v]);
-    }
-    if (i + 1 < tiles) fetch(i + 1);
+      }
+    f.convert_bc(sm.B, sm.B);
+    f.done();
+    f.load(a, tile_rows(i + S::STAGES - 1), REV ? -kRows : kRows);
     __syncthreads();
     const int e = entry(k.c);
 #pragma unroll
     for (int rr = 0; rr < kRows; ++rr) {
       const int r = REV ? kRows - 1 - rr : rr;
-      const ulonglong2 du = *reinterpret_cast<const ulonglong2*>(&sdu[r][e]);
-      const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&sB[r][k.n]);
+      const ulonglong2 du = *reinterpret_cast<const ulonglong2*>(&sm.du[r][e]);
+      const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&sm.B[r][k.n]);
       const u64 a0 = ex2x2(mul2(du.x, A2[0])), a1 = ex2x2(mul2(du.x, A2[1]));
       if (REV) {
         h[0] = mul2(a0, fma2(du.y, b.x, h[0]));
@@ -371,10 +510,12 @@ __global__ void __launch_bounds__(Cfg<LPC>::THREADS) scan_carry_kernel(ScanArgs 
 template <typename T, int LPC>
 struct FwdSmem {
   using F = Cfg<LPC>;
+  static constexpr int STAGES = sizeof(T) == 2 ? 4 : 3;
   float4 du[kRows][F::CH];  // dt, dt, dt x, dt x
   float2 gx[kRows][F::PAD]; // D x, gate
   float B[kRows][F::NP], C[kRows][F::NP];
   T out[kRows][F::PAD];
+  Ring<T, LPC, true, true, false, true, true, STAGES> ring;
 };
 
 // One block: one segment of a sequence and CH channels of one group.
@@ -387,63 +528,71 @@ __global__ void __launch_bounds__(Cfg<LPC>::THREADS, 3) scan_fwd_kernel(ScanArgs
   const Span p = seq::slot_span(a.rows, blockIdx.y, a.seg_rows);
   if (p.len < 0) return;
   const int seg = (int)(blockIdx.y - p.slot0);
-  const T* xs = at<T>(a.x, a, p, a.x_batch, a.x_row) + k.d0;
-  const T* dts = at<T>(a.dt, a, p, a.dt_batch, a.dt_row) + k.d0;
-  const T* zs = a.z ? at<T>(a.z, a, p, a.z_batch, a.z_row) + k.d0 : nullptr;
-  const T* Bs = at<T>(a.B, a, p, a.b_batch, a.b_row) + (long long)k.g * a.state;
-  const T* Cs = at<T>(a.C, a, p, a.c_batch, a.c_row) + (long long)k.g * a.state;
-  T* ys = static_cast<T*>(a.y) + row0(a, p) * a.dim + k.d0;
   const long long r1 = min(p.r0 + a.seg_rows, p.len);
   const int tiles = (int)((r1 - p.r0 + kRows - 1) / kRows);
-  Fetch<T, LPC, true, true, false, true, true> f;
-  auto tile_rows = [&](int i) { return (int)min((long long)kRows, r1 - (p.r0 + (long long)i * kRows)); };
-  auto fetch = [&](int i) {
-    f.load(a, k, xs, dts, zs, nullptr, Bs, Cs, p.r0 + (long long)i * kRows, tile_rows(i));
+  constexpr int STAGES = FwdSmem<T, LPC>::STAGES;
+  Fetch<T, LPC, true, true, false, true, true, STAGES> f(s.ring, a, k, p, p.r0);
+  T* py = static_cast<T*>(a.y) + (row0(a, p) + p.r0 + f.r) * a.dim + k.d0 + f.m;
+  auto tile_rows = [&](int i) {
+    return i < tiles ? (int)min((long long)kRows, r1 - (p.r0 + (long long)i * kRows)) : 0;
   };
-  auto put = [&](int i) {  // tile i's results, each row's channels together
-    const int rows = tile_rows(i);
+  auto put = [&](int rows) {  // a tile's results, four channels of a row together
 #pragma unroll
     for (int v = 0; v < F::UPT; ++v) {
-      const int u = threadIdx.x + v * F::THREADS, r = u / (F::CH / 4), m = u % (F::CH / 4) * 4;
-      if ((F::UNITS % F::THREADS == 0 || u < F::UNITS) && r < rows)
-        store_unit(ys + (p.r0 + (long long)i * kRows + r) * a.dim + m,
-                   *reinterpret_cast<const seq::Vec<T, 4>*>(&s.out[r][m]), k.ch - m, a.vec);
+      const int r = f.r + v * f.RSTEP;
+      if (f.has_unit(v) && r < rows)
+        store_unit(py + (long long)v * f.RSTEP * a.dim, *reinterpret_cast<const seq::Vec<T, 4>*>(&s.out[r][f.m]),
+                   f.valid, a.vec);
     }
+    py += (long long)kRows * a.dim;
   };
-  if (tiles > 0) fetch(0);
+  for (int i = 0; i < STAGES - 1; ++i) f.load(a, tile_rows(i), kRows);
   u64 A2[2], h[2] = {0, 0};
   load_decay(A2, a, k);
   if (k.own) {
     if (a.init) load4(h, a.init + ((long long)p.s * a.dim + k.d) * a.state, k.n, a.state);
     if (seg > 0) segment_start<false>(h, a, p, A2, seg, k.d, k.n);
   }
-  const long long ck0 = a.ck_out ? seq::seq_slot0(a.rows, p.s, kRows) + p.r0 / kRows : 0;
+  float* ck = nullptr;
+  if (a.ck_out && k.own)
+    ck = a.ck_out + ((seq::seq_slot0(a.rows, p.s, kRows) + p.r0 / kRows) * a.dim + k.d) * a.state;
   const int e = entry(k.c);
   for (int i = 0; i < tiles; ++i) {
     const int rows = tile_rows(i);
-    if (a.ck_out && k.own) store4(a.ck_out + ((ck0 + i) * a.dim + k.d) * a.state, h, k.n, a.state);
+    if (ck) {
+      store4(ck, h, k.n, a.state);
+      ck += (long long)a.dim * a.state;
+    }
+    f.wait();
     __syncthreads();
-    if (i > 0) put(i - 1);
+    if (i > 0) put(kRows);
 #pragma unroll
-    for (int v = 0; v < F::UPT; ++v) {
-      const int u = threadIdx.x + v * F::THREADS, r = u / (F::CH / 4), m = u % (F::CH / 4) * 4;
-      if (F::UNITS % F::THREADS == 0 || u < F::UNITS)
+    for (int v = 0; v < F::UPT; ++v)
+      if (f.has_unit(v)) {
+        const auto tdt = f.unit(f.AT, v), tx = f.unit(f.AX, v);
+        seq::Vec<T, 4> tz;
+        if (a.z) tz = f.unit(f.AZ, v);
+        const int r = f.r + v * f.RSTEP;
+        float px[4], g[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float raw;
-          const float dt = f.step(a, k, v, j, rows, raw), x = DT<T>::to_f(f.x[v].v[j]), w = dt * x;
-          const float D = a.D && m + j < k.ch ? __ldg(a.D + k.d0 + m + j) : 0.f;
-          s.du[r][entry(m + j)] = make_float4(dt, dt, w, w);
-          s.gx[r][m + j] = make_float2(D * x, zs ? seq::silu(DT<T>::to_f(f.z[v].v[j])) : 1.f);
+          float slope;
+          const float dt = f.template step<false>(a, DT<T>::to_f(tdt.v[j]), v, j, rows, slope);
+          const float x = DT<T>::to_f(tx.v[j]), w = dt * x;
+          px[j] = s.ring.D[f.m + j] * x;
+          g[j] = 1.f;
+          if (a.z) {
+            g[j] = DT<T>::to_f(tz.v[j]);
+            g[j] *= logistic(g[j]);
+          }
+          s.du[r][entry(f.m + j)] = make_float4(dt, dt, w, w);
         }
-    }
-#pragma unroll
-    for (int v = 0; v < F::BPT; ++v) {
-      const int u = threadIdx.x + v * F::THREADS;
-      s.B[u / F::NP][u % F::NP] = DT<T>::to_f(f.b[v]);
-      s.C[u / F::NP][u % F::NP] = DT<T>::to_f(f.c[v]);
-    }
-    if (i + 1 < tiles) fetch(i + 1);
+        *reinterpret_cast<float4*>(&s.gx[r][f.m]) = make_float4(px[0], g[0], px[1], g[1]);
+        *reinterpret_cast<float4*>(&s.gx[r][f.m + 2]) = make_float4(px[2], g[2], px[3], g[3]);
+      }
+    f.convert_bc(s.B, s.C);
+    f.done();
+    f.load(a, tile_rows(i + STAGES - 1), kRows);
     __syncthreads();
 #pragma unroll
     for (int r0 = 0; r0 < kRows; r0 += 4) {
@@ -470,7 +619,7 @@ __global__ void __launch_bounds__(Cfg<LPC>::THREADS, 3) scan_fwd_kernel(ScanArgs
   }
   if (tiles > 0) {
     __syncthreads();
-    put(tiles - 1);
+    put(tile_rows(tiles - 1));
   }
   if (a.final_state && k.own && seg == p.n_slots - 1)
     store4(a.final_state + ((long long)p.s * a.dim + k.d) * a.state, h, k.n, a.state);
@@ -479,6 +628,7 @@ __global__ void __launch_bounds__(Cfg<LPC>::THREADS, 3) scan_fwd_kernel(ScanArgs
 template <typename T, int LPC>
 struct BwdSmem {
   using F = Cfg<LPC>;
+  static constexpr int STAGES = sizeof(T) == 2 ? 3 : 2;
   float4 du[kRows][F::CH];   // dt, dt, dt x, dt x
   float4 gp[kRows][F::CH];   // gp, gp, D gp, x
   float2 sg[kRows][F::PAD];  // softplus'(raw), dy silu'(z)
@@ -486,6 +636,7 @@ struct BwdSmem {
   float B[kRows][F::NP], C[kRows][F::NP];
   float bc[2][F::WARPS][kHalf][2 * F::NP];  // sums over a warp's channels, one half tile after the other
   T dx[kRows][F::PAD], ddt[kRows][F::PAD], dz[kRows][F::PAD];
+  Ring<T, LPC, true, true, true, true, true, STAGES> ring;
 };
 
 // Sums of 8 values over the channels of a warp: scattered over the lanes as far as they go. Returns how many values
@@ -544,37 +695,34 @@ __global__ void __launch_bounds__(Cfg<LPC>::THREADS, 2) scan_bwd_kernel(ScanArgs
     return;
   }
   const int seg = (int)(blockIdx.y - p.slot0), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const T* xs = at<T>(a.x, a, p, a.x_batch, a.x_row) + k.d0;
-  const T* dts = at<T>(a.dt, a, p, a.dt_batch, a.dt_row) + k.d0;
-  const T* zs = a.z ? at<T>(a.z, a, p, a.z_batch, a.z_row) + k.d0 : nullptr;
-  const T* Bs = at<T>(a.B, a, p, a.b_batch, a.b_row) + (long long)k.g * a.state;
-  const T* Cs = at<T>(a.C, a, p, a.c_batch, a.c_row) + (long long)k.g * a.state;
   const long long r00 = row0(a, p);
-  const T* gys = static_cast<const T*>(a.dy) + r00 * a.dim + k.d0;
   const long long total_rows = a.rows.offsets ? a.rows.length : a.rows.length * a.rows.n_seq;
-  float* bc_out = a.part_bc + ((k.tile * total_rows + r00) * a.groups + k.g) * 2 * F::NP;
   const long long r1 = min(p.r0 + a.seg_rows, p.len);
   const int tiles = (int)((r1 - p.r0 + kRows - 1) / kRows);
-  const long long ck0 = seq::seq_slot0(a.rows, p.s, kRows) + p.r0 / kRows;
+  const long long last = p.r0 + (tiles - 1ll) * kRows;  // first row of the last tile
+  float* bc_out = a.part_bc + ((k.tile * total_rows + r00 + last) * a.groups + k.g) * 2 * F::NP;
+  const float* ck = a.ck + ((seq::seq_slot0(a.rows, p.s, kRows) + last / kRows) * a.dim + k.d) * a.state;
 
-  Fetch<T, LPC, true, true, true, true, true> f;
-  auto tile_row0 = [&](int i) { return p.r0 + (long long)i * kRows; };
-  auto tile_rows = [&](int i) { return (int)min((long long)kRows, r1 - tile_row0(i)); };
-  auto put = [&](int i) {
-    const int rows = tile_rows(i);
+  constexpr int STAGES = BwdSmem<T, LPC>::STAGES;
+  Fetch<T, LPC, true, true, true, true, true, STAGES> f(s.ring, a, k, p, last);
+  long long po = (r00 + last + f.r) * a.dim + k.d0 + f.m;  // where a tile's results go
+  auto put = [&](int rows) {
 #pragma unroll
     for (int v = 0; v < F::UPT; ++v) {
-      const int u = threadIdx.x + v * F::THREADS, r = u / (F::CH / 4), m = u % (F::CH / 4) * 4;
-      if ((F::UNITS % F::THREADS == 0 || u < F::UNITS) && r < rows) {
-        const long long o = (r00 + tile_row0(i) + r) * a.dim + k.d0 + m;
+      const int r = f.r + v * f.RSTEP;
+      if (f.has_unit(v) && r < rows) {
+        const long long o = po + (long long)v * f.RSTEP * a.dim;
         using V4 = seq::Vec<T, 4>;
-        store_unit(static_cast<T*>(a.dx) + o, *reinterpret_cast<const V4*>(&s.dx[r][m]), k.ch - m, a.vec);
-        store_unit(static_cast<T*>(a.ddt) + o, *reinterpret_cast<const V4*>(&s.ddt[r][m]), k.ch - m, a.vec);
-        if (a.dz) store_unit(static_cast<T*>(a.dz) + o, *reinterpret_cast<const V4*>(&s.dz[r][m]), k.ch - m, a.vec);
+        store_unit(static_cast<T*>(a.dx) + o, *reinterpret_cast<const V4*>(&s.dx[r][f.m]), f.valid, a.vec);
+        store_unit(static_cast<T*>(a.ddt) + o, *reinterpret_cast<const V4*>(&s.ddt[r][f.m]), f.valid, a.vec);
+        if (a.dz) store_unit(static_cast<T*>(a.dz) + o, *reinterpret_cast<const V4*>(&s.dz[r][f.m]), f.valid, a.vec);
       }
     }
+    po -= (long long)kRows * a.dim;
   };
-  if (tiles > 0) f.load(a, k, xs, dts, zs, gys, Bs, Cs, tile_row0(tiles - 1), tile_rows(tiles - 1));
+  const int last_rows = (int)(r1 - last);
+  auto tile_rows = [&](int i) { return i < 0 ? 0 : i == tiles - 1 ? last_rows : kRows; };
+  for (int i = 0; i < STAGES - 1; ++i) f.load(a, tile_rows(tiles - 1 - i), -kRows);
   u64 A2[2], gh[2] = {0, 0}, gA[2] = {0, 0};
   load_decay(A2, a, k);
   if (k.own) {
@@ -586,39 +734,42 @@ __global__ void __launch_bounds__(Cfg<LPC>::THREADS, 2) scan_bwd_kernel(ScanArgs
   int buf = 0;
   for (int i = tiles - 1; i >= 0; --i) {
     const int rows = tile_rows(i);
-    u64 h0[2] = {0, 0};
-    if (k.own) load4(h0, a.ck + ((ck0 + i) * a.dim + k.d) * a.state, k.n, a.state);
+    u64 h0[2] = {0, 0};  // the states before the tile
+    if (k.own) load4(h0, ck, k.n, a.state);
+    ck -= (long long)a.dim * a.state;
+    f.wait();
     __syncthreads();
-    if (i + 1 < tiles) put(i + 1);
+    if (i + 1 < tiles) put(tile_rows(i + 1));
 #pragma unroll
-    for (int v = 0; v < F::UPT; ++v) {
-      const int u = threadIdx.x + v * F::THREADS, r = u / (F::CH / 4), m = u % (F::CH / 4) * 4;
-      if (F::UNITS % F::THREADS == 0 || u < F::UNITS)
+    for (int v = 0; v < F::UPT; ++v)
+      if (f.has_unit(v)) {
+        const auto tdt = f.unit(f.AT, v), tx = f.unit(f.AX, v), tg = f.unit(f.AG, v);
+        seq::Vec<T, 4> tz;
+        if (a.z) tz = f.unit(f.AZ, v);
+        const int r = f.r + v * f.RSTEP;
+        float slope[4], gz[4], px[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          float raw;
-          const float dt = f.step(a, k, v, j, rows, raw), x = DT<T>::to_f(f.x[v].v[j]), w = dt * x;
-          const float D = a.D && m + j < k.ch ? __ldg(a.D + k.d0 + m + j) : 0.f;
-          const float gy = DT<T>::to_f(f.gy[v].v[j]);
-          float gp = gy, gz = 0.f;
-          if (zs) {
-            const float z = DT<T>::to_f(f.z[v].v[j]);
-            gp *= seq::silu(z);
-            gz = gy * seq::dsilu(z);
+          const float dt = f.template step<true>(a, DT<T>::to_f(tdt.v[j]), v, j, rows, slope[j]);
+          const float x = DT<T>::to_f(tx.v[j]), w = dt * x, D = s.ring.D[f.m + j];
+          float g = DT<T>::to_f(tg.v[j]);
+          gz[j] = 0.f;
+          if (a.z) {
+            const float z = DT<T>::to_f(tz.v[j]), sig = logistic(z);
+            gz[j] = g * (sig * fmaf(z, 1.f - sig, 1.f));
+            g *= z * sig;
           }
-          s.du[r][entry(m + j)] = make_float4(dt, dt, w, w);
-          s.gp[r][entry(m + j)] = make_float4(gp, gp, D * gp, x);
-          s.sg[r][m + j] = make_float2(a.softplus ? seq::sigmoid(raw) : 1.f, gz);
-          s.px[r][m + j] = D * x;
+          px[j] = D * x;
+          s.du[r][entry(f.m + j)] = make_float4(dt, dt, w, w);
+          s.gp[r][entry(f.m + j)] = make_float4(g, g, D * g, x);
         }
-    }
-#pragma unroll
-    for (int v = 0; v < F::BPT; ++v) {
-      const int u = threadIdx.x + v * F::THREADS;
-      s.B[u / F::NP][u % F::NP] = DT<T>::to_f(f.b[v]);
-      s.C[u / F::NP][u % F::NP] = DT<T>::to_f(f.c[v]);
-    }
-    if (i > 0) f.load(a, k, xs, dts, zs, gys, Bs, Cs, tile_row0(i - 1), kRows);
+        *reinterpret_cast<float4*>(&s.sg[r][f.m]) = make_float4(slope[0], gz[0], slope[1], gz[1]);
+        *reinterpret_cast<float4*>(&s.sg[r][f.m + 2]) = make_float4(slope[2], gz[2], slope[3], gz[3]);
+        *reinterpret_cast<float4*>(&s.px[r][f.m]) = make_float4(px[0], px[1], px[2], px[3]);
+      }
+    f.convert_bc(s.B, s.C);
+    f.done();
+    f.load(a, tile_rows(i - (STAGES - 1)), -kRows);
     __syncthreads();
     u64 h8[2] = {h0[0], h0[1]};
     if (rows > kHalf) {
@@ -703,16 +854,17 @@ __global__ void __launch_bounds__(Cfg<LPC>::THREADS, 2) scan_bwd_kernel(ScanArgs
         float v = 0.f;
 #pragma unroll
         for (int w = 0; w < F::WARPS; ++w) v += s.bc[buf][w][r][m];
-        if (t + r < rows) bc_out[(tile_row0(i) + t + r) * a.groups * 2 * F::NP + m] = v;
+        if (t + r < rows) bc_out[(long long)(t + r) * a.groups * 2 * F::NP + m] = v;
       }
       buf ^= 1;
     }
     gA[0] = add2(gA[0], tA[0]);
     gA[1] = add2(gA[1], tA[1]);
+    bc_out -= (long long)kRows * a.groups * 2 * F::NP;
   }
   if (tiles > 0) {
     __syncthreads();
-    put(0);
+    put(tile_rows(0));
   }
   gD = lanes_sum<(LPC < 4 ? LPC : 4)>(gD);
   gbias = lanes_sum<(LPC < 4 ? LPC : 4)>(gbias);
@@ -884,6 +1036,15 @@ bool vectors_fit(const sf_selective_scan_desc* d, std::initializer_list<const vo
   return true;
 }
 
+// Whether 4 bytes of a row of B and C can be read as one word.
+bool words_fit(const sf_selective_scan_desc* d, std::initializer_list<const void*> ptrs) {
+  if (d->state % 2 || d->b_row_stride % 2 || d->c_row_stride % 2) return false;
+  if (!d->packed && d->n_seq > 1 && (d->b_batch_stride % 2 || d->c_batch_stride % 2)) return false;
+  for (const void* p : ptrs)
+    if (reinterpret_cast<uintptr_t>(p) % 4) return false;
+  return true;
+}
+
 template <typename K>
 bool prepare_smem(K kernel, size_t bytes) {
   return bytes <= 48 * 1024 || allow_max_smem(reinterpret_cast<const void*>(kernel));
@@ -892,7 +1053,11 @@ bool prepare_smem(K kernel, size_t bytes) {
 template <typename T, int LPC>
 sf_status run_fwd(const ScanArgs& a, dim3 grid, cudaStream_t st) {
   constexpr int threads = Cfg<LPC>::THREADS;
-  if (a.seg_rows != kWhole) scan_carry_kernel<T, LPC, false><<<grid, threads, 0, st>>>(a);
+  if (a.seg_rows != kWhole) {
+    constexpr size_t bytes = sizeof(CarrySmem<T, LPC, false>);
+    if (!prepare_smem(scan_carry_kernel<T, LPC, false>, bytes)) return SF_ERR_CUDA;
+    scan_carry_kernel<T, LPC, false><<<grid, threads, bytes, st>>>(a);
+  }
   constexpr size_t smem = sizeof(FwdSmem<T, LPC>);
   if (!prepare_smem(scan_fwd_kernel<T, LPC>, smem)) return SF_ERR_CUDA;
   scan_fwd_kernel<T, LPC><<<grid, threads, smem, st>>>(a);
@@ -901,7 +1066,11 @@ sf_status run_fwd(const ScanArgs& a, dim3 grid, cudaStream_t st) {
 template <typename T, int LPC>
 sf_status run_bwd(const ScanArgs& a, dim3 grid, cudaStream_t st) {
   constexpr int threads = Cfg<LPC>::THREADS;
-  if (a.seg_rows != kWhole) scan_carry_kernel<T, LPC, true><<<grid, threads, 0, st>>>(a);
+  if (a.seg_rows != kWhole) {
+    constexpr size_t bytes = sizeof(CarrySmem<T, LPC, true>);
+    if (!prepare_smem(scan_carry_kernel<T, LPC, true>, bytes)) return SF_ERR_CUDA;
+    scan_carry_kernel<T, LPC, true><<<grid, threads, bytes, st>>>(a);
+  }
   constexpr size_t smem = sizeof(BwdSmem<T, LPC>);
   if (!prepare_smem(scan_bwd_kernel<T, LPC>, smem)) return SF_ERR_CUDA;
   scan_bwd_kernel<T, LPC><<<grid, threads, smem, st>>>(a);
@@ -954,6 +1123,7 @@ extern "C" sf_status sf_selective_scan(const void* x, const void* dt, const floa
   a.final_state = final_state;
   a.ck_out = static_cast<float*>(checkpoints);
   a.vec = vectors_fit(d, {x, dt, z, y});
+  a.words = words_fit(d, {B, C});
   a.seg_rows = segment_rows(d, kFwdBlocks);
   const long long carry = carry_floats(d, a.seg_rows), slots = slots_of(d, a.seg_rows);
   if (carry && (!workspace || workspace_bytes < (size_t)carry * sizeof(float))) return SF_ERR_WORKSPACE;
@@ -1018,6 +1188,7 @@ extern "C" sf_status sf_selective_scan_backward(const void* x, const void* dt, c
     a.seg_state = ws + l.carry;
     a.seg_dt = a.seg_state + slots * d->dim * d->state;
     a.vec = vectors_fit(d, {x, dt, z, dy, dx, ddt, dz});
+    a.words = words_fit(d, {B, C});
     const dim3 grid(tiles_of(d) * d->groups, (unsigned)slots);
     sf_status status = SF_OK;
     SF_SCAN_TYPES(d->dtype, SF_SCAN_LANES(d->state, status = (run_bwd<T, L>(a, grid, st))))
