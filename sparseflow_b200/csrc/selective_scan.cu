@@ -36,7 +36,8 @@ constexpr int kThreads = 128;  // of the single-token kernel
 constexpr int kS = 4;          // states per lane
 constexpr int kMaxState = 128;
 constexpr int kRows = 16;      // rows per tile, and per checkpoint
-constexpr int kHalf = 8;       // rows whose states the backward pass keeps in registers
+constexpr int kHalf = 8;       // rows between two additions over the warps in the backward pass
+constexpr int kPart = 4;       // rows whose states the backward pass keeps in registers
 constexpr float kLog2e = 1.4426950408889634f;
 
 struct ScanArgs {
@@ -731,7 +732,6 @@ __global__ void __launch_bounds__(Cfg<LPC>::THREADS, 2) scan_bwd_kernel(ScanArgs
   }
   float gD = 0.f, gbias = 0.f;
   const int e = entry(k.c), first = sums_first<LPC>(lane);
-  int buf = 0;
   for (int i = tiles - 1; i >= 0; --i) {
     const int rows = tile_rows(i);
     u64 h0[2] = {0, 0};  // the states before the tile
@@ -771,25 +771,27 @@ __global__ void __launch_bounds__(Cfg<LPC>::THREADS, 2) scan_bwd_kernel(ScanArgs
     f.done();
     f.load(a, tile_rows(i - (STAGES - 1)), -kRows);
     __syncthreads();
-    u64 h8[2] = {h0[0], h0[1]};
-    if (rows > kHalf) {
+    // The states before each part of kPart rows, then the parts from the last to the first.
+    u64 hb[kRows / kPart][2] = {{h0[0], h0[1]}};
 #pragma unroll
-      for (int r = 0; r < kHalf; ++r) {
-        const ulonglong2 du = *reinterpret_cast<const ulonglong2*>(&s.du[r][e]);
-        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&s.B[r][k.n]);
-        h8[0] = fma2(ex2x2(mul2(du.x, A2[0])), h8[0], mul2(du.y, b.x));
-        h8[1] = fma2(ex2x2(mul2(du.x, A2[1])), h8[1], mul2(du.y, b.y));
-      }
+    for (int r = 0; r < kRows - kPart; ++r) {
+      if (r % kPart == 0 && r + kPart >= rows) break;
+      const ulonglong2 du = *reinterpret_cast<const ulonglong2*>(&s.du[r][e]);
+      const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&s.B[r][k.n]);
+      h0[0] = fma2(ex2x2(mul2(du.x, A2[0])), h0[0], mul2(du.y, b.x));
+      h0[1] = fma2(ex2x2(mul2(du.x, A2[1])), h0[1], mul2(du.y, b.y));
+      if (r % kPart == kPart - 1) hb[r / kPart + 1][0] = h0[0], hb[r / kPart + 1][1] = h0[1];
     }
     u64 tA[2] = {0, 0};  // this tile's share of gA: sums of sums keep more digits than one long one
-#pragma unroll 1
-    for (int half = rows > kHalf ? 1 : 0; half >= 0; --half) {
-      const int t = half * kHalf;
-      u64 hs[kHalf + 1][2], as[kHalf][2];
-      hs[0][0] = half ? h8[0] : h0[0];
-      hs[0][1] = half ? h8[1] : h0[1];
 #pragma unroll
-      for (int r = 0; r < kHalf; ++r) {
+    for (int part = kRows / kPart - 1; part >= 0; --part) {
+      const int t = part * kPart;
+      if (t >= rows) continue;
+      u64 hs[kPart + 1][2], as[kPart][2];
+      hs[0][0] = hb[part][0];
+      hs[0][1] = hb[part][1];
+#pragma unroll
+      for (int r = 0; r < kPart; ++r) {
         const ulonglong2 du = *reinterpret_cast<const ulonglong2*>(&s.du[t + r][e]);
         const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&s.B[t + r][k.n]);
         as[r][0] = ex2x2(mul2(du.x, A2[0]));
@@ -797,66 +799,63 @@ __global__ void __launch_bounds__(Cfg<LPC>::THREADS, 2) scan_bwd_kernel(ScanArgs
         hs[r + 1][0] = fma2(as[r][0], hs[r][0], mul2(du.y, b.x));
         hs[r + 1][1] = fma2(as[r][1], hs[r][1], mul2(du.y, b.y));
       }
+      float pre[4], S[4], qa[4];
 #pragma unroll
-      for (int r4 = kHalf - 4; r4 >= 0; r4 -= 4) {
-        float pre[4], S[4], qa[4];
+      for (int r = kPart - 1; r >= 0; --r) {
+        const ulonglong2 du = *reinterpret_cast<const ulonglong2*>(&s.du[t + r][e]);
+        const u64 gp = *reinterpret_cast<const u64*>(&s.gp[t + r][e]);
+        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&s.B[t + r][k.n]);
+        const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(&s.C[t + r][k.n]);
+        pre[r] = sum2(fma2(c.x, hs[r + 1][0], mul2(c.y, hs[r + 1][1])));
+        gh[0] = fma2(gp, c.x, gh[0]);
+        gh[1] = fma2(gp, c.y, gh[1]);
+        S[r] = sum2(fma2(gh[0], b.x, mul2(gh[1], b.y)));
+        float v[8];
+        unpack2(v[0], v[1], mul2(gh[0], du.y));
+        unpack2(v[2], v[3], mul2(gh[1], du.y));
+        unpack2(v[4], v[5], mul2(gp, hs[r + 1][0]));
+        unpack2(v[6], v[7], mul2(gp, hs[r + 1][1]));
+        gh[0] = mul2(gh[0], as[r][0]);
+        gh[1] = mul2(gh[1], as[r][1]);
+        const u64 q0 = mul2(gh[0], hs[r][0]), q1 = mul2(gh[1], hs[r][1]);
+        qa[r] = sum2(fma2(q0, A2[0], mul2(q1, A2[1])));
+        tA[0] = fma2(q0, du.x, tA[0]);
+        tA[1] = fma2(q1, du.x, tA[1]);
+        channels_sum<LPC>(v, lane);
+        // value i < 4: state n + i of gB, else of gC
+        if (LPC >= 4 || (lane & 3 & ~(LPC - 1)) == 0)
 #pragma unroll
-        for (int rr = 3; rr >= 0; --rr) {
-          const int r = r4 + rr;
-          const ulonglong2 du = *reinterpret_cast<const ulonglong2*>(&s.du[t + r][e]);
-          const u64 gp = *reinterpret_cast<const u64*>(&s.gp[t + r][e]);
-          const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&s.B[t + r][k.n]);
-          const ulonglong2 c = *reinterpret_cast<const ulonglong2*>(&s.C[t + r][k.n]);
-          pre[rr] = sum2(fma2(c.x, hs[r + 1][0], mul2(c.y, hs[r + 1][1])));
-          gh[0] = fma2(gp, c.x, gh[0]);
-          gh[1] = fma2(gp, c.y, gh[1]);
-          S[rr] = sum2(fma2(gh[0], b.x, mul2(gh[1], b.y)));
-          float v[8];
-          unpack2(v[0], v[1], mul2(gh[0], du.y));
-          unpack2(v[2], v[3], mul2(gh[1], du.y));
-          unpack2(v[4], v[5], mul2(gp, hs[r + 1][0]));
-          unpack2(v[6], v[7], mul2(gp, hs[r + 1][1]));
-          gh[0] = mul2(gh[0], as[r][0]);
-          gh[1] = mul2(gh[1], as[r][1]);
-          const u64 q0 = mul2(gh[0], hs[r][0]), q1 = mul2(gh[1], hs[r][1]);
-          qa[rr] = sum2(fma2(q0, A2[0], mul2(q1, A2[1])));
-          tA[0] = fma2(q0, du.x, tA[0]);
-          tA[1] = fma2(q1, du.x, tA[1]);
-          channels_sum<LPC>(v, lane);
-          // value i < 4: state n + i of gB, else of gC
-          if (LPC >= 4 || (lane & 3 & ~(LPC - 1)) == 0)
+          for (int j = 0; j < kSumsPerLane<LPC>; ++j)
+            s.bc[part / 2 % 2][warp][t % kHalf + r][((first + j) >> 2) * F::NP + k.n + ((first + j) & 3)] = v[j];
+      }
+      float po4[kRowsPerLane<LPC>], So[kRowsPerLane<LPC>], qo[kRowsPerLane<LPC>];
+      scatter4<LPC>(po4, pre, k.q);
+      scatter4<LPC>(So, S, k.q);
+      scatter4<LPC>(qo, qa, k.q);
+      if (LPC <= 4 || k.q < 4)
 #pragma unroll
-            for (int j = 0; j < kSumsPerLane<LPC>; ++j)
-              s.bc[buf][warp][r][((first + j) >> 2) * F::NP + k.n + ((first + j) & 3)] = v[j];
+        for (int j = 0; j < kRowsPerLane<LPC>; ++j) {
+          const int r = t + scatter_row<LPC>(k.q) + j;
+          const float4 g = s.gp[r][e];
+          const float2 sg = s.sg[r][k.c];
+          const float dt = s.du[r][e].x;
+          const float gdt = fmaf(g.w, So[j], qo[j] * (1.f / kLog2e)) * sg.x;
+          s.dx[r][k.c] = DT<T>::from_f(fmaf(dt, So[j], g.z));
+          s.ddt[r][k.c] = DT<T>::from_f(gdt);
+          s.dz[r][k.c] = DT<T>::from_f((po4[j] + s.px[r][k.c]) * sg.y);
+          gD = fmaf(g.x, g.w, gD);
+          gbias += r < rows ? gdt : 0.f;
         }
-        float po[kRowsPerLane<LPC>], So[kRowsPerLane<LPC>], qo[kRowsPerLane<LPC>];
-        scatter4<LPC>(po, pre, k.q);
-        scatter4<LPC>(So, S, k.q);
-        scatter4<LPC>(qo, qa, k.q);
-        if (LPC <= 4 || k.q < 4)
+      if (t % kHalf == 0) {  // both parts of a half are done
+        __syncthreads();
+        for (int u = threadIdx.x; u < kHalf * 2 * F::NP; u += F::THREADS) {
+          const int r = u / (2 * F::NP), m = u % (2 * F::NP);
+          float v = 0.f;
 #pragma unroll
-          for (int j = 0; j < kRowsPerLane<LPC>; ++j) {
-            const int r = t + r4 + scatter_row<LPC>(k.q) + j;
-            const float4 g = s.gp[r][e];
-            const float2 sg = s.sg[r][k.c];
-            const float dt = s.du[r][e].x;
-            const float gdt = fmaf(g.w, So[j], qo[j] * (1.f / kLog2e)) * sg.x;
-            s.dx[r][k.c] = DT<T>::from_f(fmaf(dt, So[j], g.z));
-            s.ddt[r][k.c] = DT<T>::from_f(gdt);
-            s.dz[r][k.c] = DT<T>::from_f((po[j] + s.px[r][k.c]) * sg.y);
-            gD = fmaf(g.x, g.w, gD);
-            gbias += t + r4 + scatter_row<LPC>(k.q) + j < rows ? gdt : 0.f;
-          }
+          for (int w = 0; w < F::WARPS; ++w) v += s.bc[part / 2 % 2][w][r][m];
+          if (t + r < rows) bc_out[(long long)(t + r) * a.groups * 2 * F::NP + m] = v;
+        }
       }
-      __syncthreads();
-      for (int u = threadIdx.x; u < kHalf * 2 * F::NP; u += F::THREADS) {
-        const int r = u / (2 * F::NP), m = u % (2 * F::NP);
-        float v = 0.f;
-#pragma unroll
-        for (int w = 0; w < F::WARPS; ++w) v += s.bc[buf][w][r][m];
-        if (t + r < rows) bc_out[(long long)(t + r) * a.groups * 2 * F::NP + m] = v;
-      }
-      buf ^= 1;
     }
     gA[0] = add2(gA[0], tA[0]);
     gA[1] = add2(gA[1], tA[1]);
