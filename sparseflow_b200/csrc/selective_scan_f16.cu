@@ -1,0 +1,7 @@
+// fp16 instantiations of the selective scan kernels.
+#include "selective_scan.cuh"
+
+namespace sf {
+template sf_status scan_forward<__half>(const ScanArgs&, int, bool, dim3, cudaStream_t);
+template sf_status scan_backward<__half>(const ScanArgs&, int, bool, dim3, cudaStream_t);
+}  // namespace sf

@@ -1,0 +1,7 @@
+// fp32 instantiations of the selective scan kernels.
+#include "selective_scan.cuh"
+
+namespace sf {
+template sf_status scan_forward<float>(const ScanArgs&, int, bool, dim3, cudaStream_t);
+template sf_status scan_backward<float>(const ScanArgs&, int, bool, dim3, cudaStream_t);
+}  // namespace sf
