@@ -715,12 +715,12 @@ struct BwdSmem {
   using F = Cfg<LPC, CPT>;
   static constexpr int STAGES = 2;  // a tile takes longer than the latency of memory
   float2 du[kRows][F::CH];   // dt, dt x
-  float2 gx[kRows][F::CH];   // gp, x
-  float2 sg[kRows][F::PAD];  // softplus'(raw), dy silu'(z)
+  float2 gx[kRows][F::CH];   // gp, x; when a part is done: dx, -
+  float2 sg[kRows][F::PAD];  // softplus'(raw), dy silu'(z); when a part is done: ddt, dz
   float B[kRows][F::NP], C[kRows][F::NP];
   float bc[2][F::WARPS][kHalf][2 * F::NP];  // sums over a warp's channels, one half tile after the other
-  T dx[kRows][F::PAD], ddt[kRows][F::PAD], dz[kRows][F::PAD];
-  ulonglong2 hb[kRows / kPart - 1][CPT][F::THREADS];  // each thread's states before the parts but the first
+  float4 ck[2][CPT][F::THREADS];                      // each thread's states before a tile, and before the next
+  ulonglong2 hb[kRows / kPart - 1][CPT][F::THREADS];  // and before its parts but the first
   Ring<T, LPC, CPT, VEC, true, true, true, true, true, STAGES> ring;
 };
 
@@ -800,16 +800,39 @@ __global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, CPT == 2 ? 3 : 2) scan
       const int r = f.r + v * f.RSTEP;
       if (f.has_unit(v) && r < rows) {
         const long long o = po + (long long)v * f.RSTEP * a.dim;
-        using V4 = seq::Vec<T, 4>;
-        store_unit<VEC>(static_cast<T*>(a.dx) + o, *reinterpret_cast<const V4*>(&s.dx[r][f.m]), f.valid);
-        store_unit<VEC>(static_cast<T*>(a.ddt) + o, *reinterpret_cast<const V4*>(&s.ddt[r][f.m]), f.valid);
-        if (a.dz) store_unit<VEC>(static_cast<T*>(a.dz) + o, *reinterpret_cast<const V4*>(&s.dz[r][f.m]), f.valid);
+        seq::Vec<T, 4> dx, ddt, dz;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          dx.v[j] = DT<T>::from_f(s.gx[r][entry(f.m + j)].x);
+          ddt.v[j] = DT<T>::from_f(s.sg[r][f.m + j].x);
+          dz.v[j] = DT<T>::from_f(s.sg[r][f.m + j].y);
+        }
+        store_unit<VEC>(static_cast<T*>(a.dx) + o, dx, f.valid);
+        store_unit<VEC>(static_cast<T*>(a.ddt) + o, ddt, f.valid);
+        if (a.dz) store_unit<VEC>(static_cast<T*>(a.dz) + o, dz, f.valid);
       }
     }
     po -= (long long)kRows * a.dim;
   };
+  // The checkpoint of a tile into this thread's place of it, in the copies' group of the tile above.
+  auto load_ck = [&](int i) {
+#pragma unroll
+    for (int j = 0; j < CPT; ++j) {
+      float4* dst = &s.ck[i & 1][j][threadIdx.x];
+      const float* src = ck + (long long)k.chan(j) * a.state;
+      if ((a.state & 3) == 0) {
+        cp_async(dst, k.own(j) && k.n < a.state ? src + k.n : a.ck, 16, k.own(j) && k.n < a.state);
+      } else {
+        float v[kS] = {};
+        if (k.own(j)) load4(v, src, k.n, a.state);
+        *dst = make_float4(v[0], v[1], v[2], v[3]);
+      }
+    }
+    ck -= (long long)a.dim * a.state;
+  };
   const int last_rows = (int)(r1 - last);
   auto tile_rows = [&](int i) { return i < 0 ? 0 : i == tiles - 1 ? last_rows : kRows; };
+  if (tiles > 0) load_ck(tiles - 1);
   for (int i = 0; i < STAGES - 1; ++i) f.load(a, tile_rows(tiles - 1 - i), -kRows);
   u64 A2[CPT][2], gh[CPT][2] = {}, gA[CPT][2] = {};
   float D[CPT], gD[CPT] = {}, gbias[CPT] = {};
@@ -824,11 +847,6 @@ __global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, CPT == 2 ? 3 : 2) scan
   const int first = sums_first<LPC>(lane);
   for (int i = tiles - 1; i >= 0; --i) {
     const int rows = tile_rows(i);
-    u64 h0[CPT][2] = {};  // the states before the tile
-#pragma unroll
-    for (int j = 0; j < CPT; ++j)
-      if (k.own(j)) load4(h0[j], ck + (long long)k.chan(j) * a.state, k.n, a.state);
-    ck -= (long long)a.dim * a.state;
     f.wait();
     __syncthreads();
     if (i + 1 < tiles) put(tile_rows(i + 1));
@@ -862,39 +880,44 @@ __global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, CPT == 2 ? 3 : 2) scan
       }
     f.convert_bc(s.B, s.C);
     f.done();
+    if (i > 0) load_ck(i - 1);
     f.load(a, tile_rows(i - (STAGES - 1)), -kRows);
     __syncthreads();
+    const int parts = (rows + kPart - 1) / kPart;
     {
       u64 h[CPT][2];
 #pragma unroll
-      for (int j = 0; j < CPT; ++j) h[j][0] = h0[j][0], h[j][1] = h0[j][1];
+      for (int j = 0; j < CPT; ++j) {
+        const ulonglong2 v = *reinterpret_cast<const ulonglong2*>(&s.ck[i & 1][j][threadIdx.x]);
+        h[j][0] = v.x, h[j][1] = v.y;
+      }
+#pragma unroll 1
+      for (int part = 0; part < parts - 1; ++part) {
 #pragma unroll
-      for (int r = 0; r < kRows - kPart; ++r) {
-        if (r % kPart == 0 && r + kPart >= rows) break;
-        const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&s.B[r][k.n]);
+        for (int r = 0; r < kPart; ++r) {
+          const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(&s.B[part * kPart + r][k.n]);
 #pragma unroll
-        for (int j = 0; j < CPT; ++j) {
-          u64 dt, u;
-          load_du(dt, u, &s.du[r][entry(k.chan(j))]);
-          h[j][0] = fma2(ex2x2(mul2(dt, A2[j][0])), h[j][0], mul2(u, b.x));
-          h[j][1] = fma2(ex2x2(mul2(dt, A2[j][1])), h[j][1], mul2(u, b.y));
-          if (r % kPart == kPart - 1) s.hb[r / kPart][j][threadIdx.x] = make_ulonglong2(h[j][0], h[j][1]);
+          for (int j = 0; j < CPT; ++j) {
+            u64 dt, u;
+            load_du(dt, u, &s.du[part * kPart + r][entry(k.chan(j))]);
+            h[j][0] = fma2(ex2x2(mul2(dt, A2[j][0])), h[j][0], mul2(u, b.x));
+            h[j][1] = fma2(ex2x2(mul2(dt, A2[j][1])), h[j][1], mul2(u, b.y));
+          }
         }
+#pragma unroll
+        for (int j = 0; j < CPT; ++j) s.hb[part][j][threadIdx.x] = make_ulonglong2(h[j][0], h[j][1]);
       }
     }
     u64 tA[CPT][2] = {};  // this tile's share of gA: sums of sums keep more digits than one long one
-#pragma unroll
-    for (int part = kRows / kPart - 1; part >= 0; --part) {
+#pragma unroll 1
+    for (int part = parts - 1; part >= 0; --part) {
       const int t = part * kPart;
-      if (t >= rows) continue;
       u64 hs[CPT][kPart + 1][2], as[CPT][kPart][2];
 #pragma unroll
       for (int j = 0; j < CPT; ++j) {
-        hs[j][0][0] = h0[j][0], hs[j][0][1] = h0[j][1];
-        if (part > 0) {
-          const ulonglong2 v = s.hb[part > 0 ? part - 1 : 0][j][threadIdx.x];
-          hs[j][0][0] = v.x, hs[j][0][1] = v.y;
-        }
+        const ulonglong2 v = part > 0 ? s.hb[part - 1][j][threadIdx.x]
+                                      : *reinterpret_cast<const ulonglong2*>(&s.ck[i & 1][j][threadIdx.x]);
+        hs[j][0][0] = v.x, hs[j][0][1] = v.y;
       }
 #pragma unroll
       for (int r = 0; r < kPart; ++r) {
@@ -946,7 +969,7 @@ __global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, CPT == 2 ? 3 : 2) scan
         if (LPC >= 4 || (lane & 3 & ~(LPC - 1)) == 0)
 #pragma unroll
           for (int j = 0; j < kSumsPerLane<LPC>; ++j)
-            s.bc[part / 2 % 2][warp][t % kHalf + r][((first + j) >> 2) * F::NP + k.n + ((first + j) & 3)] = v[j];
+            s.bc[part >> 1 & 1][warp][t % kHalf + r][((first + j) >> 2) * F::NP + k.n + ((first + j) & 3)] = v[j];
       }
 #pragma unroll
       for (int j = 0; j < CPT; ++j) {
@@ -961,9 +984,8 @@ __global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, CPT == 2 ? 3 : 2) scan
             const float2 g = s.gx[r][entry(c)], sg = s.sg[r][c];
             const float dt = s.du[r][entry(c)].x;
             const float gdt = fmaf(g.y, So[l], qo[l] * (1.f / kLog2e)) * sg.x;
-            s.dx[r][c] = DT<T>::from_f(fmaf(dt, So[l], D[j] * g.x));
-            s.ddt[r][c] = DT<T>::from_f(gdt);
-            s.dz[r][c] = DT<T>::from_f(fmaf(D[j], g.y, po4[l]) * sg.y);
+            s.gx[r][entry(c)].x = fmaf(dt, So[l], D[j] * g.x);
+            s.sg[r][c] = make_float2(gdt, fmaf(D[j], g.y, po4[l]) * sg.y);
             gD[j] = fmaf(g.x, g.y, gD[j]);
             gbias[j] += r < rows ? gdt : 0.f;
           }
@@ -974,7 +996,7 @@ __global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, CPT == 2 ? 3 : 2) scan
           const int r = u / (2 * F::NP), m = u % (2 * F::NP);
           float v = 0.f;
 #pragma unroll
-          for (int w = 0; w < F::WARPS; ++w) v += s.bc[part / 2 % 2][w][r][m];
+          for (int w = 0; w < F::WARPS; ++w) v += s.bc[part >> 1 & 1][w][r][m];
           if (t + r < rows) bc_out[(long long)(t + r) * a.groups * 2 * F::NP + m] = v;
         }
       }
