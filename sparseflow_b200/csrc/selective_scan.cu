@@ -89,20 +89,35 @@ int tiles_of(const sf_selective_scan_desc* d) {  // blocks for the channels of a
   return (per + ch - 1) / ch;
 }
 
-// Rows per segment: sequences whole where their channels alone give `want` blocks; else cut so that they do, but
-// not below 128 rows, nor into more than 32 segments.
-long long segment_rows(const sf_selective_scan_desc* d, long long want) {
-  const long long blocks = (long long)tiles_of(d) * d->groups * d->n_seq;
-  if (blocks >= want || d->length <= 256) return kWhole;
+// Rows per segment. Measured on a B200 (bf16, 16 states, sequences of 2048 rows, times in ms): whole, a block takes as
+// long alone on its SM as t[0], two or more together as t[1], t[2] ..; cut into about 1400 blocks in all, so that the
+// last round of them is short beside the rest, the time goes with the work, `cut` a block's sequence (the kernel that
+// finds the segments' shares included). Whole against cut, forward: 64 blocks 0.23 / 0.12, 160: 0.31 / 0.26, 192:
+// 0.31 / 0.30, 256: 0.31 / 0.38, 512: 0.50 / 0.75; backward: 128 blocks 0.76 / 0.52, 256: 1.02 / 0.96, 320: 1.29 / 1.16,
+// 384: 1.29 / 1.39, 512: 1.97 / 1.86. The cheaper is taken; 0.01 ms stands for the launch that cutting adds. Packed
+// sequences count as of equal length (the host does not know theirs).
+struct SegmentCosts {
+  int resident;  // blocks on an SM
+  double t[4], cut;
+};
+constexpr SegmentCosts kFwdCosts = {4, {0.232, 0.309, 0.400, 0.500}, 1.62e-3};
+constexpr SegmentCosts kBwdCosts = {3, {0.750, 1.000, 1.290, 0.}, 3.62e-3};
+
+long long segment_rows(const sf_selective_scan_desc* d, const SegmentCosts& k) {
+  if (d->n_seq == 0 || d->length == 0) return kWhole;
+  const long long across = (long long)tiles_of(d) * d->groups, blocks = across * d->n_seq;
   const long long total = d->packed ? d->length : d->length * d->n_seq;
-  const long long cuts = (want + (long long)tiles_of(d) * d->groups - 1) / ((long long)tiles_of(d) * d->groups);
-  long long rows = (total + cuts - 1) / cuts;
-  if (rows < 128) rows = 128;
-  if (rows < (d->length + 31) / 32) rows = (d->length + 31) / 32;
+  const double length = (double)total / d->n_seq / 2048.;
+  const long long w = (blocks + 147) / 148;
+  double whole = (double)(w / k.resident) * k.t[k.resident - 1];
+  if (w % k.resident) whole += k.t[w % k.resident - 1];
+  if (whole * length <= k.cut * blocks * length + 0.01) return kWhole;
+  long long rows = (total * across + 1399) / 1400;
+  if (rows < 64) rows = 64;
+  if (rows < (d->length + 63) / 64) rows = (d->length + 63) / 64;
   rows = (rows + kRows - 1) / kRows * kRows;
   return rows >= d->length ? kWhole : rows;
 }
-constexpr long long kFwdBlocks = 444, kBwdBlocks = 296;  // three, two blocks for each SM
 long long slots_of(const sf_selective_scan_desc* d, long long seg) {
   return seq::total_slots(d->length, d->n_seq, d->packed, seg);
 }
@@ -208,7 +223,7 @@ extern "C" size_t sf_selective_scan_checkpoint_bytes(const sf_selective_scan_des
 
 extern "C" size_t sf_selective_scan_workspace_size(const sf_selective_scan_desc* d) {
   if (!valid(d) || d->n_seq == 0) return 0;
-  return (size_t)carry_floats(d, segment_rows(d, kFwdBlocks)) * sizeof(float);
+  return (size_t)carry_floats(d, segment_rows(d, kFwdCosts)) * sizeof(float);
 }
 
 extern "C" sf_status sf_selective_scan(const void* x, const void* dt, const float* A, const void* B, const void* C,
@@ -226,7 +241,7 @@ extern "C" sf_status sf_selective_scan(const void* x, const void* dt, const floa
   a.final_state = final_state;
   a.ck_out = static_cast<float*>(checkpoints);
   const bool vec = vectors_fit(d, {x, dt, z, y}) && words_fit(d, {B, C});
-  a.seg_rows = segment_rows(d, kFwdBlocks);
+  a.seg_rows = segment_rows(d, kFwdCosts);
   const long long carry = carry_floats(d, a.seg_rows), slots = slots_of(d, a.seg_rows);
   if (carry && (!workspace || workspace_bytes < (size_t)carry * sizeof(float))) return SF_ERR_WORKSPACE;
   for (const void* p : {static_cast<const void*>(A), static_cast<const void*>(initial_state),
@@ -245,7 +260,7 @@ extern "C" sf_status sf_selective_scan(const void* x, const void* dt, const floa
 
 extern "C" size_t sf_selective_scan_backward_workspace_size(const sf_selective_scan_desc* d) {
   if (!valid(d)) return 0;
-  return (size_t)bwd_layout(d, segment_rows(d, kBwdBlocks)).total * sizeof(float);
+  return (size_t)bwd_layout(d, segment_rows(d, kBwdCosts)).total * sizeof(float);
 }
 
 extern "C" sf_status sf_selective_scan_backward(const void* x, const void* dt, const float* A, const void* B,
@@ -264,7 +279,7 @@ extern "C" sf_status sf_selective_scan_backward(const void* x, const void* dt, c
   if (rows > 0 && (!x || !dt || !B || !C || !checkpoints || !dy || !dx || !ddt || !dB || !dC))
     return SF_ERR_INVALID_ARG;
   if ((z && rows > 0 && !dz) || (D && !dD) || (dt_bias && !d_dt_bias)) return SF_ERR_INVALID_ARG;
-  const long long seg = segment_rows(d, kBwdBlocks), slots = slots_of(d, seg);
+  const long long seg = segment_rows(d, kBwdCosts), slots = slots_of(d, seg);
   const BwdLayout l = bwd_layout(d, seg);
   if (some && (!workspace || workspace_bytes < (size_t)l.total * sizeof(float))) return SF_ERR_WORKSPACE;
   if (some && !aligned16(workspace)) return SF_ERR_ALIGNMENT;
