@@ -93,13 +93,13 @@ __device__ __forceinline__ void load_w8(float (&o)[kV], const void* p, int c, in
 // act(gate) and its derivative.
 __device__ __forceinline__ float gate_act(float g, int kind) {
   if (kind == SF_GATE_SILU) return seq::silu(g);
-  if (kind == SF_GATE_SIGMOID) return seq::sigmoid(g);
+  if (kind == SF_GATE_SIGMOID) return seq::logistic(g);
   return g;
 }
 __device__ __forceinline__ float gate_dact(float g, int kind) {
   if (kind == SF_GATE_SILU) return seq::dsilu(g);
   if (kind == SF_GATE_SIGMOID) {
-    const float s = seq::sigmoid(g);
+    const float s = seq::logistic(g);
     return s * (1.f - s);
   }
   return 1.f;

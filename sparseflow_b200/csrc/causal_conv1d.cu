@@ -5,20 +5,26 @@
 //   g = dy act'(pre);  dx[t] = sum_k w[k] g[t + (W-1) - k];
 //   dw[k] = sum_t g[t] x[t - (W-1) + k];  dbias = sum_t g[t]
 //
-// About 2 W + 5 operations an element against 2 |x| bytes: HBM-bound. A thread
-// owns V neighbouring channels (16 or 8 bytes of a row, so a warp reads whole
-// sectors) and walks down a slot of rows with the last W rows in registers:
-// every x is read once, but for the W - 1 rows above each slot.
+// About W + 9 instructions an element forward against 2 |x| bytes, 3 W + 15 backward against 3 |x|: HBM-bound, if
+// enough bytes are on their way. A thread owns V neighbouring channels (8 or 16 bytes of a row, so a warp reads whole
+// sectors) and walks down a slot of rows with the last W rows in registers; the rows of a group (kGroup) are loaded
+// together before the first of them is used. Every x is read once, but for the W - 1 rows above each slot, which come
+// from L2. Products and sums are pairs of fp32 (mul/fma .f32x2).
 #include "sequence.cuh"
 
 namespace sf {
 namespace {
 
+using seq::fma2;
+using seq::pack2;
 using seq::Rows;
 using seq::Span;
+using seq::u64;
+using seq::unpack2;
 
 constexpr int kConvThreads = 128;
 constexpr int kMaxWidth = 8;
+constexpr int kFwdGroup = 8, kBwdGroup = 4;  // rows loaded together
 
 struct ConvArgs {
   const void *x, *weight, *bias, *init, *dy, *dfinal;
@@ -30,21 +36,47 @@ struct ConvArgs {
   int dim, width, silu, w_dtype;
 };
 
-// Row `t` of the sequence (t < 0: of the state before it; rows above that and channels past dim are 0).
+// V channels of a row as pairs (one channel: a pair whose second half is 0).
+template <int V>
+constexpr int kPairs = (V + 1) / 2;
 template <typename T, int V>
-__device__ __forceinline__ void load_row(float (&out)[V], const ConvArgs& a, const T* xs, const Span& p, long long t,
-                                         int d) {
-  if (t >= 0) {
-    seq::load_vec<T, V>(out, xs + t * a.x_row);
-    return;
-  }
-  const long long j = t + (a.width - 1);
-  if (a.init && j >= 0) {
-    seq::load_vec<T, V>(out, static_cast<const T*>(a.init) + ((long long)p.s * (a.width - 1) + j) * a.dim + d);
-  } else {
+__device__ __forceinline__ void to_pairs(u64 (&o)[kPairs<V>], const seq::Vec<T, V>& v) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) out[i] = 0.f;
+  for (int i = 0; i < kPairs<V>; ++i)
+    o[i] = pack2(DT<T>::to_f(v.v[2 * i]), 2 * i + 1 < V ? DT<T>::to_f(v.v[(2 * i + 1) % V]) : 0.f);
+}
+template <typename T, int V>
+__device__ __forceinline__ seq::Vec<T, V> from_pairs(const u64 (&p)[kPairs<V>]) {
+  seq::Vec<T, V> v;
+#pragma unroll
+  for (int i = 0; i < kPairs<V>; ++i) {
+    float lo, hi;
+    unpack2(lo, hi, p[i]);
+    v.v[2 * i] = DT<T>::from_f(lo);
+    if (2 * i + 1 < V) v.v[(2 * i + 1) % V] = DT<T>::from_f(hi);
   }
+  return v;
+}
+template <typename T, int V>
+__device__ __forceinline__ seq::Vec<T, V> load_raw(const T* p) {
+  return *reinterpret_cast<const seq::Vec<T, V>*>(p);
+}
+template <typename T, int V>
+__device__ __forceinline__ void store_raw(T* p, const seq::Vec<T, V>& v) {
+  *reinterpret_cast<seq::Vec<T, V>*>(p) = v;
+}
+
+// Row `t` of the sequence (t < 0: of the state before it; rows above that are 0).
+template <typename T, int V>
+__device__ __forceinline__ seq::Vec<T, V> load_row(const ConvArgs& a, const T* xs, const Span& p, long long t, int d) {
+  if (t >= 0) return load_raw<T, V>(xs + t * a.x_row);
+  const long long j = t + (a.width - 1);
+  if (a.init && j >= 0)
+    return load_raw<T, V>(static_cast<const T*>(a.init) + ((long long)p.s * (a.width - 1) + j) * a.dim + d);
+  seq::Vec<T, V> z;
+#pragma unroll
+  for (int i = 0; i < V; ++i) z.v[i] = DT<T>::from_f(0.f);
+  return z;
 }
 
 // First element of the sequence for channel d, and of its rows in a contiguous tensor.
@@ -56,94 +88,172 @@ __device__ __forceinline__ long long seq_row0(const ConvArgs& a, const Span& p) 
   return a.rows.offsets ? p.begin : (long long)p.s * a.rows.length;
 }
 
-// W taps; WT is W rounded up to 4 or 8, the taps before the first (k < WT - W) are skipped, not multiplied by 0:
-// the row they would meet may hold an infinity.
+// W taps: WT = W up to 4, else 8, where the taps before the first (k < WT - W) are skipped, not multiplied by 0: the
+// row they would meet may hold an infinity.
+template <int WT>
+__device__ __forceinline__ int skipped(const ConvArgs& a) {
+  return WT <= 4 ? 0 : WT - a.width;
+}
 template <int V, int WT>
-__device__ __forceinline__ void load_weights(float (&w)[WT][V], float (&b)[V], const ConvArgs& a, int d) {
+__device__ __forceinline__ void load_weights(u64 (&w)[WT][kPairs<V>], u64 (&b)[kPairs<V>], const ConvArgs& a, int d) {
 #pragma unroll
-  for (int i = 0; i < V; ++i) {
+  for (int i = 0; i < kPairs<V>; ++i) {
+    float v[2];
+#pragma unroll
+    for (int k = 0; k < WT; ++k) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        v[h] = k >= skipped<WT>(a) && 2 * i + h < V
+                   ? seq::load_param(a.weight, (long long)(d + 2 * i + h) * a.width + k - skipped<WT>(a), a.w_dtype)
+                   : 0.f;
+      w[k][i] = pack2(v[0], v[1]);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      v[h] = a.bias && 2 * i + h < V ? seq::load_param(a.bias, d + 2 * i + h, a.w_dtype) : 0.f;
+    b[i] = pack2(v[0], v[1]);
+  }
+}
+
+// The same through shared memory, for blocks that walk down many rows: the block's weights [channels][W] are read once,
+// in order, and turned to [tap][channel] (a thread's own reads would touch a sector each).
+template <int V, int WT>
+struct Weights {
+  float w[WT][kConvThreads * V], b[kConvThreads * V];
+};
+template <int V, int WT>
+__device__ __forceinline__ void stage_weights(Weights<V, WT>& s, const ConvArgs& a, int d0) {
+  const int n = min(kConvThreads * V, a.dim - d0), skip = skipped<WT>(a);
+  for (int i = threadIdx.x; i < n * a.width; i += kConvThreads)
+    s.w[skip + i % a.width][i / a.width] = seq::load_param(a.weight, (long long)d0 * a.width + i, a.w_dtype);
+  for (int i = threadIdx.x; i < n; i += kConvThreads)
+    s.b[i] = a.bias ? seq::load_param(a.bias, d0 + i, a.w_dtype) : 0.f;
+}
+template <int V, int WT>
+__device__ __forceinline__ void own_weights(u64 (&w)[WT][kPairs<V>], u64 (&b)[kPairs<V>], const Weights<V, WT>& s,
+                                            int skip) {
+#pragma unroll
+  for (int i = 0; i < kPairs<V>; ++i) {
+    const int c = threadIdx.x * V + 2 * i;
+#pragma unroll
+    for (int k = 0; k < WT; ++k) w[k][i] = k >= skip ? pack2(s.w[k][c], 2 * i + 1 < V ? s.w[k][c + 1] : 0.f) : 0;
+    b[i] = pack2(s.b[c], 2 * i + 1 < V ? s.b[c + 1] : 0.f);
+  }
+}
+
+// bias + sum over the taps of w[k] row[k]
+template <int P, int WT>
+__device__ __forceinline__ void taps(u64 (&o)[P], const u64 (&b)[P], const u64 (&w)[WT][P], const u64 (&row)[WT][P],
+                                     int skip) {
+#pragma unroll
+  for (int i = 0; i < P; ++i) {
+    o[i] = b[i];
 #pragma unroll
     for (int k = 0; k < WT; ++k)
-      w[k][i] = k >= WT - a.width
-                    ? seq::load_param(a.weight, (long long)(d + i) * a.width + k - (WT - a.width), a.w_dtype)
-                    : 0.f;
-    b[i] = a.bias ? seq::load_param(a.bias, d + i, a.w_dtype) : 0.f;
+      if (k >= skip) o[i] = fma2(w[k][i], row[k][i], o[i]);
   }
+}
+template <int P, int WT>
+__device__ __forceinline__ void shift(u64 (&row)[WT][P]) {
+#pragma unroll
+  for (int k = 0; k + 1 < WT; ++k)
+#pragma unroll
+    for (int i = 0; i < P; ++i) row[k][i] = row[k + 1][i];
 }
 
 template <typename T, int V, int WT>
-__global__ void __launch_bounds__(kConvThreads) conv_fwd_kernel(ConvArgs a) {
-  const int d = (blockIdx.y * kConvThreads + threadIdx.x) * V;
-  if (d >= a.dim) return;
+__global__ void __launch_bounds__(kConvThreads, WT <= 4 ? 4 : 2) conv_fwd_kernel(ConvArgs a) {
+  constexpr int P = kPairs<V>;
+  __shared__ Weights<V, WT> sw;
+  const int d0 = blockIdx.y * kConvThreads * V, d = d0 + threadIdx.x * V;
   const Span p = seq::slot_span(a.rows, blockIdx.x, a.slot_rows);
   if (p.len < 0) return;
+  stage_weights<V, WT>(sw, a, d0);
+  __syncthreads();
+  if (d >= a.dim) return;
   const T* xs = seq_x<T>(a, p, d);
-  T* ys = static_cast<T*>(a.y) + seq_row0(a, p) * a.dim + d;
   const long long r1 = min(p.r0 + a.slot_rows, p.len);
+  const int skip = skipped<WT>(a);
 
-  float w[WT][V], b[V], win[WT][V];  // win[WT-1]: the newest row
-  load_weights<V, WT>(w, b, a, d);
+  u64 w[WT][P], b[P], win[WT][P];  // win[WT-1]: the newest row
+  own_weights<V, WT>(w, b, sw, skip);
 #pragma unroll
-  for (int k = 1; k < WT; ++k) load_row<T, V>(win[k], a, xs, p, p.r0 - WT + k, d);
-  for (long long t = p.r0; t < r1; ++t) {
+  for (int k = 1; k < WT; ++k) to_pairs<T, V>(win[k], load_row<T, V>(a, xs, p, p.r0 - WT + k, d));
+  const T* px = xs + p.r0 * a.x_row;
+  T* py = static_cast<T*>(a.y) + (seq_row0(a, p) + p.r0) * a.dim + d;
+  auto one = [&](const seq::Vec<T, V>& x, T* y) {
+    shift<P, WT>(win);
+    to_pairs<T, V>(win[WT - 1], x);
+    u64 o[P];
+    taps<P, WT>(o, b, w, win, skip);
+    if (a.silu) {
 #pragma unroll
-    for (int k = 0; k + 1 < WT; ++k)
-#pragma unroll
-      for (int i = 0; i < V; ++i) win[k][i] = win[k + 1][i];
-    seq::load_vec<T, V>(win[WT - 1], xs + t * a.x_row);
-    float o[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      o[i] = b[i];
-#pragma unroll
-      for (int k = 0; k < WT; ++k)
-        if (k >= WT - a.width) o[i] = fmaf(w[k][i], win[k][i], o[i]);
-      if (a.silu) o[i] = seq::silu(o[i]);
+      for (int i = 0; i < P; ++i) {
+        float lo, hi;
+        unpack2(lo, hi, o[i]);
+        o[i] = pack2(seq::silu(lo), seq::silu(hi));
+      }
     }
-    seq::store_vec<T, V>(ys + t * a.dim, o);
+    store_raw<T, V>(y, from_pairs<T, V>(o));
+  };
+  seq::Vec<T, V> raw[kFwdGroup];
+  long long t = p.r0;
+  // Whole groups without conditions, so that the moving window costs no moves, then the rows that are left.
+  for (; t + kFwdGroup <= r1; t += kFwdGroup) {
+#pragma unroll
+    for (int u = 0; u < kFwdGroup; ++u) raw[u] = load_raw<T, V>(px + u * a.x_row);
+#pragma unroll
+    for (int u = 0; u < kFwdGroup; ++u) one(raw[u], py + (long long)u * a.dim);
+    px += kFwdGroup * a.x_row;
+    py += (long long)kFwdGroup * a.dim;
+  }
+  if (t < r1) {
+#pragma unroll
+    for (int u = 0; u < kFwdGroup; ++u)
+      if (t + u < r1) raw[u] = load_raw<T, V>(px + u * a.x_row);
+#pragma unroll
+    for (int u = 0; u < kFwdGroup; ++u)
+      if (t + u < r1) one(raw[u], py + (long long)u * a.dim);
   }
   if (a.final_state && p.r0 == 0) {
-    for (int j = 0; j < a.width - 1; ++j) {
-      float o[V];
-      load_row<T, V>(o, a, xs, p, p.len - (a.width - 1) + j, d);
-      seq::store_vec<T, V>(
-          static_cast<T*>(a.final_state) + ((long long)p.s * (a.width - 1) + j) * a.dim + d, o);
-    }
+    for (int j = 0; j < a.width - 1; ++j)
+      store_raw<T, V>(static_cast<T*>(a.final_state) + ((long long)p.s * (a.width - 1) + j) * a.dim + d,
+                      load_row<T, V>(a, xs, p, p.len - (a.width - 1) + j, d));
   }
 }
 
-// The gradient of pre at row t (0 past the sequence's end), from the W rows up to t.
+// The gradient of pre at a row with gradient dy, from the W rows up to it.
 template <typename T, int V, int WT>
-__device__ __forceinline__ void pre_grad(float (&g)[V], const ConvArgs& a, const float (&w)[WT][V],
-                                         const float (&b)[V], const float (&win)[WT][V], const T* dys, long long t,
-                                         long long len) {
-  if (t >= len) {
+__device__ __forceinline__ void pre_grad(u64 (&g)[kPairs<V>], const ConvArgs& a, const u64 (&w)[WT][kPairs<V>],
+                                         const u64 (&b)[kPairs<V>], const u64 (&win)[WT][kPairs<V>],
+                                         const seq::Vec<T, V>& dy) {
+  constexpr int P = kPairs<V>;
+  to_pairs<T, V>(g, dy);
+  if (!a.silu) return;
+  u64 o[P];
+  taps<P, WT>(o, b, w, win, skipped<WT>(a));
 #pragma unroll
-    for (int i = 0; i < V; ++i) g[i] = 0.f;
-    return;
-  }
-  seq::load_vec<T, V>(g, dys + t * a.dim);
-  if (a.silu) {
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      float o = b[i];
-#pragma unroll
-      for (int k = 0; k < WT; ++k)
-        if (k >= WT - a.width) o = fmaf(w[k][i], win[k][i], o);
-      g[i] *= seq::dsilu(o);
-    }
+  for (int i = 0; i < P; ++i) {
+    float lo, hi;
+    unpack2(lo, hi, o[i]);
+    g[i] = seq::mul2(g[i], pack2(seq::dsilu(lo), seq::dsilu(hi)));
   }
 }
 
 // Rows [r0, r1) of a slot: dx of these rows, which needs g up to W - 1 rows further down, and the sums over these
-// rows of dw and dbias, written to partial[slot][W + 1][dim] for the reduction kernel.
+// rows of dw and dbias, written to partial[slot][W + 1][dim] for the reduction kernel. The weights are kept aligned to
+// the oldest tap too (wr), so that dx[t - (W-1)] = sum_j wr[j] g[t - j] has constant indices.
 template <typename T, int V, int WT>
-__global__ void __launch_bounds__(kConvThreads) conv_bwd_kernel(ConvArgs a) {
-  const int d = (blockIdx.y * kConvThreads + threadIdx.x) * V;
-  if (d >= a.dim) return;
-  const int W = a.width;
+__global__ void __launch_bounds__(kConvThreads, WT <= 4 ? 4 : 2) conv_bwd_kernel(ConvArgs a) {
+  constexpr int P = kPairs<V>;
+  __shared__ Weights<V, WT> sw;
+  const int d0 = blockIdx.y * kConvThreads * V, d = d0 + threadIdx.x * V;
+  const int W = WT <= 4 ? WT : a.width, skip = WT - W;
   float* part = a.partial + (long long)blockIdx.x * (W + 1) * a.dim + d;
   const Span p = seq::slot_span(a.rows, blockIdx.x, a.slot_rows);
+  if (p.len >= 0) stage_weights<V, WT>(sw, a, d0);
+  __syncthreads();
+  if (d >= a.dim) return;
   if (p.len < 0) {  // a slot of no sequence still has a place in the sums
     for (int k = 0; k <= W; ++k)
 #pragma unroll
@@ -156,109 +266,162 @@ __global__ void __launch_bounds__(kConvThreads) conv_bwd_kernel(ConvArgs a) {
   T* dxs = static_cast<T*>(a.dx) + row0 * a.dim + d;
   const long long r1 = min(p.r0 + a.slot_rows, p.len);
 
-  float w[WT][V], b[V], win[WT][V], gw[WT][V], dw[WT][V] = {}, db[V] = {};
-  load_weights<V, WT>(w, b, a, d);
+  u64 w[WT][P], b[P], win[WT][P], gw[WT][P], dw[WT][P], db[P];  // gw[WT-1-j]: g of j rows ago
+  own_weights<V, WT>(w, b, sw, skip);
 #pragma unroll
   for (int k = 0; k < WT; ++k)
 #pragma unroll
-    for (int i = 0; i < V; ++i) gw[k][i] = 0.f;
+    for (int i = 0; i < P; ++i) gw[k][i] = dw[k][i] = db[i] = 0;
 #pragma unroll
-  for (int k = 1; k < WT; ++k) load_row<T, V>(win[k], a, xs, p, p.r0 - WT + k, d);
-  if (p.r0 < r1) {
-    for (long long t = p.r0; t < r1 + W - 1; ++t) {
+  for (int k = 1; k < WT; ++k) to_pairs<T, V>(win[k], load_row<T, V>(a, xs, p, p.r0 - WT + k, d));
+  // Row t with its gradient of pre in gw[WT - 1]: the row whose gradient is complete now is t - (W-1).
+  auto finish = [&](long long t) {
+    const long long v = t - (W - 1);
+    u64 o[P];  // sum over taps j of w[j] g[t - j]
 #pragma unroll
-      for (int k = 0; k + 1 < WT; ++k)
+    for (int i = 0; i < P; ++i) o[i] = 0;
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          win[k][i] = win[k + 1][i];
-          gw[k][i] = gw[k + 1][i];  // gw[WT-1-j]: g of j rows ago
-        }
-      if (t < p.len) seq::load_vec<T, V>(win[WT - 1], xs + t * a.x_row);
-      pre_grad<T, V, WT>(gw[WT - 1], a, w, b, win, dys, t, p.len);
-      if (t < r1) {
+    for (int s = 0; s < WT; ++s)
+      if (s == skip) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-          db[i] += gw[WT - 1][i];
+        for (int j = 0; j + s < WT; ++j)
 #pragma unroll
-          for (int k = 0; k < WT; ++k)
-            if (k >= WT - W) dw[k][i] = fmaf(gw[WT - 1][i], win[k][i], dw[k][i]);
-        }
+          for (int i = 0; i < P; ++i) o[i] = fma2(w[j + s][i], gw[WT - 1 - j][i], o[i]);
       }
-      const long long u = t - (W - 1);  // the row whose gradient is complete now
-      if (u >= p.r0) {
-        float o[V];
+    if (t >= p.len && a.dfinal && v >= 0) {
+      u64 f[P];
+      to_pairs<T, V>(f, load_raw<T, V>(static_cast<const T*>(a.dfinal) +
+                                       ((long long)p.s * (W - 1) + t - p.len) * a.dim + d));
 #pragma unroll
-        for (int i = 0; i < V; ++i) o[i] = 0.f;
-        // dx[u] = sum over taps j = 0..W-1 of w[j] g[u + (W-1) - j] = w[j] g[t - j]
+      for (int i = 0; i < P; ++i) o[i] = seq::add2(o[i], f[i]);
+    }
+    if (v >= p.r0) store_raw<T, V>(dxs + v * a.dim, from_pairs<T, V>(o));
+  };
+  auto add_sums = [&]() {
 #pragma unroll
-        for (int j = 0; j < WT; ++j)
-          if (j < W) {
+    for (int i = 0; i < P; ++i) {
+      db[i] = seq::add2(db[i], gw[WT - 1][i]);
 #pragma unroll
-            for (int kk = 0; kk < WT; ++kk)
-              if (kk == j + WT - W)
+      for (int k = 0; k < WT; ++k)
+        if (k >= skip) dw[k][i] = fma2(gw[WT - 1][i], win[k][i], dw[k][i]);
+    }
+  };
+  seq::Vec<T, V> rx[kBwdGroup], rg[kBwdGroup];
+  long long t = p.r0;
+  // Whole groups of the slot's rows without conditions, so that the moving windows cost no moves.
+  for (; t + kBwdGroup <= r1; t += kBwdGroup) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) o[i] = fmaf(w[kk][i], gw[WT - 1 - j][i], o[i]);
-          }
-        if (a.dfinal && u >= p.len - (W - 1)) {
-          float f[V];
-          seq::load_vec<T, V>(f, static_cast<const T*>(a.dfinal) +
-                                     ((long long)p.s * (W - 1) + u - (p.len - (W - 1))) * a.dim + d);
+    for (int u = 0; u < kBwdGroup; ++u) {
+      rx[u] = load_raw<T, V>(xs + (t + u) * a.x_row);
+      rg[u] = load_raw<T, V>(dys + (t + u) * a.dim);
+    }
 #pragma unroll
-          for (int i = 0; i < V; ++i) o[i] += f[i];
-        }
-        seq::store_vec<T, V>(dxs + u * a.dim, o);
-      }
+    for (int u = 0; u < kBwdGroup; ++u) {
+      shift<P, WT>(win);
+      shift<P, WT>(gw);
+      to_pairs<T, V>(win[WT - 1], rx[u]);
+      pre_grad<T, V, WT>(gw[WT - 1], a, w, b, win, rg[u]);
+      add_sums();
+      finish(t + u);
     }
   }
-  for (int k = 0; k < W; ++k)
+  // The rows that are left, and the W - 1 below the slot whose gradients its last rows need (past the end: 0).
+  const long long end = p.r0 < r1 ? r1 + W - 1 : r1;
+  for (; t < end; t += kBwdGroup) {
 #pragma unroll
-    for (int kk = 0; kk < WT; ++kk)
-      if (kk == k + WT - W)
+    for (int u = 0; u < kBwdGroup; ++u)
+      if (t + u < end && t + u < p.len) {
+        rx[u] = load_raw<T, V>(xs + (t + u) * a.x_row);
+        rg[u] = load_raw<T, V>(dys + (t + u) * a.dim);
+      }
 #pragma unroll
-        for (int i = 0; i < V; ++i) part[(long long)k * a.dim + i] = dw[kk][i];
+    for (int u = 0; u < kBwdGroup; ++u)
+      if (t + u < end) {
+        shift<P, WT>(win);
+        shift<P, WT>(gw);
+        if (t + u < p.len) {
+          to_pairs<T, V>(win[WT - 1], rx[u]);
+          pre_grad<T, V, WT>(gw[WT - 1], a, w, b, win, rg[u]);
+        } else {
 #pragma unroll
-  for (int i = 0; i < V; ++i) part[(long long)W * a.dim + i] = db[i];
+          for (int i = 0; i < P; ++i) gw[WT - 1][i] = 0;
+        }
+        if (t + u < r1) add_sums();
+        finish(t + u);
+      }
+  }
+  auto put = [&](int k, const u64 (&v)[P]) {
+#pragma unroll
+    for (int i = 0; i < P; ++i) {
+      float lo, hi;
+      unpack2(lo, hi, v[i]);
+      part[(long long)k * a.dim + 2 * i] = lo;
+      if (2 * i + 1 < V) part[(long long)k * a.dim + 2 * i + 1] = hi;
+    }
+  };
+#pragma unroll
+  for (int k = 0; k < WT; ++k)
+    if (k >= skip) put(k - skip, dw[k]);
+  put(W, db);
 
-  // Gradient of the state before the sequence: virtual rows -(W-1) .. -1 under the first W - 1 rows.
+  // Gradient of the state before the sequence: virtual rows -(W-1) .. -1 under the first W - 1 rows. Row t reaches
+  // virtual row v by tap v + (W-1) - t, so each row's g is found once and added to those above it.
   if (a.dinit && p.r0 == 0) {
     T* di = static_cast<T*>(a.dinit) + (long long)p.s * (W - 1) * a.dim + d;
-    for (int j = 0; j < W - 1; ++j) {
-      float o[V];
+    u64 o[WT - 1][P];  // o[WT - 2 - j]: virtual row -1 - j
 #pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = 0.f;
-      const long long v = j - (W - 1);
-      for (long long t = 0; t <= v + W - 1 && t < p.len; ++t) {
-        float g[V], wn[WT][V];
+    for (int j = 0; j < WT - 1; ++j)
 #pragma unroll
-        for (int k = 0; k < WT; ++k) load_row<T, V>(wn[k], a, xs, p, t - (WT - 1) + k, d);
-        pre_grad<T, V, WT>(g, a, w, b, wn, dys, t, p.len);
-        const int tap = (int)(v + (W - 1) - t);
+      for (int i = 0; i < P; ++i) o[j][i] = 0;
 #pragma unroll
-        for (int kk = 0; kk < WT; ++kk)
-          if (kk == tap + WT - W)
+    for (int t = 0; t < WT - 1; ++t)
+      if (t < W - 1 && t < p.len) {
+        u64 g[P], wn[WT][P];
 #pragma unroll
-            for (int i = 0; i < V; ++i) o[i] = fmaf(w[kk][i], g[i], o[i]);
+        for (int k = 0; k < WT; ++k) to_pairs<T, V>(wn[k], load_row<T, V>(a, xs, p, t - (WT - 1) + k, d));
+        pre_grad<T, V, WT>(g, a, w, b, wn, load_raw<T, V>(dys + (long long)t * a.dim));
+        // wn[k] is virtual row t - (WT-1) + k, that is o[t + k] where it is below 0
+#pragma unroll
+        for (int k = 0; k + t < WT - 1; ++k)
+          if (k >= skip)
+#pragma unroll
+            for (int i = 0; i < P; ++i) o[t + k][i] = fma2(w[k][i], g[i], o[t + k][i]);
       }
-      // A sequence shorter than the state passes part of it on to the final state.
-      const long long f0 = v - (p.len - (W - 1));
-      if (a.dfinal && f0 >= 0) {
-        float f[V];
-        seq::load_vec<T, V>(f, static_cast<const T*>(a.dfinal) + ((long long)p.s * (W - 1) + f0) * a.dim + d);
 #pragma unroll
-        for (int i = 0; i < V; ++i) o[i] += f[i];
+    for (int j = 0; j < WT - 1; ++j)
+      if (j >= skip) {
+        const int v = j - (WT - 1);  // -(W-1) .. -1
+        // A sequence shorter than the state passes part of it on to the final state.
+        const long long f0 = v - (p.len - (W - 1));
+        if (a.dfinal && f0 >= 0) {
+          u64 f[P];
+          to_pairs<T, V>(f, load_raw<T, V>(static_cast<const T*>(a.dfinal) +
+                                           ((long long)p.s * (W - 1) + f0) * a.dim + d));
+#pragma unroll
+          for (int i = 0; i < P; ++i) o[j][i] = seq::add2(o[j][i], f[i]);
+        }
+        store_raw<T, V>(di + (long long)(j - skip) * a.dim, from_pairs<T, V>(o[j]));
       }
-      seq::store_vec<T, V>(di + (long long)j * a.dim, o);
-    }
   }
 }
 
-// Sums partial[slots][W + 1][dim] over the slots in order: dweight [dim, W] and dbias [dim].
-__global__ void conv_bwd_reduce_kernel(const float* partial, long long slots, int dim, int W, int w_dtype,
-                                       void* dweight, void* dbias) {
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= (long long)(W + 1) * dim) return;
+// Sums partial[slots][W + 1][dim] over the slots: dweight [dim, W] and dbias [dim]. A warp has 32 values and each of
+// the block's 8 warps every eighth slot; the order is fixed.
+__global__ void __launch_bounds__(256) conv_bwd_reduce_kernel(const float* partial, long long slots, int dim, int W,
+                                                              int w_dtype, void* dweight, void* dbias) {
+  __shared__ float sums[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const long long n = (long long)(W + 1) * dim, i = (long long)blockIdx.x * 32 + lane;
   float s = 0.f;
-  for (long long j = 0; j < slots; ++j) s += partial[j * (W + 1) * dim + i];
+  if (i < n) {
+#pragma unroll 8
+    for (long long j = warp; j < slots; j += 8) s += partial[j * n + i];
+  }
+  sums[warp][lane] = s;
+  __syncthreads();
+  if (warp != 0 || i >= n) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) s += sums[w][lane];
   const int k = (int)(i / dim), d = (int)(i % dim);
   if (k < W) seq::store_param(dweight, (long long)d * W + k, w_dtype, s);
   else if (dbias) seq::store_param(dbias, d, w_dtype, s);
@@ -267,37 +430,43 @@ __global__ void conv_bwd_reduce_kernel(const float* partial, long long slots, in
 template <typename T, int V, int WT>
 __global__ void __launch_bounds__(kConvThreads) conv_update_kernel(ConvArgs a, T* pool, const int32_t* idx,
                                                                    int n_slots) {
+  constexpr int P = kPairs<V>;
   const int d = (blockIdx.y * kConvThreads + threadIdx.x) * V;
   if (d >= a.dim) return;
-  const int row = blockIdx.x, W = a.width;
+  const int row = blockIdx.x, W = WT <= 4 ? WT : a.width, skip = WT - W;
   T* yp = static_cast<T*>(a.y) + (long long)row * a.dim + d;
   const int slot = idx ? idx[row] : row;
-  float o[V];
+  u64 o[P];
   if (slot < 0 || slot >= n_slots) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = 0.f;
-    seq::store_vec<T, V>(yp, o);
+    for (int i = 0; i < P; ++i) o[i] = 0;
+    store_raw<T, V>(yp, from_pairs<T, V>(o));
     return;
   }
   T* st = pool + (long long)slot * (W - 1) * a.dim + d;
-  float w[WT][V], win[WT][V];
-  load_weights<V, WT>(w, o, a, d);
-  seq::load_vec<T, V>(win[WT - 1], static_cast<const T*>(a.x) + (long long)row * a.x_row + d);
+  u64 w[WT][P], b[P], win[WT][P];
+  seq::Vec<T, V> raw[WT];
+  raw[WT - 1] = load_raw<T, V>(static_cast<const T*>(a.x) + (long long)row * a.x_row + d);
 #pragma unroll
   for (int k = 0; k + 1 < WT; ++k)
-    if (k >= WT - W) seq::load_vec<T, V>(win[k], st + (long long)(k - (WT - W)) * a.dim);
+    if (k >= skip) raw[k] = load_raw<T, V>(st + (long long)(k - skip) * a.dim);
+  load_weights<V, WT>(w, b, a, d);
 #pragma unroll
   for (int k = 0; k < WT; ++k)
-    if (k >= WT - W) {
+    if (k >= skip) to_pairs<T, V>(win[k], raw[k]);
+  taps<P, WT>(o, b, w, win, skip);
 #pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = fmaf(w[k][i], win[k][i], o[i]);
-      if (k > WT - W) seq::store_vec<T, V>(st + (long long)(k - 1 - (WT - W)) * a.dim, win[k]);
-    }
+  for (int k = 1; k < WT; ++k)
+    if (k > skip) store_raw<T, V>(st + (long long)(k - 1 - skip) * a.dim, raw[k]);
   if (a.silu) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = seq::silu(o[i]);
+    for (int i = 0; i < P; ++i) {
+      float lo, hi;
+      unpack2(lo, hi, o[i]);
+      o[i] = pack2(seq::silu(lo), seq::silu(hi));
+    }
   }
-  seq::store_vec<T, V>(yp, o);
+  store_raw<T, V>(yp, from_pairs<T, V>(o));
 }
 
 bool valid(const sf_causal_conv1d_desc* d) {
@@ -305,12 +474,11 @@ bool valid(const sf_causal_conv1d_desc* d) {
          dtype_size(d->dtype) != 0 && dtype_size(d->w_dtype) != 0;
 }
 
-// Channels per thread: a 16-byte vector where every row of every tensor begins on one, else one channel.
-template <typename T>
-bool vectors_fit(int V, const sf_causal_conv1d_desc* d, bool packed, std::initializer_list<const void*> ptrs) {
-  if (d->dim % V || d->x_row_stride % V || (!packed && d->n_seq > 1 && d->x_batch_stride % V)) return false;
+// Whether every row of every tensor begins where a vector of V channels can be read; else a thread has one channel.
+bool vectors_fit(int V, const sf_causal_conv1d_desc* d, bool batched, std::initializer_list<const void*> ptrs) {
+  if (d->dim % V || d->x_row_stride % V || (batched && d->n_seq > 1 && d->x_batch_stride % V)) return false;
   for (const void* p : ptrs)
-    if (reinterpret_cast<uintptr_t>(p) % (V * sizeof(T))) return false;
+    if (reinterpret_cast<uintptr_t>(p) % (V * dtype_size(d->dtype))) return false;
   return true;
 }
 
@@ -333,31 +501,36 @@ ConvArgs base_args(const void* x, const void* weight, const void* bias, const vo
 
 int channel_blocks(int dim, int V) { return (dim + V * kConvThreads - 1) / (V * kConvThreads); }
 
-constexpr long long kFwdRows = 32, kBwdRows = 64;
+// Rows per slot: as many as leave `want` blocks (the W - 1 rows above a slot are read again, and in the backward pass
+// its sums are written and read), between 8 and `most`.
+long long slot_rows(const sf_causal_conv1d_desc* d, int V, long long want, long long most) {
+  const long long across = channel_blocks(d->dim, V);
+  long long rows = most;
+  while (rows > 8 && seq::total_slots(d->length, d->n_seq, d->packed, rows) * across < want) rows /= 2;
+  return rows;
+}
+// Vector widths (bytes): 16 forward; 8 backward and above 4 taps, whose windows would not fit the registers.
+int fwd_vec(const sf_causal_conv1d_desc* d) { return (d->width <= 4 ? 16 : 8) / (int)dtype_size(d->dtype); }
+int bwd_vec(const sf_causal_conv1d_desc* d) { return 8 / (int)dtype_size(d->dtype); }
+long long fwd_rows(const sf_causal_conv1d_desc* d) { return slot_rows(d, fwd_vec(d), 148 * 6, 64); }
+long long bwd_rows(const sf_causal_conv1d_desc* d) { return slot_rows(d, bwd_vec(d), 148 * 6, 128); }
 
-template <typename T, int V>
-sf_status run_fwd(const ConvArgs& a, cudaStream_t st) {
-  const dim3 grid((unsigned)seq::total_slots(a.rows.length, a.rows.n_seq, a.rows.offsets != nullptr, a.slot_rows), channel_blocks(a.dim, V));
-  if (a.width <= 4) conv_fwd_kernel<T, V, 4><<<grid, kConvThreads, 0, st>>>(a);
-  else conv_fwd_kernel<T, V, 8><<<grid, kConvThreads, 0, st>>>(a);
+template <typename T, int V, int WT>
+sf_status run_fwd(const ConvArgs& a, dim3 grid, cudaStream_t st) {
+  grid.y = channel_blocks(a.dim, V);
+  conv_fwd_kernel<T, V, WT><<<grid, kConvThreads, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
 }
-template <typename T, int V>
-sf_status run_bwd(const ConvArgs& a, void* dweight, void* dbias, cudaStream_t st) {
-  const long long slots = seq::total_slots(a.rows.length, a.rows.n_seq, a.rows.offsets != nullptr, a.slot_rows);
-  const dim3 grid((unsigned)slots, channel_blocks(a.dim, V));
-  if (a.width <= 4) conv_bwd_kernel<T, V, 4><<<grid, kConvThreads, 0, st>>>(a);
-  else conv_bwd_kernel<T, V, 8><<<grid, kConvThreads, 0, st>>>(a);
-  const long long n = (long long)(a.width + 1) * a.dim;
-  conv_bwd_reduce_kernel<<<(unsigned)((n + 127) / 128), 128, 0, st>>>(a.partial, slots, a.dim, a.width, a.w_dtype,
-                                                                      dweight, dbias);
+template <typename T, int V, int WT>
+sf_status run_bwd(const ConvArgs& a, dim3 grid, cudaStream_t st) {
+  grid.y = channel_blocks(a.dim, V);
+  conv_bwd_kernel<T, V, WT><<<grid, kConvThreads, 0, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
 }
-template <typename T, int V>
-sf_status run_update(const ConvArgs& a, void* pool, const int32_t* idx, int n_slots, cudaStream_t st) {
-  const dim3 grid(a.rows.n_seq, channel_blocks(a.dim, V));
-  if (a.width <= 4) conv_update_kernel<T, V, 4><<<grid, kConvThreads, 0, st>>>(a, static_cast<T*>(pool), idx, n_slots);
-  else conv_update_kernel<T, V, 8><<<grid, kConvThreads, 0, st>>>(a, static_cast<T*>(pool), idx, n_slots);
+template <typename T, int V, int WT>
+sf_status run_update(const ConvArgs& a, dim3 grid, void* pool, const int32_t* idx, int n_slots, cudaStream_t st) {
+  grid.y = channel_blocks(a.dim, V);
+  conv_update_kernel<T, V, WT><<<grid, kConvThreads, 0, st>>>(a, static_cast<T*>(pool), idx, n_slots);
   return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
 }
 
@@ -366,26 +539,24 @@ sf_status run_update(const ConvArgs& a, void* pool, const int32_t* idx, int n_sl
 
 using namespace sf;
 
-// f(type tag, vector width) for the data type: `fits` says whether 16-byte vectors do.
-#define SF_SEQ_DISPATCH(DTYPE, FITS, CALL)                                                 \
-  switch (DTYPE) {                                                                         \
-    case SF_DTYPE_F32: {                                                                   \
-      using T = float;                                                                     \
-      if (FITS(4)) { constexpr int V = 4; return CALL; }                                   \
-      constexpr int V = 1; return CALL;                                                    \
-    }                                                                                      \
-    case SF_DTYPE_F16: {                                                                   \
-      using T = __half;                                                                    \
-      if (FITS(8)) { constexpr int V = 8; return CALL; }                                   \
-      constexpr int V = 1; return CALL;                                                    \
-    }                                                                                      \
-    case SF_DTYPE_BF16: {                                                                  \
-      using T = __nv_bfloat16;                                                             \
-      if (FITS(8)) { constexpr int V = 8; return CALL; }                                   \
-      constexpr int V = 1; return CALL;                                                    \
-    }                                                                                      \
-  }                                                                                        \
-  return SF_ERR_INVALID_ARG
+// CALL<T, V, WT> for the data type, with `BYTES` of channels a thread where `fit` (else one channel), 2, 3, 4 taps or up to 8.
+#define SF_CONV_TYPE(TYPE, BYTES4, BYTES8, CALL, ...)                                        \
+  {                                                                                          \
+    using T = TYPE;                                                                          \
+    constexpr int V4 = BYTES4 / (int)sizeof(T), V8 = BYTES8 / (int)sizeof(T);                \
+    switch (d->width) {                                                                      \
+      case 2: return fit ? CALL<T, V4, 2>(__VA_ARGS__) : CALL<T, 1, 2>(__VA_ARGS__);         \
+      case 3: return fit ? CALL<T, V4, 3>(__VA_ARGS__) : CALL<T, 1, 3>(__VA_ARGS__);         \
+      case 4: return fit ? CALL<T, V4, 4>(__VA_ARGS__) : CALL<T, 1, 4>(__VA_ARGS__);         \
+      default: return fit ? CALL<T, V8, 8>(__VA_ARGS__) : CALL<T, 1, 8>(__VA_ARGS__);        \
+    }                                                                                        \
+  }
+#define SF_CONV_DISPATCH(BYTES4, BYTES8, CALL, ...)                                          \
+  switch (d->dtype) {                                                                        \
+    case SF_DTYPE_F32: SF_CONV_TYPE(float, BYTES4, BYTES8, CALL, __VA_ARGS__)                \
+    case SF_DTYPE_F16: SF_CONV_TYPE(__half, BYTES4, BYTES8, CALL, __VA_ARGS__)               \
+    default: SF_CONV_TYPE(__nv_bfloat16, BYTES4, BYTES8, CALL, __VA_ARGS__)                  \
+  }
 
 extern "C" sf_status sf_causal_conv1d(const void* x, const void* weight, const void* bias, const void* initial_state,
                                       const int32_t* seq_offsets, void* y, void* final_state,
@@ -397,18 +568,24 @@ extern "C" sf_status sf_causal_conv1d(const void* x, const void* weight, const v
   ConvArgs a = base_args(x, weight, bias, initial_state, seq_offsets, d);
   a.y = y;
   a.final_state = final_state;
-  a.slot_rows = kFwdRows;
-  if (seq::total_slots(a.rows.length, a.rows.n_seq, a.rows.offsets != nullptr, a.slot_rows) > INT32_MAX) return SF_ERR_UNSUPPORTED;
+  const bool fit = vectors_fit(fwd_vec(d), d, !d->packed, {x, initial_state, y, final_state});
+  a.slot_rows = fwd_rows(d);
+  const long long slots = seq::total_slots(d->length, d->n_seq, d->packed, a.slot_rows);
+  if (slots > INT32_MAX) return SF_ERR_UNSUPPORTED;
+  const dim3 grid((unsigned)slots);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define FITS(n) vectors_fit<T>(n, d, seq_offsets != nullptr, {x, initial_state, y, final_state})
-  SF_SEQ_DISPATCH(d->dtype, FITS, (run_fwd<T, V>(a, st)));
-#undef FITS
+  SF_CONV_DISPATCH(16, 8, run_fwd, a, grid, st)
 }
 
 extern "C" size_t sf_causal_conv1d_backward_workspace_size(const sf_causal_conv1d_desc* d) {
   if (!valid(d)) return 0;
-  return (size_t)seq::total_slots(d->length, d->n_seq, d->packed, kBwdRows) * (d->width + 1) * d->dim *
+  return (size_t)seq::total_slots(d->length, d->n_seq, d->packed, bwd_rows(d)) * (d->width + 1) * d->dim *
          sizeof(float);
+}
+
+static sf_status conv_backward(const ConvArgs& a, const sf_causal_conv1d_desc* d, bool fit, dim3 grid,
+                               cudaStream_t st) {
+  SF_CONV_DISPATCH(8, 8, run_bwd, a, grid, st)
 }
 
 extern "C" sf_status sf_causal_conv1d_backward(const void* x, const void* weight, const void* bias,
@@ -423,25 +600,28 @@ extern "C" sf_status sf_causal_conv1d_backward(const void* x, const void* weight
   if (bias && !dbias) return SF_ERR_INVALID_ARG;
   if (d->n_seq > 0 && (!workspace || workspace_bytes < sf_causal_conv1d_backward_workspace_size(d)))
     return SF_ERR_WORKSPACE;
-  if (d->n_seq > 0 && (reinterpret_cast<uintptr_t>(workspace) & 15u)) return SF_ERR_ALIGNMENT;
+  if (d->n_seq > 0 && !aligned16(workspace)) return SF_ERR_ALIGNMENT;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (d->n_seq == 0) {  // no rows: the sums are 0
-    const long long n = (long long)(d->width + 1) * d->dim;
-    conv_bwd_reduce_kernel<<<(unsigned)((n + 127) / 128), 128, 0, st>>>(nullptr, 0, d->dim, d->width, d->w_dtype,
-                                                                        dweight, dbias);
-    return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
-  }
   ConvArgs a = base_args(x, weight, bias, initial_state, seq_offsets, d);
-  a.dy = dy;
-  a.dfinal = d_final_state;
-  a.dx = dx;
-  a.dinit = d_initial_state;
-  a.partial = static_cast<float*>(workspace);
-  a.slot_rows = kBwdRows;
-  if (seq::total_slots(a.rows.length, a.rows.n_seq, a.rows.offsets != nullptr, a.slot_rows) > INT32_MAX) return SF_ERR_UNSUPPORTED;
-#define FITS(n) vectors_fit<T>(n, d, seq_offsets != nullptr, {x, initial_state, dy, d_final_state, dx, d_initial_state})
-  SF_SEQ_DISPATCH(d->dtype, FITS, (run_bwd<T, V>(a, dweight, bias ? dbias : nullptr, st)));
-#undef FITS
+  long long slots = 0;  // without sequences the sums are 0
+  if (d->n_seq > 0) {
+    a.dy = dy;
+    a.dfinal = d_final_state;
+    a.dx = dx;
+    a.dinit = d_initial_state;
+    a.partial = static_cast<float*>(workspace);
+    a.slot_rows = bwd_rows(d);
+    slots = seq::total_slots(d->length, d->n_seq, d->packed, a.slot_rows);
+    if (slots > INT32_MAX) return SF_ERR_UNSUPPORTED;
+    const bool fit = vectors_fit(bwd_vec(d), d, !d->packed,
+                                 {x, initial_state, dy, d_final_state, dx, d_initial_state});
+    const sf_status s = conv_backward(a, d, fit, dim3((unsigned)slots), st);
+    if (s != SF_OK) return s;
+  }
+  const long long n = (long long)(d->width + 1) * d->dim;
+  conv_bwd_reduce_kernel<<<(unsigned)((n + 31) / 32), 256, 0, st>>>(a.partial, slots, d->dim, d->width, d->w_dtype,
+                                                                    dweight, bias ? dbias : nullptr);
+  return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
 }
 
 extern "C" sf_status sf_causal_conv1d_update(const void* x, void* state_pool, const void* weight, const void* bias,
@@ -452,8 +632,8 @@ extern "C" sf_status sf_causal_conv1d_update(const void* x, void* state_pool, co
   if (!x || !y || !state_pool) return SF_ERR_INVALID_ARG;
   ConvArgs a = base_args(x, weight, bias, nullptr, nullptr, d);
   a.y = y;
+  const bool fit = vectors_fit(bwd_vec(d), d, false, {x, state_pool, y});
+  const dim3 grid(d->n_seq);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define FITS(n) vectors_fit<T>(n, d, true, {x, state_pool, y})
-  SF_SEQ_DISPATCH(d->dtype, FITS, (run_update<T, V>(a, state_pool, state_indices, n_slots, st)));
-#undef FITS
+  SF_CONV_DISPATCH(8, 8, run_update, a, grid, state_pool, state_indices, n_slots, st)
 }

@@ -48,7 +48,8 @@ __global__ void __launch_bounds__(kThreads) scan_update_kernel(ScanArgs a, float
     const int g = d / (a.dim / a.groups);
     float dt = DT<T>::to_f(static_cast<const T*>(a.dt)[(long long)row * a.dt_row + d]);
     if (a.dt_bias) dt += a.dt_bias[d];
-    if (a.softplus) dt = seq::softplus(dt);
+    float e;
+    if (a.softplus) dt = softplus(dt, e);
     const float x = DT<T>::to_f(static_cast<const T*>(a.x)[(long long)row * a.x_row + d]);
     const T* Bp = static_cast<const T*>(a.B) + (long long)row * a.b_row + (long long)g * a.state;
     const T* Cp = static_cast<const T*>(a.C) + (long long)row * a.c_row + (long long)g * a.state;

@@ -32,7 +32,7 @@ namespace sf {
 
 using seq::Rows;
 using seq::Span;
-typedef unsigned long long u64;
+using seq::u64;
 
 constexpr int kThreads = 128;  // of the single-token kernel
 constexpr int kS = 4;          // states per lane
@@ -41,7 +41,7 @@ constexpr int kRows = 16;      // rows per tile, and per checkpoint
 constexpr int kHalf = 8;       // rows between two additions over the warps in the backward pass
 constexpr int kCpt = 2;        // channels per lane
 constexpr int kPart = 4;       // rows whose states the backward pass keeps in registers
-constexpr float kLog2e = 1.4426950408889634f;
+using seq::kLog2e;
 
 struct ScanArgs {
   const void *x, *dt, *B, *C, *z, *dy;
@@ -67,67 +67,13 @@ sf_status scan_backward(const ScanArgs& a, int lanes, bool vec, dim3 grid, cudaS
 
 namespace {
 
-__device__ __forceinline__ float ex2(float v) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
-// Pairs of fp32: each half is rounded like the scalar operation.
-__device__ __forceinline__ u64 pack2(float lo, float hi) {
-  u64 r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpack2(float& lo, float& hi, u64 v) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ u64 mul2(u64 a, u64 b) {
-  u64 r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ u64 fma2(u64 a, u64 b, u64 c) {
-  u64 r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ u64 add2(u64 a, u64 b) {
-  u64 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ float sum2(u64 a) {
-  float lo, hi;
-  unpack2(lo, hi, a);
-  return lo + hi;
-}
-__device__ __forceinline__ float rcp(float v) {
-  float r;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
-  return r;
-}
+using namespace seq;
+
 __device__ __forceinline__ u64 ex2x2(u64 v) {
   float lo, hi;
   unpack2(lo, hi, v);
   return pack2(ex2(lo), ex2(hi));
 }
-
-// softplus(v) = max(v, 0) + log(1 + e) with e = exp(-|v|), which is returned too. log(1 + e) = 2 atanh(s), s = e / (2 + e)
-// <= 1/3, is odd in s: s times a polynomial of degree 4 in s^2, fitted by weighted least squares to a relative error
-// of 8e-9 (of fp32 coefficients) over [0, 1/9]. Small e keep all their digits (a time step of 1e-3 is e = 1e-3), which
-// log(1 + e) from a logarithm would not. (Scalar: pairs would need a move for every coefficient.)
-__device__ __forceinline__ float softplus(float v, float& e) {
-  e = ex2(-kLog2e * fabsf(v));
-  const float s = e * rcp(2.f + e), q = s * s;
-  float c = 0.28178343176841736f;
-  c = fmaf(c, q, 0.27960601449012756f);
-  c = fmaf(c, q, 0.40024909377098083f);
-  c = fmaf(c, q, 0.6666631698608398f);
-  c = fmaf(c, q, 2.f);
-  return fmaf(s, c, fmaxf(v, 0.f));
-}
-// 1 / (1 + exp(-v))
-__device__ __forceinline__ float logistic(float v) { return rcp(1.f + ex2(-kLog2e * v)); }
 
 template <typename T>
 __device__ __forceinline__ const T* at(const void* p, const ScanArgs& a, const Span& s, long long batch,
