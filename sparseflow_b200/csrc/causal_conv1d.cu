@@ -7,9 +7,9 @@
 //
 // About W + 9 instructions an element forward against 2 |x| bytes, 3 W + 15 backward against 3 |x|: HBM-bound, if
 // enough bytes are on their way. A thread owns V neighbouring channels (8 or 16 bytes of a row, so a warp reads whole
-// sectors) and walks down a slot of rows with the last W rows in registers; the rows of a group (kGroup) are loaded
-// together before the first of them is used. Every x is read once, but for the W - 1 rows above each slot, which come
-// from L2. Products and sums are pairs of fp32 (mul/fma .f32x2).
+// sectors) and walks down a slot of rows with the last W rows in registers. The rows ahead are copied asynchronously
+// to a ring in shared memory, each thread its own, so no barrier guards it. Every x is read once, but for the W - 1
+// rows above each slot, which come from L2. Products and sums are pairs of fp32 (mul/fma .f32x2).
 #include "sequence.cuh"
 
 namespace sf {
@@ -24,7 +24,8 @@ using seq::unpack2;
 
 constexpr int kConvThreads = 128;
 constexpr int kMaxWidth = 8;
-constexpr int kFwdGroup = 8, kBwdGroup = 4;  // rows loaded together
+constexpr int kFwdGroup = 8, kBwdGroup = 4;  // rows copied together
+constexpr int kFwdStages = 3, kBwdStages = 4;  // groups in the ring
 
 struct ConvArgs {
   const void *x, *weight, *bias, *init, *dy, *dfinal;
@@ -65,6 +66,14 @@ template <typename T, int V>
 __device__ __forceinline__ void store_raw(T* p, const seq::Vec<T, V>& v) {
   *reinterpret_cast<seq::Vec<T, V>*>(p) = v;
 }
+
+// A thread's rows on their way: groups of G rows of N arrays. Single 16-bit channels, which no copy fits, are read when
+// they are needed.
+template <typename T, int V, int N, int G, int STAGES>
+struct Ring {
+  static constexpr bool ASYNC = V * sizeof(T) >= 4;
+  seq::Vec<T, V> v[ASYNC ? STAGES : 1][N][G][kConvThreads];
+};
 
 // Row `t` of the sequence (t < 0: of the state before it; rows above that are 0).
 template <typename T, int V>
@@ -161,32 +170,52 @@ __device__ __forceinline__ void shift(u64 (&row)[WT][P]) {
     for (int i = 0; i < P; ++i) row[k][i] = row[k + 1][i];
 }
 
-template <typename T, int V, int WT>
+template <typename T, int V, int WT, bool SILU>
 __global__ void __launch_bounds__(kConvThreads, WT <= 4 ? 4 : 2) conv_fwd_kernel(ConvArgs a) {
-  constexpr int P = kPairs<V>;
-  __shared__ Weights<V, WT> sw;
+  constexpr int P = kPairs<V>, G = kFwdGroup;
+  using R = Ring<T, V, 1, G, kFwdStages>;
+  extern __shared__ __align__(16) char smem[];
+  R& ring = *reinterpret_cast<R*>(smem);
+  Weights<V, WT>& sw = *reinterpret_cast<Weights<V, WT>*>(smem + sizeof(R));
   const int d0 = blockIdx.y * kConvThreads * V, d = d0 + threadIdx.x * V;
   const Span p = seq::slot_span(a.rows, blockIdx.x, a.slot_rows);
   if (p.len < 0) return;
+  const T* xs = seq_x<T>(a, p, d);
+  const long long r1 = min(p.r0 + a.slot_rows, p.len);
+  const T* px = xs + p.r0 * a.x_row;  // the next group to copy
+  long long tl = p.r0;
+  int put = 0, get = 0;
+  auto load = [&]() {
+    if (d < a.dim) {
+#pragma unroll
+      for (int u = 0; u < G; ++u) {
+        if (tl + u >= r1) break;
+        if constexpr (R::ASYNC) seq::cp_async(&ring.v[put][0][u][threadIdx.x], px + u * a.x_row, V * sizeof(T), true);
+      }
+    }
+    tl += G;
+    px += G * a.x_row;
+    seq::cp_async_commit();
+    put = put + 1 == kFwdStages ? 0 : put + 1;
+  };
+  if constexpr (R::ASYNC)
+    for (int i = 0; i < kFwdStages - 1; ++i) load();
   stage_weights<V, WT>(sw, a, d0);
   __syncthreads();
   if (d >= a.dim) return;
-  const T* xs = seq_x<T>(a, p, d);
-  const long long r1 = min(p.r0 + a.slot_rows, p.len);
   const int skip = skipped<WT>(a);
 
   u64 w[WT][P], b[P], win[WT][P];  // win[WT-1]: the newest row
   own_weights<V, WT>(w, b, sw, skip);
 #pragma unroll
   for (int k = 1; k < WT; ++k) to_pairs<T, V>(win[k], load_row<T, V>(a, xs, p, p.r0 - WT + k, d));
-  const T* px = xs + p.r0 * a.x_row;
   T* py = static_cast<T*>(a.y) + (seq_row0(a, p) + p.r0) * a.dim + d;
   auto one = [&](const seq::Vec<T, V>& x, T* y) {
     shift<P, WT>(win);
     to_pairs<T, V>(win[WT - 1], x);
     u64 o[P];
     taps<P, WT>(o, b, w, win, skip);
-    if (a.silu) {
+    if (SILU) {
 #pragma unroll
       for (int i = 0; i < P; ++i) {
         float lo, hi;
@@ -196,24 +225,28 @@ __global__ void __launch_bounds__(kConvThreads, WT <= 4 ? 4 : 2) conv_fwd_kernel
     }
     store_raw<T, V>(y, from_pairs<T, V>(o));
   };
-  seq::Vec<T, V> raw[kFwdGroup];
-  long long t = p.r0;
   // Whole groups without conditions, so that the moving window costs no moves, then the rows that are left.
-  for (; t + kFwdGroup <= r1; t += kFwdGroup) {
+  for (long long t = p.r0; t < r1; t += G) {
+    if constexpr (R::ASYNC) {
+      seq::cp_async_wait<kFwdStages - 2>();
+    } else {
 #pragma unroll
-    for (int u = 0; u < kFwdGroup; ++u) raw[u] = load_raw<T, V>(px + u * a.x_row);
+      for (int u = 0; u < G; ++u)
+        if (t + u < r1) ring.v[0][0][u][threadIdx.x] = load_raw<T, V>(xs + (t + u) * a.x_row);
+    }
+    if (t + G <= r1) {
 #pragma unroll
-    for (int u = 0; u < kFwdGroup; ++u) one(raw[u], py + (long long)u * a.dim);
-    px += kFwdGroup * a.x_row;
-    py += (long long)kFwdGroup * a.dim;
-  }
-  if (t < r1) {
+      for (int u = 0; u < G; ++u) one(ring.v[get][0][u][threadIdx.x], py + (long long)u * a.dim);
+    } else {
 #pragma unroll
-    for (int u = 0; u < kFwdGroup; ++u)
-      if (t + u < r1) raw[u] = load_raw<T, V>(px + u * a.x_row);
-#pragma unroll
-    for (int u = 0; u < kFwdGroup; ++u)
-      if (t + u < r1) one(raw[u], py + (long long)u * a.dim);
+      for (int u = 0; u < G; ++u)
+        if (t + u < r1) one(ring.v[get][0][u][threadIdx.x], py + (long long)u * a.dim);
+    }
+    py += (long long)G * a.dim;
+    if constexpr (R::ASYNC) {
+      get = get + 1 == kFwdStages ? 0 : get + 1;
+      load();
+    }
   }
   if (a.final_state && p.r0 == 0) {
     for (int j = 0; j < a.width - 1; ++j)
@@ -223,13 +256,13 @@ __global__ void __launch_bounds__(kConvThreads, WT <= 4 ? 4 : 2) conv_fwd_kernel
 }
 
 // The gradient of pre at a row with gradient dy, from the W rows up to it.
-template <typename T, int V, int WT>
+template <typename T, int V, int WT, bool SILU>
 __device__ __forceinline__ void pre_grad(u64 (&g)[kPairs<V>], const ConvArgs& a, const u64 (&w)[WT][kPairs<V>],
                                          const u64 (&b)[kPairs<V>], const u64 (&win)[WT][kPairs<V>],
                                          const seq::Vec<T, V>& dy) {
   constexpr int P = kPairs<V>;
   to_pairs<T, V>(g, dy);
-  if (!a.silu) return;
+  if (!SILU) return;
   u64 o[P];
   taps<P, WT>(o, b, w, win, skipped<WT>(a));
 #pragma unroll
@@ -243,10 +276,13 @@ __device__ __forceinline__ void pre_grad(u64 (&g)[kPairs<V>], const ConvArgs& a,
 // Rows [r0, r1) of a slot: dx of these rows, which needs g up to W - 1 rows further down, and the sums over these
 // rows of dw and dbias, written to partial[slot][W + 1][dim] for the reduction kernel. The weights are kept aligned to
 // the oldest tap too (wr), so that dx[t - (W-1)] = sum_j wr[j] g[t - j] has constant indices.
-template <typename T, int V, int WT>
+template <typename T, int V, int WT, bool SILU>
 __global__ void __launch_bounds__(kConvThreads, WT <= 4 ? 4 : 2) conv_bwd_kernel(ConvArgs a) {
-  constexpr int P = kPairs<V>;
-  __shared__ Weights<V, WT> sw;
+  constexpr int P = kPairs<V>, G = kBwdGroup;
+  using R = Ring<T, V, 2, G, kBwdStages>;
+  extern __shared__ __align__(16) char smem[];
+  R& ring = *reinterpret_cast<R*>(smem);
+  Weights<V, WT>& sw = *reinterpret_cast<Weights<V, WT>*>(smem + sizeof(R));
   const int d0 = blockIdx.y * kConvThreads * V, d = d0 + threadIdx.x * V;
   const int W = WT <= 4 ? WT : a.width, skip = WT - W;
   float* part = a.partial + (long long)blockIdx.x * (W + 1) * a.dim + d;
@@ -274,10 +310,31 @@ __global__ void __launch_bounds__(kConvThreads, WT <= 4 ? 4 : 2) conv_bwd_kernel
     for (int i = 0; i < P; ++i) gw[k][i] = dw[k][i] = db[i] = 0;
 #pragma unroll
   for (int k = 1; k < WT; ++k) to_pairs<T, V>(win[k], load_row<T, V>(a, xs, p, p.r0 - WT + k, d));
-  // Row t with its gradient of pre in gw[WT - 1]: the row whose gradient is complete now is t - (W-1).
-  auto finish = [&](long long t) {
-    const long long v = t - (W - 1);
-    u64 o[P];  // sum over taps j of w[j] g[t - j]
+  const long long end = p.r0 < r1 ? r1 + W - 1 : r1;  // the slot's rows, and those whose gradients its last ones need
+  const long long in = min(end, p.len);               // those that there are
+  const T *px = xs + p.r0 * a.x_row, *pg = dys + p.r0 * a.dim;  // the next group to copy
+  T* po = dxs + (p.r0 - (W - 1)) * a.dim;                       // where the gradient that row t completes goes
+  long long tl = p.r0;
+  int put_at = 0, get = 0;
+  auto load = [&]() {
+    if constexpr (R::ASYNC) {
+#pragma unroll
+      for (int u = 0; u < G; ++u) {
+        if (tl + u >= in) break;
+        seq::cp_async(&ring.v[put_at][0][u][threadIdx.x], px + u * a.x_row, V * sizeof(T), true);
+        seq::cp_async(&ring.v[put_at][1][u][threadIdx.x], pg + (long long)u * a.dim, V * sizeof(T), true);
+      }
+      seq::cp_async_commit();
+      put_at = put_at + 1 == kBwdStages ? 0 : put_at + 1;
+      tl += G;
+      px += G * a.x_row;
+      pg += (long long)G * a.dim;
+    }
+  };
+  for (int i = 0; i < kBwdStages - 1; ++i) load();
+
+  // dx of row t - (W-1), which g of row t (in gw[WT - 1]) completes: sum over taps j of w[j] g[t - j].
+  auto dx_row = [&](u64 (&o)[P]) {
 #pragma unroll
     for (int i = 0; i < P; ++i) o[i] = 0;
 #pragma unroll
@@ -288,14 +345,12 @@ __global__ void __launch_bounds__(kConvThreads, WT <= 4 ? 4 : 2) conv_bwd_kernel
 #pragma unroll
           for (int i = 0; i < P; ++i) o[i] = fma2(w[j + s][i], gw[WT - 1 - j][i], o[i]);
       }
-    if (t >= p.len && a.dfinal && v >= 0) {
-      u64 f[P];
-      to_pairs<T, V>(f, load_raw<T, V>(static_cast<const T*>(a.dfinal) +
-                                       ((long long)p.s * (W - 1) + t - p.len) * a.dim + d));
-#pragma unroll
-      for (int i = 0; i < P; ++i) o[i] = seq::add2(o[i], f[i]);
-    }
-    if (v >= p.r0) store_raw<T, V>(dxs + v * a.dim, from_pairs<T, V>(o));
+  };
+  auto row = [&](int u) {
+    shift<P, WT>(win);
+    shift<P, WT>(gw);
+    to_pairs<T, V>(win[WT - 1], ring.v[get][0][u][threadIdx.x]);
+    pre_grad<T, V, WT, SILU>(gw[WT - 1], a, w, b, win, ring.v[get][1][u][threadIdx.x]);
   };
   auto add_sums = [&]() {
 #pragma unroll
@@ -306,49 +361,56 @@ __global__ void __launch_bounds__(kConvThreads, WT <= 4 ? 4 : 2) conv_bwd_kernel
         if (k >= skip) dw[k][i] = fma2(gw[WT - 1][i], win[k][i], dw[k][i]);
     }
   };
-  seq::Vec<T, V> rx[kBwdGroup], rg[kBwdGroup];
-  long long t = p.r0;
-  // Whole groups of the slot's rows without conditions, so that the moving windows cost no moves.
-  for (; t + kBwdGroup <= r1; t += kBwdGroup) {
+  for (long long t = p.r0; t < end; t += G) {
+    if constexpr (R::ASYNC) {
+      seq::cp_async_wait<kBwdStages - 2>();
+    } else {
 #pragma unroll
-    for (int u = 0; u < kBwdGroup; ++u) {
-      rx[u] = load_raw<T, V>(xs + (t + u) * a.x_row);
-      rg[u] = load_raw<T, V>(dys + (t + u) * a.dim);
-    }
-#pragma unroll
-    for (int u = 0; u < kBwdGroup; ++u) {
-      shift<P, WT>(win);
-      shift<P, WT>(gw);
-      to_pairs<T, V>(win[WT - 1], rx[u]);
-      pre_grad<T, V, WT>(gw[WT - 1], a, w, b, win, rg[u]);
-      add_sums();
-      finish(t + u);
-    }
-  }
-  // The rows that are left, and the W - 1 below the slot whose gradients its last rows need (past the end: 0).
-  const long long end = p.r0 < r1 ? r1 + W - 1 : r1;
-  for (; t < end; t += kBwdGroup) {
-#pragma unroll
-    for (int u = 0; u < kBwdGroup; ++u)
-      if (t + u < end && t + u < p.len) {
-        rx[u] = load_raw<T, V>(xs + (t + u) * a.x_row);
-        rg[u] = load_raw<T, V>(dys + (t + u) * a.dim);
-      }
-#pragma unroll
-    for (int u = 0; u < kBwdGroup; ++u)
-      if (t + u < end) {
-        shift<P, WT>(win);
-        shift<P, WT>(gw);
-        if (t + u < p.len) {
-          to_pairs<T, V>(win[WT - 1], rx[u]);
-          pre_grad<T, V, WT>(gw[WT - 1], a, w, b, win, rg[u]);
-        } else {
-#pragma unroll
-          for (int i = 0; i < P; ++i) gw[WT - 1][i] = 0;
+      for (int u = 0; u < G; ++u)
+        if (t + u < in) {
+          ring.v[0][0][u][threadIdx.x] = load_raw<T, V>(xs + (t + u) * a.x_row);
+          ring.v[0][1][u][threadIdx.x] = load_raw<T, V>(dys + (t + u) * a.dim);
         }
-        if (t + u < r1) add_sums();
-        finish(t + u);
+    }
+    if (t + G <= r1) {  // the slot's own rows, without conditions, so that the moving windows cost no moves
+      const bool above = t > p.r0;
+#pragma unroll
+      for (int u = 0; u < G; ++u) {
+        u64 o[P];
+        row(u);
+        add_sums();
+        dx_row(o);
+        if (above || u >= W - 1) store_raw<T, V>(po + (long long)u * a.dim, from_pairs<T, V>(o));
       }
+    } else {
+#pragma unroll
+      for (int u = 0; u < G; ++u)
+        if (t + u < end) {
+          if (t + u < p.len) {
+            row(u);
+          } else {
+            shift<P, WT>(win);
+            shift<P, WT>(gw);
+#pragma unroll
+            for (int i = 0; i < P; ++i) gw[WT - 1][i] = 0;
+          }
+          if (t + u < r1) add_sums();
+          const long long v = t + u - (W - 1);
+          u64 o[P];
+          dx_row(o);
+          if (v >= p.r0 && a.dfinal && t + u >= p.len) {
+            u64 f[P];
+            to_pairs<T, V>(f, load_raw<T, V>(static_cast<const T*>(a.dfinal) +
+                                             ((long long)p.s * (W - 1) + t + u - p.len) * a.dim + d));
+#pragma unroll
+            for (int i = 0; i < P; ++i) o[i] = seq::add2(o[i], f[i]);
+          }
+          if (v >= p.r0) store_raw<T, V>(po + (long long)u * a.dim, from_pairs<T, V>(o));
+        }
+    }
+    po += (long long)G * a.dim;
+    get = !R::ASYNC || get + 1 == kBwdStages ? 0 : get + 1;
+    load();
   }
   auto put = [&](int k, const u64 (&v)[P]) {
 #pragma unroll
@@ -379,7 +441,7 @@ __global__ void __launch_bounds__(kConvThreads, WT <= 4 ? 4 : 2) conv_bwd_kernel
         u64 g[P], wn[WT][P];
 #pragma unroll
         for (int k = 0; k < WT; ++k) to_pairs<T, V>(wn[k], load_row<T, V>(a, xs, p, t - (WT - 1) + k, d));
-        pre_grad<T, V, WT>(g, a, w, b, wn, load_raw<T, V>(dys + (long long)t * a.dim));
+        pre_grad<T, V, WT, SILU>(g, a, w, b, wn, load_raw<T, V>(dys + (long long)t * a.dim));
         // wn[k] is virtual row t - (WT-1) + k, that is o[t + k] where it is below 0
 #pragma unroll
         for (int k = 0; k + t < WT - 1; ++k)
@@ -518,13 +580,19 @@ long long bwd_rows(const sf_causal_conv1d_desc* d) { return slot_rows(d, bwd_vec
 template <typename T, int V, int WT>
 sf_status run_fwd(const ConvArgs& a, dim3 grid, cudaStream_t st) {
   grid.y = channel_blocks(a.dim, V);
-  conv_fwd_kernel<T, V, WT><<<grid, kConvThreads, 0, st>>>(a);
+  constexpr size_t smem = sizeof(Ring<T, V, 1, kFwdGroup, kFwdStages>) + sizeof(Weights<V, WT>);
+  auto kernel = a.silu ? conv_fwd_kernel<T, V, WT, true> : conv_fwd_kernel<T, V, WT, false>;
+  if (smem > 48 * 1024 && !allow_max_smem(reinterpret_cast<const void*>(kernel))) return SF_ERR_CUDA;
+  kernel<<<grid, kConvThreads, smem, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
 }
 template <typename T, int V, int WT>
 sf_status run_bwd(const ConvArgs& a, dim3 grid, cudaStream_t st) {
   grid.y = channel_blocks(a.dim, V);
-  conv_bwd_kernel<T, V, WT><<<grid, kConvThreads, 0, st>>>(a);
+  constexpr size_t smem = sizeof(Ring<T, V, 2, kBwdGroup, kBwdStages>) + sizeof(Weights<V, WT>);
+  auto kernel = a.silu ? conv_bwd_kernel<T, V, WT, true> : conv_bwd_kernel<T, V, WT, false>;
+  if (smem > 48 * 1024 && !allow_max_smem(reinterpret_cast<const void*>(kernel))) return SF_ERR_CUDA;
+  kernel<<<grid, kConvThreads, smem, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
 }
 template <typename T, int V, int WT>

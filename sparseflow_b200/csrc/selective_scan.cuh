@@ -203,20 +203,6 @@ struct Place {
   __device__ __forceinline__ bool own(int j) const { return chan(j) < ch; }
 };
 
-__device__ __forceinline__ void cp_async(void* dst, const void* src, int bytes, bool in) {
-  const uint32_t d = smem_u32(dst);
-  const int n = in ? bytes : 0;  // bytes past n are filled with 0
-  if (bytes == 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
-  if (bytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
-  if (bytes == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-
 // Tiles' elements on their way: x, dt, z and dy of four channels and one row, and words of B and C, copied
 // asynchronously to a ring of STAGES tiles in shared memory. A thread copies what it will convert itself, so no barrier
 // guards the ring, and it has the same channels in every tile. (In registers the tile ahead was spilled, which waits

@@ -48,6 +48,21 @@ __device__ __forceinline__ float rcp(float v) {
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
+// Asynchronous copy of 4, 8 or 16 bytes to shared memory, zeros where `in` is false (then nothing is read).
+__device__ __forceinline__ void cp_async(void* dst, const void* src, int bytes, bool in) {
+  const uint32_t d = smem_u32(dst);
+  const int n = in ? bytes : 0;  // bytes past n are filled with 0
+  if (bytes == 4) asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
+  if (bytes == 8) asm volatile("cp.async.ca.shared.global [%0], [%1], 8, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
+  if (bytes == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(d), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
 // V consecutive elements of T, loaded and stored as one word where V > 1.
 template <typename T, int V>
 struct alignas(sizeof(T) * V) Vec {
