@@ -171,7 +171,7 @@ __device__ __forceinline__ void shift(u64 (&row)[WT][P]) {
 }
 
 template <typename T, int V, int WT, bool SILU>
-__global__ void __launch_bounds__(kConvThreads, WT <= 4 ? 4 : 2) conv_fwd_kernel(ConvArgs a) {
+__global__ void __launch_bounds__(kConvThreads, WT <= 4 ? 6 : 3) conv_fwd_kernel(ConvArgs a) {
   constexpr int P = kPairs<V>, G = kFwdGroup;
   using R = Ring<T, V, 1, G, kFwdStages>;
   extern __shared__ __align__(16) char smem[];
@@ -572,7 +572,7 @@ long long slot_rows(const sf_causal_conv1d_desc* d, int V, long long want, long 
   return rows;
 }
 // Vector widths (bytes): 16 forward; 8 backward and above 4 taps, whose windows would not fit the registers.
-int fwd_vec(const sf_causal_conv1d_desc* d) { return (d->width <= 4 ? 16 : 8) / (int)dtype_size(d->dtype); }
+int fwd_vec(const sf_causal_conv1d_desc* d) { return 8 / (int)dtype_size(d->dtype); }
 int bwd_vec(const sf_causal_conv1d_desc* d) { return 8 / (int)dtype_size(d->dtype); }
 long long fwd_rows(const sf_causal_conv1d_desc* d) { return slot_rows(d, fwd_vec(d), 148 * 6, 64); }
 long long bwd_rows(const sf_causal_conv1d_desc* d) { return slot_rows(d, bwd_vec(d), 148 * 6, 128); }
@@ -642,7 +642,7 @@ extern "C" sf_status sf_causal_conv1d(const void* x, const void* weight, const v
   if (slots > INT32_MAX) return SF_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)slots);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  SF_CONV_DISPATCH(16, 8, run_fwd, a, grid, st)
+  SF_CONV_DISPATCH(8, 8, run_fwd, a, grid, st)
 }
 
 extern "C" size_t sf_causal_conv1d_backward_workspace_size(const sf_causal_conv1d_desc* d) {
