@@ -13,14 +13,28 @@
 // - c2 rstd2 mean(e rh), so one reduction of three sums serves both.
 // r' is computed again from y, residual and gate: the stored one is rounded to the residual's type.
 //
-// About 14 operations an element forward and 36 backward against 4 to 7 tensors moved: HBM-bound. A block of
-// threads holds whole rows in registers, 8 neighbouring channels a thread and vector.
+// The sums over rows need one accumulator for both weights behind the norm: with Q = sum dt act(gate) yh,
+// dscale = w_post Q and dw_post = scale Q.
+//
+// About 14 operations an element forward and 36 backward against 4 to 7 tensors moved: HBM-bound. A block holds whole
+// rows, 8 neighbouring channels a thread, and walks down a range of rows with the weights and the sums over rows in
+// registers, while the rows ahead are copied asynchronously to a ring in shared memory, each thread its own channels
+// (no barrier guards the ring). Rows of more than kRingDim channels, or that 16-byte copies do not fit, take the
+// kernels without a ring, which read them twice where registers do not hold them.
 #include "sequence.cuh"
 
 namespace sf {
 namespace {
 
+using seq::add2;
+using seq::fma2;
+using seq::mul2;
+using seq::pack2;
+using seq::u64;
+using seq::unpack2;
+
 constexpr int kV = 8;             // channels per vector: 16 bytes of a 16-bit type
+constexpr int kRingDim = 4096;    // 512 threads
 constexpr int kMaxDim = 16384;    // 1024 threads, two vectors each
 
 struct NormArgs {
@@ -29,7 +43,7 @@ struct NormArgs {
   float* rstd;
   const void *dr, *dx;
   void *dy, *dres, *dgate;
-  float *part_w, *part_gate;  // backward partial sums: [blocks][3][dim], [blocks][dim]
+  float *part_w, *part_gate;  // backward partial sums: [blocks][2][dim] (Q, dw_pre), [blocks][dim]
   long long rows, y_row, res_row, gate_row, rows_per_gate;
   int dim, w_dtype, gate_kind;
   float alpha, eps;
@@ -208,7 +222,7 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(NormArgs a, long long gr
   const long long first = (long long)blockIdx.y * group_rows;
   const long long begin = first + blockIdx.x * per, end = min(begin + per, first + group_rows);
   const bool shared_gate = a.part_gate != nullptr;
-  float gpost[K][kV] = {}, gpre[K][kV] = {}, gscale[K][kV] = {}, ggate[K][kV] = {};
+  float Q[K][kV] = {}, gpre[K][kV] = {}, ggate[K][kV] = {};
   for (long long row = begin; row < end; ++row) {
     const float rstd1 = a.w_post ? a.rstd[row] : 1.f, rstd2 = a.w_pre ? a.rstd[a.rows + row] : 0.f;
     float yh[K][kV], rh[K][kV], dt[K][kV], dx[K][kV];
@@ -284,10 +298,8 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(NormArgs a, long long gr
       }
 #pragma unroll
       for (int i = 0; i < kV; ++i) {
-        const float da = dt[k][i] * act[i];
-        gscale[k][i] = fmaf(da, wpost[i] * yh[k][i], gscale[k][i]);
-        const float du = da * sc[i];
-        gpost[k][i] = fmaf(du, yh[k][i], gpost[k][i]);
+        const float da = dt[k][i] * act[i], du = da * sc[i];
+        Q[k][i] = fmaf(da, yh[k][i], Q[k][i]);
         o[i] = rstd1 * fmaf(wpost[i], du, -yh[k][i] * c1);
       }
       store8<T>(static_cast<T*>(a.dy) + row * a.dim, o, c, a.dim, a.vec);
@@ -299,30 +311,331 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(NormArgs a, long long gr
     }
   }
   const long long block = (long long)blockIdx.y * gridDim.x + blockIdx.x;
-  float* pw = a.part_w + block * 3 * a.dim;
+  float* pw = a.part_w + block * 2 * a.dim;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const int c = (k * blockDim.x + threadIdx.x) * kV;
 #pragma unroll
     for (int i = 0; i < kV; ++i)
       if (c + i < a.dim) {
-        pw[c + i] = gpost[k][i];
+        pw[c + i] = Q[k][i];
         pw[a.dim + c + i] = gpre[k][i];
-        pw[2 * a.dim + c + i] = gscale[k][i];
         if (shared_gate) a.part_gate[block * a.dim + c + i] = ggate[k][i];
       }
   }
 }
 
-// out[g][i] = sum over j < blocks of part[g][j][stride] at i, in order.
-__global__ void norm_reduce_kernel(const float* part, long long blocks, long long stride, int n, int dtype,
-                                   void* out) {
-  const int i = blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n) return;
+// ---------------------------------------------------------------------------------------------------------------------
+// Kernels with a ring
+// ---------------------------------------------------------------------------------------------------------------------
+
+// 8 channels of a row of E: one or two 16-byte words, word h of thread t at [h][t].
+template <typename E>
+constexpr int kWords = sizeof(E) / 2;
+template <typename E>
+__device__ __forceinline__ void copy8(float4* slot, const void* row0, long long row, int c, bool in) {
+  const E* p = static_cast<const E*>(row0) + row + c;
+#pragma unroll
+  for (int h = 0; h < kWords<E>; ++h)
+    if (in) seq::cp_async(slot + h * blockDim.x + threadIdx.x, p + h * (16 / (int)sizeof(E)), 16, true);
+}
+template <typename E>
+__device__ __forceinline__ void get8(u64 (&o)[4], const float4* slot) {
+  float4 w[kWords<E>];
+#pragma unroll
+  for (int h = 0; h < kWords<E>; ++h) w[h] = slot[h * blockDim.x + threadIdx.x];
+  const E* e = reinterpret_cast<const E*>(w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = pack2(DT<E>::to_f(e[2 * i]), DT<E>::to_f(e[2 * i + 1]));
+}
+template <typename E>
+__device__ __forceinline__ void put8(void* row0, long long row, int c, const u64 (&v)[4]) {
+  E e[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    float lo, hi;
+    unpack2(lo, hi, v[i]);
+    e[2 * i] = DT<E>::from_f(lo);
+    e[2 * i + 1] = DT<E>::from_f(hi);
+  }
+  float4* p = reinterpret_cast<float4*>(static_cast<E*>(row0) + row + c);
+#pragma unroll
+  for (int h = 0; h < kWords<E>; ++h) __stcs(p + h, reinterpret_cast<const float4*>(e)[h]);
+}
+__device__ __forceinline__ void weights8(u64 (&o)[4], const void* p, int c, const NormArgs& a) {
+  float t[kV];
+  load_w8(t, p, c, a.dim, a.vec, a.w_dtype);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = pack2(t[2 * i], t[2 * i + 1]);
+}
+__device__ __forceinline__ u64 both(float v) { return pack2(v, v); }
+// act(gate) of a pair, and its derivative times another pair.
+__device__ __forceinline__ u64 act2(u64 g, int kind) {
+  if (kind == SF_GATE_LINEAR) return g;
+  float lo, hi;
+  unpack2(lo, hi, g);
+  return pack2(gate_act(lo, kind), gate_act(hi, kind));
+}
+__device__ __forceinline__ u64 dact2(u64 g, int kind) {
+  float lo, hi;
+  unpack2(lo, hi, g);
+  return pack2(gate_dact(lo, kind), gate_dact(hi, kind));
+}
+
+// Sums over the block with one barrier: `buf` alternates between two halves, so the sum before may still be read.
+template <int N>
+__device__ __forceinline__ void ring_sum(float (&v)[N], float (*buf)[16 * N], int& half) {
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+  const int warps = blockDim.x >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warps == 1) return;
+  if (lane == 0)
+#pragma unroll
+    for (int n = 0; n < N; ++n) buf[half][w * N + n] = v[n];
+  __syncthreads();
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    float s = lane < warps ? buf[half][lane * N + n] : 0.f;
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
+    v[n] = __shfl_sync(0xffffffffu, s, 0);
+  }
+  half ^= 1;
+}
+
+template <typename T, typename R>
+struct FwdRing {
+  static constexpr int STAGES = sizeof(T) == 4 ? 2 : 3;
+  static constexpr int Y = 0, GATE = kWords<T>, RES = 2 * kWords<T>, WORDS = 2 * kWords<T> + kWords<R>;
+};
+template <typename T, typename R>
+__global__ void __launch_bounds__(512, 2) norm_fwd_ring_kernel(NormArgs a) {
+  using S = FwdRing<T, R>;
+  extern __shared__ __align__(16) float4 ring[];
+  const int c = threadIdx.x * kV, n = blockDim.x;
+  float(*buf)[16] = reinterpret_cast<float(*)[16]>(ring + S::STAGES * S::WORDS * n);
+  const bool own = c < a.dim;
+  const float inv = 1.f / (float)a.dim;
+  const bool gated = a.gate_kind != SF_GATE_NONE;
+  long long ahead = blockIdx.x;
+  int put = 0, get = 0, half = 0;
+  auto load = [&]() {
+    if (ahead < a.rows && own) {
+      float4* s = ring + put * S::WORDS * n;
+      copy8<T>(s + S::Y * n, a.y, ahead * a.y_row, c, true);
+      if (gated) copy8<T>(s + S::GATE * n, a.gate, ahead / a.rows_per_gate * a.gate_row, c, true);
+      if (a.res) copy8<R>(s + S::RES * n, a.res, ahead * a.res_row, c, true);
+    }
+    seq::cp_async_commit();
+    ahead += gridDim.x;
+    put = put + 1 == S::STAGES ? 0 : put + 1;
+  };
+  for (int i = 0; i < S::STAGES - 1; ++i) load();
+  u64 ws[4], wpre[4];
+  weights8(ws, a.w_post, c, a);
+  weights8(wpre, a.scale, c, a);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) ws[i] = mul2(ws[i], wpre[i]);
+  weights8(wpre, a.w_pre, c, a);
+  const u64 alpha = both(a.alpha);
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    seq::cp_async_wait<S::STAGES - 2>();
+    const float4* s = ring + get * S::WORDS * n;
+    u64 r[4] = {0, 0, 0, 0};
+    if (own) get8<T>(r, s + S::Y * n);
+    float rstd1 = 1.f, sum[1];
+    if (a.w_post) {
+      u64 q = mul2(r[0], r[0]);
+#pragma unroll
+      for (int i = 1; i < 4; ++i) q = fma2(r[i], r[i], q);
+      sum[0] = seq::sum2(q);
+      ring_sum<1>(sum, buf, half);
+      rstd1 = rsqrtf(sum[0] * inv + a.eps);
+    }
+    if (own) {
+      const u64 k = both(rstd1);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) r[i] = mul2(r[i], mul2(k, ws[i]));
+      if (gated) {
+        u64 g[4];
+        get8<T>(g, s + S::GATE * n);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = mul2(r[i], act2(g[i], a.gate_kind));
+      }
+      if (a.res) {
+        u64 t[4];
+        get8<R>(t, s + S::RES * n);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = fma2(alpha, t[i], r[i]);
+      }
+      if (a.r_out) put8<R>(a.r_out, row * a.dim, c, r);
+    }
+    get = get + 1 == S::STAGES ? 0 : get + 1;
+    load();
+    float rstd2 = 1.f;
+    if (a.w_pre) {
+      u64 q = mul2(r[0], r[0]);
+#pragma unroll
+      for (int i = 1; i < 4; ++i) q = fma2(r[i], r[i], q);
+      sum[0] = seq::sum2(q);
+      ring_sum<1>(sum, buf, half);
+      rstd2 = rsqrtf(sum[0] * inv + a.eps);
+      if (own) {
+        const u64 k = both(rstd2);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = mul2(r[i], mul2(k, wpre[i]));
+        put8<T>(a.x_out, row * a.dim, c, r);
+      }
+    }
+    if (a.rstd && threadIdx.x == 0) {
+      a.rstd[row] = rstd1;
+      a.rstd[a.rows + row] = rstd2;
+    }
+  }
+}
+
+template <typename T, typename R>
+struct BwdRing {
+  static constexpr int STAGES = sizeof(T) == 4 ? 2 : 3;
+  static constexpr int Y = 0, GATE = kWords<T>, DX = 2 * kWords<T>, RES = 3 * kWords<T>, DR = RES + kWords<R>;
+  static constexpr int WORDS = 3 * kWords<T> + 2 * kWords<R>;
+};
+// Rows as in norm_bwd_kernel; part_w[block][0]: Q, [1]: dw_pre.
+template <typename T, typename R>
+__global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long long group_rows, long long per) {
+  using S = BwdRing<T, R>;
+  extern __shared__ __align__(16) float4 ring[];
+  const int c = threadIdx.x * kV, n = blockDim.x;
+  float(*buf)[48] = reinterpret_cast<float(*)[48]>(ring + S::STAGES * S::WORDS * n);
+  const bool own = c < a.dim;
+  const float inv = 1.f / (float)a.dim;
+  const bool gated = a.gate_kind != SF_GATE_NONE, shared_gate = a.part_gate != nullptr, pre = a.w_pre && a.dx;
+  const long long first = (long long)blockIdx.y * group_rows;
+  const long long begin = first + blockIdx.x * per, end = min(begin + per, first + group_rows);
+  long long ahead = begin;
+  int put = 0, get = 0, half = 0;
+  float next1 = 1.f, next2 = 0.f;
+  auto load = [&]() {
+    if (ahead < end && own) {
+      float4* s = ring + put * S::WORDS * n;
+      copy8<T>(s + S::Y * n, a.y, ahead * a.y_row, c, true);
+      if (gated) copy8<T>(s + S::GATE * n, a.gate, ahead / a.rows_per_gate * a.gate_row, c, true);
+      if (a.res) copy8<R>(s + S::RES * n, a.res, ahead * a.res_row, c, true);
+      if (pre) copy8<T>(s + S::DX * n, a.dx, ahead * a.dim, c, true);
+      if (a.dr) copy8<R>(s + S::DR * n, a.dr, ahead * a.dim, c, true);
+    }
+    seq::cp_async_commit();
+    ++ahead;
+    put = put + 1 == S::STAGES ? 0 : put + 1;
+  };
+  auto load_rstd = [&](long long row) {
+    if (row >= end) return;
+    if (a.w_post) next1 = a.rstd[row];
+    if (a.w_pre) next2 = a.rstd[a.rows + row];
+  };
+  for (int i = 0; i < S::STAGES - 1; ++i) load();
+  load_rstd(begin);
+  u64 ws[4], wpre[4], Q[4] = {}, gpre[4] = {}, ggate[4] = {};
+  weights8(ws, a.w_post, c, a);
+  weights8(wpre, a.scale, c, a);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) ws[i] = mul2(ws[i], wpre[i]);
+  weights8(wpre, a.w_pre, c, a);
+  const u64 alpha = both(a.alpha);
+  for (long long row = begin; row < end; ++row) {
+    seq::cp_async_wait<S::STAGES - 2>();
+    const float4* s = ring + get * S::WORDS * n;
+    const float rstd1 = next1, rstd2 = next2;
+    load_rstd(row + 1);
+    u64 yh[4] = {}, act[4], rh[4] = {}, dt[4] = {}, g[4];
+    float sum[3] = {0.f, 0.f, 0.f};
+    const u64 k1 = both(rstd1), k2 = both(rstd2);
+    if (own) {
+      get8<T>(yh, s + S::Y * n);
+      if (gated) get8<T>(g, s + S::GATE * n);
+      if (a.res) get8<R>(rh, s + S::RES * n);
+      if (a.dr) get8<R>(dt, s + S::DR * n);
+      u64 dx[4] = {}, s0 = 0, s1 = 0, s2 = 0;
+      if (pre) get8<T>(dx, s + S::DX * n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        yh[i] = mul2(yh[i], k1);
+        u64 e = mul2(ws[i], yh[i]);  // scale act(gate) u
+        if (gated) {
+          act[i] = act2(g[i], a.gate_kind);
+          e = mul2(e, act[i]);
+        }
+        rh[i] = mul2(fma2(alpha, rh[i], e), k2);
+        gpre[i] = fma2(dx[i], rh[i], gpre[i]);
+        const u64 q = mul2(wpre[i], dx[i]);
+        s0 = fma2(q, rh[i], s0);
+        dt[i] = fma2(k2, q, dt[i]);
+        s1 = fma2(e, dt[i], s1);
+        s2 = fma2(e, rh[i], s2);
+      }
+      sum[0] = seq::sum2(s0), sum[1] = seq::sum2(s1), sum[2] = seq::sum2(s2);
+    }
+    ring_sum<3>(sum, buf, half);
+    const float c2 = sum[0] * inv * rstd2, c1 = a.w_post ? (sum[1] - c2 * sum[2]) * inv : 0.f;
+    if (own) {
+      const u64 m2 = both(-c2), m1 = both(-c1 * rstd1);
+      u64 o[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        dt[i] = fma2(m2, rh[i], dt[i]);
+        const u64 da = gated ? mul2(dt[i], act[i]) : dt[i];
+        Q[i] = fma2(da, yh[i], Q[i]);
+        o[i] = fma2(m1, yh[i], mul2(k1, mul2(ws[i], da)));
+      }
+      put8<T>(a.dy, row * a.dim, c, o);
+      if (gated) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          o[i] = mul2(mul2(dt[i], yh[i]), ws[i]);
+          if (a.gate_kind != SF_GATE_LINEAR) o[i] = mul2(o[i], dact2(g[i], a.gate_kind));
+          if (shared_gate) ggate[i] = add2(ggate[i], o[i]);
+        }
+        if (!shared_gate) put8<T>(a.dgate, row * a.dim, c, o);
+      }
+      if (a.dres) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = mul2(alpha, dt[i]);
+        put8<R>(a.dres, row * a.dim, c, o);
+      }
+    }
+    get = get + 1 == S::STAGES ? 0 : get + 1;
+    load();
+  }
+  if (!own) return;
+  const long long block = (long long)blockIdx.y * gridDim.x + blockIdx.x;
+  put8<float>(a.part_w + block * 2 * a.dim, 0, c, Q);
+  put8<float>(a.part_w + (block * 2 + 1) * a.dim, 0, c, gpre);
+  if (shared_gate) put8<float>(a.part_gate + block * a.dim, 0, c, ggate);
+}
+
+// out[g][i] = factor[i] sum over j < blocks of part[g][j][stride] at i, to at most two outputs (a null output is left
+// out, a null factor is 1). A warp has 32 values and each of the block's 8 warps every eighth block: a fixed order.
+__global__ void __launch_bounds__(256) norm_reduce_kernel(const float* part, long long blocks, long long stride, int n,
+                                                          int dtype, void* out0, const void* factor0, void* out1,
+                                                          const void* factor1, int factor_dtype) {
+  __shared__ float sums[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
   const float* p = part + (long long)blockIdx.y * blocks * stride + i;
   float s = 0.f;
-  for (long long j = 0; j < blocks; ++j) s += p[j * stride];
-  seq::store_param(out, (long long)blockIdx.y * n + i, dtype, s);
+  if (i < n) {
+#pragma unroll 8
+    for (long long j = warp; j < blocks; j += 8) s += p[j * stride];
+  }
+  sums[warp][lane] = s;
+  __syncthreads();
+  if (warp != 0 || i >= n) return;
+#pragma unroll
+  for (int w = 1; w < 8; ++w) s += sums[w][lane];
+  const long long o = (long long)blockIdx.y * n + i;
+  if (out0) seq::store_param(out0, o, dtype, factor0 ? s * seq::load_param(factor0, i, factor_dtype) : s);
+  if (out1) seq::store_param(out1, o, dtype, factor1 ? s * seq::load_param(factor1, i, factor_dtype) : s);
 }
 
 bool valid(const sf_block_norm_desc* d) {
@@ -348,6 +661,10 @@ int threads_for(int dim, int K) {
   return (t + 31) / 32 * 32;
 }
 
+// Blocks that fill the GPU: rows of up to kRingDim channels, 512 threads an SM backward (about 110 registers each) and
+// 1024 forward; wider ones, one row in 1024 threads.
+long long bwd_blocks(int dim) { return dim <= kRingDim ? 148ll * (512 / threads_for(dim, 1)) : 296; }
+
 struct BwdPlan {
   long long groups, group_rows, blocks, per;
   bool shared_gate;
@@ -357,7 +674,7 @@ BwdPlan bwd_plan(const sf_block_norm_desc* d) {
   p.shared_gate = d->gate_kind != SF_GATE_NONE && d->rows_per_gate > 1;
   p.groups = p.shared_gate ? d->rows / d->rows_per_gate : 1;
   p.group_rows = p.shared_gate ? d->rows_per_gate : d->rows;
-  const long long want = 592;  // blocks in all: 148 SMs, a few blocks each
+  const long long want = bwd_blocks(d->dim);
   long long blocks = (want + p.groups - 1) / p.groups;
   if (blocks > p.group_rows) blocks = p.group_rows;
   if (blocks < 1) blocks = 1;
@@ -388,8 +705,20 @@ NormArgs base_args(const void* y, const void* residual, const void* gate, const 
   return a;
 }
 
+bool ring_fits(const NormArgs& a) { return a.vec && a.dim <= kRingDim; }
+
 template <typename T, typename R>
 sf_status run_fwd(const NormArgs& a, cudaStream_t st) {
+  if (ring_fits(a)) {
+    using S = FwdRing<T, R>;
+    const int threads = threads_for(a.dim, 1);
+    const size_t smem = (size_t)S::STAGES * S::WORDS * threads * sizeof(float4) + 2 * 16 * sizeof(float);
+    auto kernel = norm_fwd_ring_kernel<T, R>;
+    if (smem > 48 * 1024 && !allow_max_smem(reinterpret_cast<const void*>(kernel))) return SF_ERR_CUDA;
+    const long long most = 148ll * (1024 / threads);
+    kernel<<<(unsigned)(a.rows < most ? a.rows : most), threads, smem, st>>>(a);
+    return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
+  }
   const int K = vectors_per_thread(a.dim), threads = threads_for(a.dim, K);
   const unsigned grid = (unsigned)(a.rows < INT32_MAX ? a.rows : INT32_MAX);
   if (K == 1) norm_fwd_kernel<T, R, 1><<<grid, threads, 0, st>>>(a);
@@ -398,6 +727,15 @@ sf_status run_fwd(const NormArgs& a, cudaStream_t st) {
 }
 template <typename T, typename R>
 sf_status run_bwd(const NormArgs& a, const BwdPlan& p, cudaStream_t st) {
+  if (ring_fits(a)) {
+    using S = BwdRing<T, R>;
+    const int threads = threads_for(a.dim, 1);
+    const size_t smem = (size_t)S::STAGES * S::WORDS * threads * sizeof(float4) + 2 * 48 * sizeof(float);
+    auto kernel = norm_bwd_ring_kernel<T, R>;
+    if (smem > 48 * 1024 && !allow_max_smem(reinterpret_cast<const void*>(kernel))) return SF_ERR_CUDA;
+    kernel<<<dim3((unsigned)p.blocks, (unsigned)p.groups), threads, smem, st>>>(a, p.group_rows, p.per);
+    return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
+  }
   // The kernel wants about 90 registers with one vector a thread and 160 with two.
   const int K = a.dim > 512 * kV ? 2 : 1, threads = threads_for(a.dim, K);
   const dim3 grid((unsigned)p.blocks, (unsigned)p.groups);
@@ -448,7 +786,7 @@ extern "C" sf_status sf_block_norm(const void* y, const void* residual, const vo
 extern "C" size_t sf_block_norm_backward_workspace_size(const sf_block_norm_desc* d) {
   if (!valid(d)) return 0;
   const BwdPlan p = bwd_plan(d);
-  return (size_t)(p.blocks * p.groups) * d->dim * (p.shared_gate ? 4 : 3) * sizeof(float);
+  return (size_t)(p.blocks * p.groups) * d->dim * (p.shared_gate ? 3 : 2) * sizeof(float);
 }
 
 extern "C" sf_status sf_block_norm_backward(const void* y, const void* residual, const void* gate,
@@ -477,7 +815,7 @@ extern "C" sf_status sf_block_norm_backward(const void* y, const void* residual,
   a.dres = d_residual;
   a.dgate = d_gate;
   a.part_w = part;
-  a.part_gate = p.shared_gate ? part + blocks * 3 * d->dim : nullptr;
+  a.part_gate = p.shared_gate ? part + blocks * 2 * d->dim : nullptr;
   a.vec = vectors_fit(d, {y, residual, gate, post_weight, pre_weight, scale, d_residual_out, d_normed, dy, d_residual,
                           p.shared_gate ? nullptr : d_gate});
   if (d->rows > 0) {
@@ -485,14 +823,15 @@ extern "C" sf_status sf_block_norm_backward(const void* y, const void* residual,
     SF_NORM_DISPATCH(d, (run_bwd<T, R>(a, p, st)));
     if (status != SF_OK) return status;
   }
-  const unsigned grid = (d->dim + 127) / 128;
-  void* outs[3] = {d_post_weight, d_pre_weight, d_scale};
-  for (int i = 0; i < 3; ++i)
-    if (outs[i])
-      norm_reduce_kernel<<<grid, 128, 0, st>>>(part + (long long)i * d->dim, blocks, 3ll * d->dim, d->dim, d->w_dtype,
-                                               outs[i]);
+  const unsigned grid = (d->dim + 31) / 32;
+  if (d_post_weight || d_scale)
+    norm_reduce_kernel<<<grid, 256, 0, st>>>(part, blocks, 2ll * d->dim, d->dim, d->w_dtype, d_post_weight, scale, d_scale,
+                                             post_weight, d->w_dtype);
+  if (d_pre_weight)
+    norm_reduce_kernel<<<grid, 256, 0, st>>>(part + d->dim, blocks, 2ll * d->dim, d->dim, d->w_dtype, d_pre_weight,
+                                             nullptr, nullptr, nullptr, d->w_dtype);
   if (p.shared_gate && d_gate && d->rows > 0)
-    norm_reduce_kernel<<<dim3(grid, (unsigned)p.groups), 128, 0, st>>>(a.part_gate, p.blocks, d->dim, d->dim, d->dtype,
-                                                                       d_gate);
+    norm_reduce_kernel<<<dim3(grid, (unsigned)p.groups), 256, 0, st>>>(a.part_gate, p.blocks, d->dim, d->dim, d->dtype,
+                                                                       d_gate, nullptr, nullptr, nullptr, d->w_dtype);
   return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
 }
