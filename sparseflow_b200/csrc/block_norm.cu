@@ -369,17 +369,20 @@ __device__ __forceinline__ void weights8(u64 (&o)[4], const void* p, int c, cons
   for (int i = 0; i < 4; ++i) o[i] = pack2(t[2 * i], t[2 * i + 1]);
 }
 __device__ __forceinline__ u64 both(float v) { return pack2(v, v); }
-// act(gate) of a pair, and its derivative times another pair.
-__device__ __forceinline__ u64 act2(u64 g, int kind) {
-  if (kind == SF_GATE_LINEAR) return g;
+// act(gate) of a pair, where sig is what the logistic function gives for it (used for silu and sigmoid), and its derivative.
+__device__ __forceinline__ u64 logistic2(u64 g) {
   float lo, hi;
   unpack2(lo, hi, g);
-  return pack2(gate_act(lo, kind), gate_act(hi, kind));
+  return pack2(seq::logistic(lo), seq::logistic(hi));
 }
-__device__ __forceinline__ u64 dact2(u64 g, int kind) {
-  float lo, hi;
-  unpack2(lo, hi, g);
-  return pack2(gate_dact(lo, kind), gate_dact(hi, kind));
+template <int KIND>
+__device__ __forceinline__ u64 act2(u64 g, u64 sig) {
+  return KIND == SF_GATE_SILU ? mul2(g, sig) : KIND == SF_GATE_SIGMOID ? sig : g;
+}
+template <int KIND>
+__device__ __forceinline__ u64 dact2(u64 g, u64 sig) {
+  const u64 rest = fma2(sig, both(-1.f), both(1.f));
+  return KIND == SF_GATE_SILU ? mul2(sig, fma2(g, rest, both(1.f))) : mul2(sig, rest);
 }
 
 // Sums over the block with one barrier: `buf` alternates between two halves, so the sum before may still be read.
@@ -410,7 +413,7 @@ struct FwdRing {
   static constexpr int STAGES = sizeof(T) == 4 ? 2 : 3;
   static constexpr int Y = 0, GATE = kWords<T>, RES = 2 * kWords<T>, WORDS = 2 * kWords<T> + kWords<R>;
 };
-template <typename T, typename R>
+template <typename T, typename R, int KIND>
 __global__ void __launch_bounds__(512, 2) norm_fwd_ring_kernel(NormArgs a) {
   using S = FwdRing<T, R>;
   extern __shared__ __align__(16) float4 ring[];
@@ -418,7 +421,7 @@ __global__ void __launch_bounds__(512, 2) norm_fwd_ring_kernel(NormArgs a) {
   float(*buf)[16] = reinterpret_cast<float(*)[16]>(ring + S::STAGES * S::WORDS * n);
   const bool own = c < a.dim;
   const float inv = 1.f / (float)a.dim;
-  const bool gated = a.gate_kind != SF_GATE_NONE;
+  constexpr bool gated = KIND != SF_GATE_NONE, curved = KIND == SF_GATE_SILU || KIND == SF_GATE_SIGMOID;
   long long ahead = blockIdx.x;
   int put = 0, get = 0, half = 0;
   auto load = [&]() {
@@ -462,7 +465,7 @@ __global__ void __launch_bounds__(512, 2) norm_fwd_ring_kernel(NormArgs a) {
         u64 g[4];
         get8<T>(g, s + S::GATE * n);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = mul2(r[i], act2(g[i], a.gate_kind));
+        for (int i = 0; i < 4; ++i) r[i] = mul2(r[i], act2<KIND>(g[i], curved ? logistic2(g[i]) : 0));
       }
       if (a.res) {
         u64 t[4];
@@ -503,7 +506,7 @@ struct BwdRing {
   static constexpr int WORDS = 3 * kWords<T> + 2 * kWords<R>;
 };
 // Rows as in norm_bwd_kernel; part_w[block][0]: Q, [1]: dw_pre.
-template <typename T, typename R>
+template <typename T, typename R, int KIND>
 __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long long group_rows, long long per) {
   using S = BwdRing<T, R>;
   extern __shared__ __align__(16) float4 ring[];
@@ -511,7 +514,8 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long 
   float(*buf)[48] = reinterpret_cast<float(*)[48]>(ring + S::STAGES * S::WORDS * n);
   const bool own = c < a.dim;
   const float inv = 1.f / (float)a.dim;
-  const bool gated = a.gate_kind != SF_GATE_NONE, shared_gate = a.part_gate != nullptr, pre = a.w_pre && a.dx;
+  constexpr bool gated = KIND != SF_GATE_NONE, curved = KIND == SF_GATE_SILU || KIND == SF_GATE_SIGMOID;
+  const bool shared_gate = a.part_gate != nullptr, pre = a.w_pre && a.dx;
   const long long first = (long long)blockIdx.y * group_rows;
   const long long begin = first + blockIdx.x * per, end = min(begin + per, first + group_rows);
   long long ahead = begin;
@@ -549,24 +553,25 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long 
     const float4* s = ring + get * S::WORDS * n;
     const float rstd1 = next1, rstd2 = next2;
     load_rstd(row + 1);
-    u64 yh[4] = {}, act[4], rh[4] = {}, dt[4] = {}, g[4];
+    u64 yh[4], sig[4], rh[4], dt[4], g[4];
     float sum[3] = {0.f, 0.f, 0.f};
     const u64 k1 = both(rstd1), k2 = both(rstd2);
     if (own) {
       get8<T>(yh, s + S::Y * n);
       if (gated) get8<T>(g, s + S::GATE * n);
+      u64 dx[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rh[i] = dt[i] = dx[i] = 0;
       if (a.res) get8<R>(rh, s + S::RES * n);
       if (a.dr) get8<R>(dt, s + S::DR * n);
-      u64 dx[4] = {}, s0 = 0, s1 = 0, s2 = 0;
       if (pre) get8<T>(dx, s + S::DX * n);
+      u64 s0 = 0, s1 = 0, s2 = 0;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         yh[i] = mul2(yh[i], k1);
         u64 e = mul2(ws[i], yh[i]);  // scale act(gate) u
-        if (gated) {
-          act[i] = act2(g[i], a.gate_kind);
-          e = mul2(e, act[i]);
-        }
+        if (curved) sig[i] = logistic2(g[i]);
+        if (gated) e = mul2(e, act2<KIND>(g[i], sig[i]));
         rh[i] = mul2(fma2(alpha, rh[i], e), k2);
         gpre[i] = fma2(dx[i], rh[i], gpre[i]);
         const u64 q = mul2(wpre[i], dx[i]);
@@ -585,7 +590,7 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long 
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         dt[i] = fma2(m2, rh[i], dt[i]);
-        const u64 da = gated ? mul2(dt[i], act[i]) : dt[i];
+        const u64 da = gated ? mul2(dt[i], act2<KIND>(g[i], sig[i])) : dt[i];
         Q[i] = fma2(da, yh[i], Q[i]);
         o[i] = fma2(m1, yh[i], mul2(k1, mul2(ws[i], da)));
       }
@@ -594,10 +599,14 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           o[i] = mul2(mul2(dt[i], yh[i]), ws[i]);
-          if (a.gate_kind != SF_GATE_LINEAR) o[i] = mul2(o[i], dact2(g[i], a.gate_kind));
-          if (shared_gate) ggate[i] = add2(ggate[i], o[i]);
+          if (curved) o[i] = mul2(o[i], dact2<KIND>(g[i], sig[i]));
         }
-        if (!shared_gate) put8<T>(a.dgate, row * a.dim, c, o);
+        if (shared_gate) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) ggate[i] = add2(ggate[i], o[i]);
+        } else {
+          put8<T>(a.dgate, row * a.dim, c, o);
+        }
       }
       if (a.dres) {
 #pragma unroll
@@ -713,7 +722,10 @@ sf_status run_fwd(const NormArgs& a, cudaStream_t st) {
     using S = FwdRing<T, R>;
     const int threads = threads_for(a.dim, 1);
     const size_t smem = (size_t)S::STAGES * S::WORDS * threads * sizeof(float4) + 2 * 16 * sizeof(float);
-    auto kernel = norm_fwd_ring_kernel<T, R>;
+    auto kernel = a.gate_kind == SF_GATE_NONE     ? norm_fwd_ring_kernel<T, R, SF_GATE_NONE>
+                  : a.gate_kind == SF_GATE_LINEAR ? norm_fwd_ring_kernel<T, R, SF_GATE_LINEAR>
+                  : a.gate_kind == SF_GATE_SILU   ? norm_fwd_ring_kernel<T, R, SF_GATE_SILU>
+                                                  : norm_fwd_ring_kernel<T, R, SF_GATE_SIGMOID>;
     if (smem > 48 * 1024 && !allow_max_smem(reinterpret_cast<const void*>(kernel))) return SF_ERR_CUDA;
     const long long most = 148ll * (1024 / threads);
     kernel<<<(unsigned)(a.rows < most ? a.rows : most), threads, smem, st>>>(a);
@@ -731,7 +743,10 @@ sf_status run_bwd(const NormArgs& a, const BwdPlan& p, cudaStream_t st) {
     using S = BwdRing<T, R>;
     const int threads = threads_for(a.dim, 1);
     const size_t smem = (size_t)S::STAGES * S::WORDS * threads * sizeof(float4) + 2 * 48 * sizeof(float);
-    auto kernel = norm_bwd_ring_kernel<T, R>;
+    auto kernel = a.gate_kind == SF_GATE_NONE     ? norm_bwd_ring_kernel<T, R, SF_GATE_NONE>
+                  : a.gate_kind == SF_GATE_LINEAR ? norm_bwd_ring_kernel<T, R, SF_GATE_LINEAR>
+                  : a.gate_kind == SF_GATE_SILU   ? norm_bwd_ring_kernel<T, R, SF_GATE_SILU>
+                                                  : norm_bwd_ring_kernel<T, R, SF_GATE_SIGMOID>;
     if (smem > 48 * 1024 && !allow_max_smem(reinterpret_cast<const void*>(kernel))) return SF_ERR_CUDA;
     kernel<<<dim3((unsigned)p.blocks, (unsigned)p.groups), threads, smem, st>>>(a, p.group_rows, p.per);
     return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
