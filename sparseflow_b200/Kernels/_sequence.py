@@ -1,4 +1,7 @@
-"""Argument checks shared by the sequence operators (causal_conv1d, selective_scan, block_norm)."""
+"""Argument checks shared by the sequence operators (causal_conv1d, selective_scan, block_norm).
+
+A decoding step calls them for a few microseconds of GPU work, so they use what is cheapest to ask of a tensor.
+"""
 from __future__ import annotations
 
 from typing import Optional
@@ -8,28 +11,25 @@ import torch
 from .. import _lib
 
 
-def require_cuda(**tensors: Optional[torch.Tensor]) -> torch.device:
-    """All given tensors on one CUDA device; returns it."""
-    device = None
-    for name, t in tensors.items():
-        if t is None:
-            continue
-        if not t.is_cuda:
-            raise RuntimeError(f"{name}: the sequence operators need CUDA tensors (there is no CPU path)")
-        if device is None:
-            device = t.device
-        elif t.device != device:
-            raise ValueError(f"{name} is on {t.device}, the others on {device}")
-    return device
+def require_cuda(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    """All given tensors on one CUDA device."""
+    if not first.is_cuda:
+        raise RuntimeError("the sequence operators need CUDA tensors (there is no CPU path)")
+    index = first.get_device()
+    for t in others:
+        if t is not None and t.get_device() != index:
+            if not t.is_cuda:
+                raise RuntimeError("the sequence operators need CUDA tensors (there is no CPU path)")
+            raise ValueError(f"a tensor is on {t.device}, another on {first.device}")
 
 
 def check_shape(name: str, t: torch.Tensor, shape) -> None:
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{name}: expected shape {list(shape)}, got {list(t.shape)}")
 
 
 def check_dtype(name: str, t: torch.Tensor, dtype: torch.dtype) -> None:
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         raise TypeError(f"{name}: expected {dtype}, got {t.dtype}")
 
 
@@ -50,23 +50,34 @@ def check_offsets(seq_offsets: Optional[torch.Tensor], x: torch.Tensor):
 def rows_of(t: torch.Tensor, inner: int = 1):
     """The tensor with its last `inner` dimensions contiguous (copied only where they are not) and its batch and
     row strides; the strides of dimensions of one entry, which may be anything, are those of a contiguous tensor."""
+    shape, stride = t.shape, t.stride()
     width = 1
     for k in range(1, inner + 1):
-        if t.shape[-k] != 1 and t.stride(-k) != width:
-            t = t.contiguous()
-            break
-        width *= t.shape[-k]
-    width = 1
-    for k in range(1, inner + 1):
-        width *= t.shape[-k]
-    row = t.stride(-inner - 1) if t.shape[-inner - 1] > 1 else width
-    if t.dim() == inner + 1:
+        if stride[-k] != width and shape[-k] != 1:
+            return rows_of(t.contiguous(), inner)
+        width *= shape[-k]
+    row = stride[-inner - 1] if shape[-inner - 1] > 1 else width
+    if len(shape) == inner + 1:
         return t, 0, row
-    return t, t.stride(0) if t.shape[0] > 1 else row * t.shape[1], row
+    return t, stride[0] if shape[0] > 1 else row * shape[1], row
+
+
+def dense(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    return t if t is None or t.is_contiguous() else t.contiguous()
 
 
 def needs_grad(*tensors: Optional[torch.Tensor]) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if not torch.is_grad_enabled():
+        return False
+    for t in tensors:
+        if t is not None and t.requires_grad:
+            return True
+    return False
+
+
+def layout(t: Optional[torch.Tensor]):
+    """What the checks of a call depend on, as a key of calls that have passed them."""
+    return None if t is None else (t.shape, t.stride(), t.dtype)
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:

@@ -10,7 +10,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from ._sequence import (call_on, check_dtype, check_offsets, check_shape, check_state_indices, needs_grad, ptr,
+from ._sequence import (call_on, check_dtype, check_offsets, check_shape, check_state_indices, dense, layout, needs_grad, ptr,
                         require_cuda, rows_of)
 
 _ACTIVATIONS = {None: False, "silu": True}
@@ -32,10 +32,10 @@ def _forward(x, weight, bias, initial_state, seq_offsets, silu, want_final):
     n_seq, length, packed = check_offsets(seq_offsets, x)
     dim, width = weight.shape
     x, batch, row = rows_of(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     final = torch.empty(n_seq, width - 1, dim, dtype=x.dtype, device=x.device) if want_final else None
     desc = _lib.causal_conv1d_desc(length, batch, row, n_seq, dim, width, silu, x.dtype, weight.dtype, packed)
-    call_on(x.device, "sf_causal_conv1d", ptr(x), ptr(weight), ptr(bias), ptr(initial_state), ptr(seq_offsets), ptr(y),
+    call_on(x.get_device(), "sf_causal_conv1d", ptr(x), ptr(weight), ptr(bias), ptr(initial_state), ptr(seq_offsets), ptr(y),
             ptr(final), desc)
     return y, final, desc, x
 
@@ -60,7 +60,7 @@ class _CausalConv1d(torch.autograd.Function):
         dinit = torch.empty_like(initial_state) if initial_state is not None and ctx.needs_input_grad[3] else None
         nbytes = _lib.load().sf_causal_conv1d_backward_workspace_size(ctx.desc)
         ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=x.device)
-        call_on(x.device, "sf_causal_conv1d_backward", ptr(x), ptr(weight), ptr(bias), ptr(initial_state),
+        call_on(x.get_device(), "sf_causal_conv1d_backward", ptr(x), ptr(weight), ptr(bias), ptr(initial_state),
                 ptr(seq_offsets), ptr(dy), ptr(dfinal), ptr(dx), ptr(dweight), ptr(dbias), ptr(dinit), ctx.desc,
                 ptr(ws), nbytes)
         return dx, dweight, dbias, dinit, None, None, None
@@ -77,17 +77,14 @@ def causal_conv1d(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Te
     before each sequence, oldest first (zeros if None). Returns y, or (y, final_state) where the final state is the
     next call's initial one. Differentiable once, in x, weight, bias and the initial state.
     """
-    device = require_cuda(x=x, weight=weight, bias=bias, initial_state=initial_state, seq_offsets=seq_offsets)
-    if device is None:
-        raise ValueError("x is missing")
+    require_cuda(x, weight, bias, initial_state, seq_offsets)
     dim, width = _check(x, weight, bias, activation)
     n_seq, _, _ = check_offsets(seq_offsets, x)
     if initial_state is not None:
         check_shape("initial_state", initial_state, (n_seq, width - 1, dim))
         check_dtype("initial_state", initial_state, x.dtype)
-        initial_state = initial_state.contiguous()
-    weight = weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
+        initial_state = dense(initial_state)
+    weight, bias = dense(weight), dense(bias)
     silu = _ACTIVATIONS[activation]
     if needs_grad(x, weight, bias, initial_state):
         y, final = _CausalConv1d.apply(x, weight, bias, initial_state, seq_offsets, silu, return_final_state)
@@ -104,7 +101,24 @@ def causal_conv1d_update(x: torch.Tensor, state: torch.Tensor, weight: torch.Ten
     Row i uses slot ``state_indices[i]`` (int32 on the device, distinct), or slot i without indices. A row whose
     index is no slot (-1, say) is padding: its y is 0 and no state changes. Not differentiable.
     """
-    require_cuda(x=x, state=state, weight=weight, bias=bias, state_indices=state_indices)
+    require_cuda(x, state, weight, bias, state_indices)
+    key = (layout(x), layout(state), layout(weight), layout(bias), layout(state_indices), activation)
+    desc = _update_plans.get(key)
+    if desc is None:
+        x, weight, bias, desc = _update_plan(x, state, weight, bias, activation, state_indices, key)
+    y = x.new_empty(x.shape)
+    call_on(x.get_device(), "sf_causal_conv1d_update", x.data_ptr(), state.data_ptr(), weight.data_ptr(), ptr(bias),
+            ptr(state_indices), y.data_ptr(), state.shape[0], desc)
+    return y
+
+
+# Descriptors of the layouts that single-token calls have come with, where nothing had to be copied: a decoding loop's
+# next call with the same layouts has passed its checks.
+_update_plans: dict = {}
+
+
+def _update_plan(x, state, weight, bias, activation, state_indices, key):
+    """Checks a call and returns its operands as the kernel reads them and its descriptor."""
     if x.dim() != 2:
         raise ValueError(f"x: expected [rows, dim], got {list(x.shape)}")
     dim, width = _check(x, weight, bias, activation)
@@ -113,12 +127,13 @@ def causal_conv1d_update(x: torch.Tensor, state: torch.Tensor, weight: torch.Ten
     check_shape("state", state, (state.shape[0], width - 1, dim))
     check_dtype("state", state, x.dtype)
     check_state_indices(state_indices, x.shape[0], state.shape[0])
-    weight = weight.contiguous()
-    bias = None if bias is None else bias.contiguous()
+    given = (x, weight, bias)
+    weight, bias = dense(weight), dense(bias)
     x, _, row = rows_of(x)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     desc = _lib.causal_conv1d_desc(1, 0, row, x.shape[0], dim, width, _ACTIVATIONS[activation], x.dtype, weight.dtype,
                                    False)
-    call_on(x.device, "sf_causal_conv1d_update", ptr(x), ptr(state), ptr(weight), ptr(bias), ptr(state_indices), ptr(y),
-            state.shape[0], desc)
-    return y
+    if all(a is b for a, b in zip((x, weight, bias), given)):
+        if len(_update_plans) >= 512:
+            _update_plans.clear()
+        _update_plans[key] = desc
+    return x, weight, bias, desc

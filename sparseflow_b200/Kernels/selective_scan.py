@@ -11,7 +11,7 @@ from typing import Optional
 import torch
 
 from .. import _lib
-from ._sequence import (call_on, check_dtype, check_offsets, check_shape, check_state_indices, needs_grad, ptr,
+from ._sequence import (call_on, check_dtype, check_offsets, check_shape, check_state_indices, dense, layout, needs_grad, ptr,
                         require_cuda, rows_of)
 
 _MAX_STATE = 128
@@ -20,34 +20,38 @@ _MAX_STATE = 128
 def _check(x, dt, A, B, C, D, z, dt_bias):
     """Checks the operands against x's leading dimensions; B and C get their group dimension. Returns
     (B, C, dim, state, groups)."""
-    lead, dim = x.shape[:-1], x.shape[-1]
+    shape, kind = x.shape, x.dtype
+    dim = shape[-1]
     if A.dim() != 2 or A.shape[0] != dim or not 1 <= A.shape[1] <= _MAX_STATE:
         raise ValueError(f"A: expected [{dim}, state] with 1 to {_MAX_STATE} states, got {list(A.shape)}")
     state = A.shape[1]
-    if B.dim() == x.dim():
+    if B.dim() == len(shape):
         B = B.unsqueeze(-2)
-    if C.dim() == x.dim():
+    if C.dim() == len(shape):
         C = C.unsqueeze(-2)
     groups = B.shape[-2] if B.dim() >= 2 else 0
     if groups < 1 or dim % groups:
         raise ValueError(f"B: {groups} groups do not divide {dim} channels")
-    check_shape("B", B, (*lead, groups, state))
-    check_shape("C", C, (*lead, groups, state))
-    check_shape("dt", dt, x.shape)
-    for name, t in (("dt", dt), ("B", B), ("C", C), ("z", z)):
-        if t is not None:
-            check_dtype(name, t, x.dtype)
+    inner = (*shape[:-1], groups, state)
+    check_shape("B", B, inner)
+    check_shape("C", C, inner)
+    check_shape("dt", dt, shape)
+    check_dtype("dt", dt, kind)
+    check_dtype("B", B, kind)
+    check_dtype("C", C, kind)
     if z is not None:
-        check_shape("z", z, x.shape)
-    for name, t in (("D", D), ("dt_bias", dt_bias)):
-        if t is not None:
-            check_shape(name, t, (dim,))
+        check_dtype("z", z, kind)
+        check_shape("z", z, shape)
+    if D is not None:
+        check_shape("D", D, (dim,))
+    if dt_bias is not None:
+        check_shape("dt_bias", dt_bias, (dim,))
     return B, C, dim, state, groups
 
 
 def _float(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """Parameters are read in 32 bits; autograd sees the cast."""
-    return None if t is None else t.float().contiguous()
+    return t if t is None or (t.dtype is torch.float32 and t.is_contiguous()) else t.float().contiguous()
 
 
 def _strided(x, dt, z, B, C):
@@ -69,14 +73,14 @@ def _forward(x, dt, A, B, C, D, z, dt_bias, initial_state, seq_offsets, softplus
     x, dt, z, B, C, strides = _strided(x, dt, z, B, C)
     desc = _lib.selective_scan_desc(length, strides, n_seq, dim, state, groups, softplus, x.dtype, packed)
     lib = _lib.load()
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     final = torch.empty(n_seq, dim, state, dtype=torch.float32, device=x.device) if want_final else None
     ck = None
     if want_checkpoints:
         ck = torch.empty(lib.sf_selective_scan_checkpoint_bytes(desc) // 4, dtype=torch.float32, device=x.device)
     nbytes = lib.sf_selective_scan_workspace_size(desc)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
-    call_on(x.device, "sf_selective_scan", ptr(x), ptr(dt), ptr(A), ptr(B), ptr(C), ptr(D), ptr(z), ptr(dt_bias),
+    call_on(x.get_device(), "sf_selective_scan", ptr(x), ptr(dt), ptr(A), ptr(B), ptr(C), ptr(D), ptr(z), ptr(dt_bias),
             ptr(initial_state), ptr(seq_offsets), ptr(y), ptr(final), ptr(ck), desc, ptr(ws), nbytes)
     return y, final, ck, desc, (x, dt, z, B, C)
 
@@ -107,7 +111,7 @@ class _SelectiveScan(torch.autograd.Function):
             dinit = torch.empty(ctx.state_shape, dtype=torch.float32, device=x.device)
         nbytes = _lib.load().sf_selective_scan_backward_workspace_size(ctx.desc)
         ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=x.device)
-        call_on(x.device, "sf_selective_scan_backward", ptr(x), ptr(dt), ptr(A), ptr(B), ptr(C), ptr(D), ptr(z),
+        call_on(x.get_device(), "sf_selective_scan_backward", ptr(x), ptr(dt), ptr(A), ptr(B), ptr(C), ptr(D), ptr(z),
                 ptr(dt_bias), ptr(seq_offsets), ptr(ck), ptr(dy), ptr(dfinal), ptr(dx), ptr(ddt), ptr(dA), ptr(dB),
                 ptr(dC), ptr(dD), ptr(dz), ptr(dbias), ptr(dinit), ctx.desc, ptr(ws), nbytes)
         return dx, ddt, dA, dB, dC, dD, dz, dbias, dinit, None, None, None
@@ -127,14 +131,13 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     ``dt_softplus``. States are fp32 [n_seq, dim, state]; the initial one is 0 if None. Returns y, or
     (y, final_state). Differentiable once, in every tensor but the offsets; gradients are the same from run to run.
     """
-    require_cuda(x=x, dt=dt, A=A, B=B, C=C, D=D, z=z, dt_bias=dt_bias, initial_state=initial_state,
-                 seq_offsets=seq_offsets)
+    require_cuda(x, dt, A, B, C, D, z, dt_bias, initial_state, seq_offsets)
     n_seq, _, _ = check_offsets(seq_offsets, x)
     B, C, dim, state, _ = _check(x, dt, A, B, C, D, z, dt_bias)
     if initial_state is not None:
         check_shape("initial_state", initial_state, (n_seq, dim, state))
         check_dtype("initial_state", initial_state, torch.float32)
-        initial_state = initial_state.contiguous()
+        initial_state = dense(initial_state)
     args = (x, dt, _float(A), B, C, _float(D), z, _float(dt_bias), initial_state, seq_offsets, bool(dt_softplus),
             bool(return_final_state))
     if needs_grad(x, dt, A, B, C, D, z, dt_bias, initial_state):
@@ -154,9 +157,31 @@ def selective_scan_update(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B:
     device, distinct), or slot i without indices; a row whose index is no slot is padding: its y is 0 and no state
     changes. Not differentiable.
     """
-    require_cuda(x=x, dt=dt, A=A, B=B, C=C, state=state, D=D, z=z, dt_bias=dt_bias, state_indices=state_indices)
+    require_cuda(x, dt, A, B, C, state, D, z, dt_bias, state_indices)
+    key = (x.shape, x.stride(), x.dtype, dt.shape, dt.stride(), dt.dtype, B.shape, B.stride(), B.dtype, C.shape,
+           C.stride(), C.dtype, layout(A), layout(state), layout(D), layout(z), layout(dt_bias), layout(state_indices),
+           dt_softplus)
+    desc = _update_plans.get(key)
+    if desc is None:
+        x, dt, A, B, C, D, z, dt_bias, desc = _update_plan(x, dt, A, B, C, state, D, z, dt_bias, dt_softplus,
+                                                           state_indices, key)
+    y = x.new_empty(x.shape)
+    call_on(x.get_device(), "sf_selective_scan_update", x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(),
+            C.data_ptr(), ptr(D), ptr(z), ptr(dt_bias), state.data_ptr(), ptr(state_indices), y.data_ptr(),
+            state.shape[0], desc)
+    return y
+
+
+# Descriptors of the layouts that single-token calls have come with, where nothing had to be copied: a decoding loop's
+# next call with the same layouts has passed its checks.
+_update_plans: dict = {}
+
+
+def _update_plan(x, dt, A, B, C, state, D, z, dt_bias, dt_softplus, state_indices, key):
+    """Checks a call and returns its operands as the kernel reads them and its descriptor."""
     if x.dim() != 2:
         raise ValueError(f"x: expected [rows, dim], got {list(x.shape)}")
+    given = (x, dt, A, B, C, D, z, dt_bias)
     B, C, dim, n, groups = _check(x, dt, A, B, C, D, z, dt_bias)
     if state.dim() != 3 or not state.is_contiguous():
         raise ValueError("state: expected a contiguous [slots, dim, state] tensor")
@@ -165,8 +190,11 @@ def selective_scan_update(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B:
     check_state_indices(state_indices, x.shape[0], state.shape[0])
     A, D, dt_bias = _float(A), _float(D), _float(dt_bias)
     x, dt, z, B, C, strides = _strided(x, dt, z, B, C)
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     desc = _lib.selective_scan_desc(1, strides, x.shape[0], dim, n, groups, bool(dt_softplus), x.dtype, False)
-    call_on(x.device, "sf_selective_scan_update", ptr(x), ptr(dt), ptr(A), ptr(B), ptr(C), ptr(D), ptr(z), ptr(dt_bias),
-            ptr(state), ptr(state_indices), ptr(y), state.shape[0], desc)
-    return y
+    args = (x, dt, A, B, C, D, z, dt_bias)
+    if all(a is b or (a is not None and a.data_ptr() == b.data_ptr() and a.dtype is b.dtype)
+           for a, b in zip(args, given)):
+        if len(_update_plans) >= 512:
+            _update_plans.clear()
+        _update_plans[key] = desc
+    return (*args, desc)

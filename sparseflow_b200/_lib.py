@@ -429,15 +429,15 @@ def lif_multistep_events(x: torch.Tensor, v: torch.Tensor, spikes: torch.Tensor,
 # Sequence operators
 # ----------------------------------------------------------------------------
 
-def call_on(device: torch.device, fn: str, *args) -> None:
-    """Calls an entry point whose last argument is the stream: the current one of `device`, whose
+def call_on(idx: int, fn: str, *args) -> None:
+    """Calls an entry point whose last argument is the stream: the current one of device `idx`, whose
     context is made current for the call where another device's is."""
-    idx = device.index if device.index is not None else torch.cuda.current_device()
-    if idx == torch.cuda.current_device():
-        st = getattr(load(), fn)(*args, raw_stream(idx))
+    lib = _lib if _lib is not None else load()
+    if idx == torch._C._cuda_getDevice():
+        st = getattr(lib, fn)(*args, raw_stream(idx))
     else:
         with torch.cuda.device(idx):
-            st = getattr(load(), fn)(*args, raw_stream(idx))
+            st = getattr(lib, fn)(*args, raw_stream(idx))
     if st != SF_OK:
         _check(fn, st)
 

@@ -35,44 +35,105 @@ __global__ void scan_sum_kernel(const float* part, long long count, long long n,
   out[i] = v;
 }
 
-template <typename T, int LPC>
+// Single tokens. Memory-bound: 32 bytes of states moved for 4 exponentials a lane. A lane has 4 states of one channel
+// for 4 rows, so that A (a third of the bytes of one row) is read once for all of them; what is per channel and row
+// (softplus, the gate) is done by one lane for each row and handed on by shuffles. All loads come before the first use
+// and without branches: rows of padding and channels past the end read a valid place and write nothing.
+// VEC: B and C rows can be read four elements at a time.
+template <typename T, int LPC, bool VEC>
 __global__ void __launch_bounds__(kThreads) scan_update_kernel(ScanArgs a, float* pool, const int32_t* idx,
                                                                int n_slots) {
-  constexpr int CH = kThreads / LPC;
-  const int row = blockIdx.x, q = threadIdx.x % LPC, n = q * kS;
-  const int d = blockIdx.y * CH + threadIdx.x / LPC;
-  const int slot = idx ? idx[row] : row;
-  const bool own = d < a.dim, live = own && slot >= 0 && slot < n_slots;
-  float y = 0.f;
-  if (live) {
-    const int g = d / (a.dim / a.groups);
-    float dt = DT<T>::to_f(static_cast<const T*>(a.dt)[(long long)row * a.dt_row + d]);
-    if (a.dt_bias) dt += a.dt_bias[d];
-    float e;
-    if (a.softplus) dt = softplus(dt, e);
-    const float x = DT<T>::to_f(static_cast<const T*>(a.x)[(long long)row * a.x_row + d]);
-    const T* Bp = static_cast<const T*>(a.B) + (long long)row * a.b_row + (long long)g * a.state;
-    const T* Cp = static_cast<const T*>(a.C) + (long long)row * a.c_row + (long long)g * a.state;
-    float A[kS], h[kS];
-    float* hp = pool + ((long long)slot * a.dim + d) * a.state;
-    load4(A, a.A + (long long)d * a.state, n, a.state);
-    load4(h, hp, n, a.state);
+  constexpr int CH = kThreads / LPC, RPL = kRowsPerLane<LPC>;
+  const int lane = threadIdx.x & 31, q = threadIdx.x % LPC, n = q * kS;
+  const int c = blockIdx.x * CH + threadIdx.x / LPC, d = min(c, a.dim - 1);
+  const int row0 = blockIdx.y * 4, rows = a.rows.n_seq, g = d / (a.dim / a.groups);
+  const int mine = scatter_row<LPC>(q);  // the first of this lane's RPL rows
+  int slot[4];
 #pragma unroll
-    for (int i = 0; i < kS; ++i)
-      if (n + i < a.state) {
-        h[i] = fmaf(ex2(dt * (A[i] * kLog2e)), h[i], dt * x * DT<T>::to_f(Bp[n + i]));
-        y = fmaf(DT<T>::to_f(Cp[n + i]), h[i], y);
+  for (int r = 0; r < 4; ++r) {
+    const int row = min(row0 + r, rows - 1);
+    slot[r] = idx ? idx[row] : row;
+    if (slot[r] >= n_slots || c >= a.dim || row0 + r >= rows) slot[r] = -1;
+  }
+  float h[4][kS], Bv[4][kS], Cv[4][kS], A[kS], x[RPL], dt[RPL], z[RPL];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const long long row = min(row0 + r, rows - 1);
+    load4(h[r], pool + ((long long)max(slot[r], 0) * a.dim + d) * a.state, n, a.state);
+    const T* Bp = static_cast<const T*>(a.B) + row * a.b_row + (long long)g * a.state;
+    const T* Cp = static_cast<const T*>(a.C) + row * a.c_row + (long long)g * a.state;
+    if (VEC) {  // the state is a multiple of 4; lanes past it have h = 0
+      const int m = min(n, a.state - kS);
+      seq::load_vec<T, kS>(Bv[r], Bp + m);
+      seq::load_vec<T, kS>(Cv[r], Cp + m);
+    } else {
+#pragma unroll
+      for (int i = 0; i < kS; ++i) {
+        Bv[r][i] = n + i < a.state ? DT<T>::to_f(Bp[n + i]) : 0.f;
+        Cv[r][i] = n + i < a.state ? DT<T>::to_f(Cp[n + i]) : 0.f;
       }
-    store4(hp, h, n, a.state);
-  }
-  y = lanes_sum<LPC>(y);
-  if (q == 0 && own) {
-    if (live) {
-      if (a.D) y = fmaf(a.D[d], DT<T>::to_f(static_cast<const T*>(a.x)[(long long)row * a.x_row + d]), y);
-      if (a.z) y *= seq::silu(DT<T>::to_f(static_cast<const T*>(a.z)[(long long)row * a.z_row + d]));
     }
-    static_cast<T*>(a.y)[(long long)row * a.dim + d] = DT<T>::from_f(y);
   }
+#pragma unroll
+  for (int l = 0; l < RPL; ++l) {
+    const long long row = min(row0 + mine + l, rows - 1);
+    dt[l] = DT<T>::to_f(static_cast<const T*>(a.dt)[row * a.dt_row + d]);
+    x[l] = DT<T>::to_f(static_cast<const T*>(a.x)[row * a.x_row + d]);
+    z[l] = a.z ? DT<T>::to_f(static_cast<const T*>(a.z)[row * a.z_row + d]) : 0.f;
+  }
+  load4(A, a.A + (long long)d * a.state, n, a.state);
+  const float bias = a.dt_bias ? a.dt_bias[d] : 0.f, D = a.D ? a.D[d] : 0.f;
+#pragma unroll
+  for (int i = 0; i < kS; ++i) A[i] *= kLog2e;
+  float u[RPL], y[4];
+#pragma unroll
+  for (int l = 0; l < RPL; ++l) {
+    float e;
+    dt[l] += bias;
+    if (a.softplus) dt[l] = softplus(dt[l], e);
+    u[l] = dt[l] * x[l];
+  }
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    float step, w;
+    if constexpr (LPC == 1) {
+      step = dt[r];
+      w = u[r];
+    } else {
+      const int from = (lane & ~(LPC - 1)) | r / RPL;
+      step = __shfl_sync(0xffffffffu, dt[r % RPL], from);
+      w = __shfl_sync(0xffffffffu, u[r % RPL], from);
+    }
+    y[r] = 0.f;
+#pragma unroll
+    for (int i = 0; i < kS; ++i) {
+      // A lane past the state (VEC) has read other states' B and C: its own stay 0.
+      const float b = VEC && LPC > 1 && n >= a.state ? 0.f : Bv[r][i];
+      h[r][i] = fmaf(ex2(step * A[i]), h[r][i], w * b);
+      y[r] = fmaf(Cv[r][i], h[r][i], y[r]);
+    }
+    if (slot[r] >= 0) store4(pool + ((long long)slot[r] * a.dim + d) * a.state, h[r], n, a.state);
+  }
+  float o[RPL];
+  scatter4<LPC>(o, y, q);
+  if ((LPC > 4 && q >= 4) || c >= a.dim) return;
+#pragma unroll
+  for (int l = 0; l < RPL; ++l) {
+    const int r = mine + l;
+    if (row0 + r >= rows) continue;
+    float v = fmaf(D, x[l], o[l]);
+    if (a.z) v *= seq::silu(z[l]);
+    const int s = idx ? idx[row0 + r] : row0 + r;
+    static_cast<T*>(a.y)[(long long)(row0 + r) * a.dim + d] = DT<T>::from_f(s >= 0 && s < n_slots ? v : 0.f);
+  }
+}
+
+template <typename T, int LPC, bool VEC>
+void run_update(const ScanArgs& a, float* pool, const int32_t* idx, int n_slots, cudaStream_t st) {
+  constexpr int CH = kThreads / LPC;
+  const unsigned tiles = (a.dim + CH - 1) / CH;
+  scan_update_kernel<T, LPC, VEC>
+      <<<dim3(tiles, (a.rows.n_seq + 3) / 4), kThreads, 0, st>>>(a, pool, idx, n_slots);
 }
 
 bool valid(const sf_selective_scan_desc* d) {
@@ -333,15 +394,17 @@ extern "C" sf_status sf_selective_scan_update(const void* x, const void* dt, con
   if (!valid(d) || !A || n_slots < 0) return SF_ERR_INVALID_ARG;
   if (d->state > kMaxState) return SF_ERR_UNSUPPORTED;
   if (d->n_seq == 0 || d->dim == 0) return SF_OK;
-  if (!x || !dt || !B || !C || !y || !state_pool) return SF_ERR_INVALID_ARG;
+  if (!x || !dt || !B || !C || !y || !state_pool || n_slots == 0) return SF_ERR_INVALID_ARG;
   ScanArgs a = base_args(x, dt, A, B, C, D, z, dt_bias, nullptr, d);
   a.y = y;
   if (!aligned16(A) || !aligned16(state_pool)) return SF_ERR_ALIGNMENT;
-  const int ch = kThreads / lanes(d->state);
-  const dim3 grid(d->n_seq, (d->dim + ch - 1) / ch);
-  if (grid.y > 65535) return SF_ERR_UNSUPPORTED;
+  if (d->n_seq > 65535) return SF_ERR_UNSUPPORTED;
+  const bool vec = d->state % 4 == 0 && d->b_row_stride % 4 == 0 && d->c_row_stride % 4 == 0 &&
+                   reinterpret_cast<uintptr_t>(B) % (4 * dtype_size(d->dtype)) == 0 &&
+                   reinterpret_cast<uintptr_t>(C) % (4 * dtype_size(d->dtype)) == 0;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  SF_SCAN_TYPES(d->dtype, SF_SCAN_LANES(d->state, (scan_update_kernel<T, L><<<grid, kThreads, 0, st>>>(
-                                                      a, state_pool, state_indices, n_slots))))
+  SF_SCAN_TYPES(d->dtype,
+                SF_SCAN_LANES(d->state, (vec ? run_update<T, L, true>(a, state_pool, state_indices, n_slots, st)
+                                             : run_update<T, L, false>(a, state_pool, state_indices, n_slots, st))))
   return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
 }
