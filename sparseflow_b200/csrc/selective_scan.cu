@@ -41,7 +41,7 @@ __global__ void scan_sum_kernel(const float* part, long long count, long long n,
 // and without branches: rows of padding and channels past the end read a valid place and write nothing.
 // VEC: B and C rows can be read four elements at a time.
 template <typename T, int LPC, bool VEC>
-__global__ void __launch_bounds__(kThreads) scan_update_kernel(ScanArgs a, float* pool, const int32_t* idx,
+__global__ void __launch_bounds__(kThreads, 8) scan_update_kernel(ScanArgs a, float* pool, const int32_t* idx,
                                                                int n_slots) {
   constexpr int CH = kThreads / LPC, RPL = kRowsPerLane<LPC>;
   const int lane = threadIdx.x & 31, q = threadIdx.x % LPC, n = q * kS;
