@@ -8,6 +8,10 @@ with thin multi-step wrappers: every layer takes [T, N, ...] tensors, convs
 and BN fold T into the batch (spikingjelly's ``step_mode='m'``), and
 ``LIFNode`` (Ops/lif_node.py) follows every BN. The wrappers subclass the
 torch layers, so ``optimize`` finds and replaces the convs as usual.
+
+``SpikingStateSpaceLM`` is the language model built from the sequence
+operators (no counterpart in the reference): prompts, single tokens and
+training run the causal convolution, the selective scan and the block norms.
 """
 from __future__ import annotations
 
@@ -16,7 +20,9 @@ from typing import List, Optional
 import torch
 import torch.nn as nn
 
+from .Kernels.block_norm import block_norm
 from .Ops.lif_node import LIFNode
+from .Ops.state_space import BlockNorm, StateSpaceMixer
 
 
 def _fold(x: torch.Tensor):
@@ -159,3 +165,46 @@ def spiking_cnn_small(num_classes: int = 10) -> nn.Module:
         MSConv2d(64, 128, 1), MSBatchNorm2d(128), LIFNode(),
         MSAvgPoolFlatten(), MSLinear(128, num_classes),
     )
+
+
+class SpikingStateSpaceLM(nn.Module):
+    """Embedding, blocks of a ``StateSpaceMixer`` between ``BlockNorm``s, and a head; the residual stream is fp32.
+
+    ``forward(tokens)`` gives the logits of [batch, length] tokens (for training with spiking=False). For serving,
+    ``prefill(tokens)`` also returns the blocks' states, and ``step(tokens, states)`` takes one token of each sequence
+    and updates them in place. With ``spiking=True`` every mixer ends in a LIF neuron and an event-driven projection;
+    its membranes belong to the batch that is being served (``reset_net`` before the next one).
+    """
+
+    def __init__(self, vocab: int, dim: int, layers: int, spiking: bool = False, **mixer):
+        super().__init__()
+        self.embedding = nn.Embedding(vocab, dim)
+        self.first_weight = nn.Parameter(torch.ones(dim))
+        self.mixers = nn.ModuleList(StateSpaceMixer(dim, spiking=spiking, **mixer) for _ in range(layers))
+        self.gates = nn.ModuleList(nn.Linear(dim, dim) for _ in range(layers))
+        self.norms = nn.ModuleList(BlockNorm(dim) for _ in range(layers))
+        self.head = nn.Linear(dim, vocab, bias=False)
+
+    def _run(self, tokens, mix):
+        """mix(i, normed) is the output of block i's mixer."""
+        residual, normed = block_norm(self.embedding(tokens), pre_weight=self.first_weight, residual_dtype=torch.float32)
+        for i, (gate, norm) in enumerate(zip(self.gates, self.norms)):
+            residual, normed = norm(mix(i, normed), residual, gate(normed))
+        return self.head(normed)
+
+    def forward(self, tokens: torch.Tensor, seq_offsets: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """tokens [batch, length], or [total] of packed sequences with ``seq_offsets``."""
+        return self._run(tokens, lambda i, x: self.mixers[i](x, seq_offsets))
+
+    def prefill(self, tokens: torch.Tensor):
+        """(logits, states) of prompts [batch, length]."""
+        states = [m.new_state(tokens.shape[0]) for m in self.mixers]
+
+        def mix(i, x):
+            out, states[i] = self.mixers[i](x, state=states[i])
+            return out
+        return self._run(tokens, mix), states
+
+    def step(self, tokens: torch.Tensor, states, state_indices: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Logits [rows, vocab] of one more token [rows] for each sequence."""
+        return self._run(tokens, lambda i, x: self.mixers[i].step(x, states[i], state_indices))
