@@ -538,7 +538,7 @@ struct FwdSmem {
 
 // One block: one segment of a sequence and CH channels of one group.
 template <typename T, int LPC, int CPT, bool VEC>
-__global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, CPT == 2 ? 4 : 3) scan_fwd_kernel(ScanArgs a) {
+__global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, 3) scan_fwd_kernel(ScanArgs a) {
   using F = Cfg<LPC, CPT>;
   extern __shared__ __align__(16) char smem[];
   FwdSmem<T, LPC, CPT, VEC>& s = *reinterpret_cast<FwdSmem<T, LPC, CPT, VEC>*>(smem);
