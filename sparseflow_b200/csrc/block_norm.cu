@@ -333,11 +333,11 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(NormArgs a, long long gr
 template <typename E>
 constexpr int kWords = sizeof(E) / 2;
 template <typename E>
-__device__ __forceinline__ void copy8(float4* slot, const void* row0, long long row, int c, bool in) {
-  const E* p = static_cast<const E*>(row0) + row + c;
+__device__ __forceinline__ void copy8(float4* slot, const void* base, long long at) {
+  const E* p = static_cast<const E*>(base) + at;
 #pragma unroll
   for (int h = 0; h < kWords<E>; ++h)
-    if (in) seq::cp_async(slot + h * blockDim.x + threadIdx.x, p + h * (16 / (int)sizeof(E)), 16, true);
+    seq::cp_async(slot + h * blockDim.x + threadIdx.x, p + h * (16 / (int)sizeof(E)), 16, true);
 }
 template <typename E>
 __device__ __forceinline__ void get8(u64 (&o)[4], const float4* slot) {
@@ -349,7 +349,7 @@ __device__ __forceinline__ void get8(u64 (&o)[4], const float4* slot) {
   for (int i = 0; i < 4; ++i) o[i] = pack2(DT<E>::to_f(e[2 * i]), DT<E>::to_f(e[2 * i + 1]));
 }
 template <typename E>
-__device__ __forceinline__ void put8(void* row0, long long row, int c, const u64 (&v)[4]) {
+__device__ __forceinline__ void put8(void* base, long long at, const u64 (&v)[4]) {
   E e[8];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -358,7 +358,7 @@ __device__ __forceinline__ void put8(void* row0, long long row, int c, const u64
     e[2 * i] = DT<E>::from_f(lo);
     e[2 * i + 1] = DT<E>::from_f(hi);
   }
-  float4* p = reinterpret_cast<float4*>(static_cast<E*>(row0) + row + c);
+  float4* p = reinterpret_cast<float4*>(static_cast<E*>(base) + at);
 #pragma unroll
   for (int h = 0; h < kWords<E>; ++h) __stcs(p + h, reinterpret_cast<const float4*>(e)[h]);
 }
@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(512, 2) norm_fwd_ring_kernel(NormArgs a) {
   using S = FwdRing<T, R>;
   extern __shared__ __align__(16) float4 ring[];
   const int c = threadIdx.x * kV, n = blockDim.x;
-  float(*buf)[16] = reinterpret_cast<float(*)[16]>(ring + S::STAGES * S::WORDS * n);
+  float(*buf)[32] = reinterpret_cast<float(*)[32]>(ring + S::STAGES * S::WORDS * n);
   const bool own = c < a.dim;
   const float inv = 1.f / (float)a.dim;
   constexpr bool gated = KIND != SF_GATE_NONE, curved = KIND == SF_GATE_SILU || KIND == SF_GATE_SIGMOID;
@@ -427,9 +427,12 @@ __global__ void __launch_bounds__(512, 2) norm_fwd_ring_kernel(NormArgs a) {
   auto load = [&]() {
     if (ahead < a.rows && own) {
       float4* s = ring + put * S::WORDS * n;
-      copy8<T>(s + S::Y * n, a.y, ahead * a.y_row, c, true);
-      if (gated) copy8<T>(s + S::GATE * n, a.gate, ahead / a.rows_per_gate * a.gate_row, c, true);
-      if (a.res) copy8<R>(s + S::RES * n, a.res, ahead * a.res_row, c, true);
+      copy8<T>(s + S::Y * n, a.y, ahead * a.y_row + c);
+      if (gated) {
+        const long long g = a.rows_per_gate == 1 ? ahead : ahead / a.rows_per_gate;
+        copy8<T>(s + S::GATE * n, a.gate, g * a.gate_row + c);
+      }
+      if (a.res) copy8<R>(s + S::RES * n, a.res, ahead * a.res_row + c);
     }
     seq::cp_async_commit();
     ahead += gridDim.x;
@@ -443,24 +446,31 @@ __global__ void __launch_bounds__(512, 2) norm_fwd_ring_kernel(NormArgs a) {
   for (int i = 0; i < 4; ++i) ws[i] = mul2(ws[i], wpre[i]);
   weights8(wpre, a.w_pre, c, a);
   const u64 alpha = both(a.alpha);
-  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
-    seq::cp_async_wait<S::STAGES - 2>();
-    const float4* s = ring + get * S::WORDS * n;
-    u64 r[4] = {0, 0, 0, 0};
-    if (own) get8<T>(r, s + S::Y * n);
-    float rstd1 = 1.f, sum[1];
-    if (a.w_post) {
-      u64 q = mul2(r[0], r[0]);
+  auto squares = [](const u64 (&v)[4]) {
+    u64 q = mul2(v[0], v[0]);
 #pragma unroll
-      for (int i = 1; i < 4; ++i) q = fma2(r[i], r[i], q);
-      sum[0] = seq::sum2(q);
-      ring_sum<1>(sum, buf, half);
-      rstd1 = rsqrtf(sum[0] * inv + a.eps);
-    }
+    for (int i = 1; i < 4; ++i) q = fma2(v[i], v[i], q);
+    return seq::sum2(q);
+  };
+  // One sum over the block for each row serves both norms: that of r' for this row and of y for the next. Its copies
+  // have come by then: a row is waited for a turn before its own.
+  u64 y[4] = {0, 0, 0, 0};
+  float sum[2] = {0.f, 0.f};  // r' of this row, y of the next
+  seq::cp_async_wait<S::STAGES - 2>();
+  if (own) {
+    get8<T>(y, ring + S::Y * n);
+    sum[1] = squares(y);
+  }
+  if (a.w_post) ring_sum<2>(sum, buf, half);
+  float rstd1 = a.w_post ? rsqrtf(sum[1] * inv + a.eps) : 1.f;
+  for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    const float4* s = ring + get * S::WORDS * n;
+    const long long at = row * a.dim + c;
+    u64 r[4] = {0, 0, 0, 0};
     if (own) {
       const u64 k = both(rstd1);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) r[i] = mul2(r[i], mul2(k, ws[i]));
+      for (int i = 0; i < 4; ++i) r[i] = mul2(y[i], mul2(k, ws[i]));
       if (gated) {
         u64 g[4];
         get8<T>(g, s + S::GATE * n);
@@ -473,29 +483,30 @@ __global__ void __launch_bounds__(512, 2) norm_fwd_ring_kernel(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) r[i] = fma2(alpha, t[i], r[i]);
       }
-      if (a.r_out) put8<R>(a.r_out, row * a.dim, c, r);
+      if (a.r_out) put8<R>(a.r_out, at, r);
     }
     get = get + 1 == S::STAGES ? 0 : get + 1;
     load();
-    float rstd2 = 1.f;
-    if (a.w_pre) {
-      u64 q = mul2(r[0], r[0]);
+    seq::cp_async_wait<S::STAGES - 2>();
+    sum[0] = squares(r);
+    sum[1] = 0.f;
+    if (own) {  // the next row's y; past the last row an earlier one's, which nothing comes of
+      get8<T>(y, ring + (get * S::WORDS + S::Y) * n);
+      sum[1] = squares(y);
+    }
+    if (a.w_post || a.w_pre) ring_sum<2>(sum, buf, half);
+    const float rstd2 = a.w_pre ? rsqrtf(sum[0] * inv + a.eps) : 1.f;
+    if (a.w_pre && own) {
+      const u64 k = both(rstd2);
 #pragma unroll
-      for (int i = 1; i < 4; ++i) q = fma2(r[i], r[i], q);
-      sum[0] = seq::sum2(q);
-      ring_sum<1>(sum, buf, half);
-      rstd2 = rsqrtf(sum[0] * inv + a.eps);
-      if (own) {
-        const u64 k = both(rstd2);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r[i] = mul2(r[i], mul2(k, wpre[i]));
-        put8<T>(a.x_out, row * a.dim, c, r);
-      }
+      for (int i = 0; i < 4; ++i) r[i] = mul2(r[i], mul2(k, wpre[i]));
+      put8<T>(a.x_out, at, r);
     }
     if (a.rstd && threadIdx.x == 0) {
       a.rstd[row] = rstd1;
       a.rstd[a.rows + row] = rstd2;
     }
+    if (a.w_post) rstd1 = rsqrtf(sum[1] * inv + a.eps);
   }
 }
 
@@ -524,11 +535,13 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long 
   auto load = [&]() {
     if (ahead < end && own) {
       float4* s = ring + put * S::WORDS * n;
-      copy8<T>(s + S::Y * n, a.y, ahead * a.y_row, c, true);
-      if (gated) copy8<T>(s + S::GATE * n, a.gate, ahead / a.rows_per_gate * a.gate_row, c, true);
-      if (a.res) copy8<R>(s + S::RES * n, a.res, ahead * a.res_row, c, true);
-      if (pre) copy8<T>(s + S::DX * n, a.dx, ahead * a.dim, c, true);
-      if (a.dr) copy8<R>(s + S::DR * n, a.dr, ahead * a.dim, c, true);
+      copy8<T>(s + S::Y * n, a.y, ahead * a.y_row + c);
+      // a gate row for many rows: one for the block's group
+      if (gated) copy8<T>(s + S::GATE * n, a.gate, (shared_gate ? (long long)blockIdx.y : ahead) * a.gate_row + c);
+      if (a.res) copy8<R>(s + S::RES * n, a.res, ahead * a.res_row + c);
+      const long long at = ahead * a.dim + c;
+      if (pre) copy8<T>(s + S::DX * n, a.dx, at);
+      if (a.dr) copy8<R>(s + S::DR * n, a.dr, at);
     }
     seq::cp_async_commit();
     ++ahead;
@@ -594,7 +607,8 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long 
         Q[i] = fma2(da, yh[i], Q[i]);
         o[i] = fma2(m1, yh[i], mul2(k1, mul2(ws[i], da)));
       }
-      put8<T>(a.dy, row * a.dim, c, o);
+      const long long at = row * a.dim + c;
+      put8<T>(a.dy, at, o);
       if (gated) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -605,13 +619,13 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long 
 #pragma unroll
           for (int i = 0; i < 4; ++i) ggate[i] = add2(ggate[i], o[i]);
         } else {
-          put8<T>(a.dgate, row * a.dim, c, o);
+          put8<T>(a.dgate, at, o);
         }
       }
       if (a.dres) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[i] = mul2(alpha, dt[i]);
-        put8<R>(a.dres, row * a.dim, c, o);
+        put8<R>(a.dres, at, o);
       }
     }
     get = get + 1 == S::STAGES ? 0 : get + 1;
@@ -619,9 +633,9 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long 
   }
   if (!own) return;
   const long long block = (long long)blockIdx.y * gridDim.x + blockIdx.x;
-  put8<float>(a.part_w + block * 2 * a.dim, 0, c, Q);
-  put8<float>(a.part_w + (block * 2 + 1) * a.dim, 0, c, gpre);
-  if (shared_gate) put8<float>(a.part_gate + block * a.dim, 0, c, ggate);
+  put8<float>(a.part_w, block * 2 * a.dim + c, Q);
+  put8<float>(a.part_w, (block * 2 + 1) * a.dim + c, gpre);
+  if (shared_gate) put8<float>(a.part_gate, block * a.dim + c, ggate);
 }
 
 // out[g][i] = factor[i] sum over j < blocks of part[g][j][stride] at i, to at most two outputs (a null output is left
@@ -721,7 +735,7 @@ sf_status run_fwd(const NormArgs& a, cudaStream_t st) {
   if (ring_fits(a)) {
     using S = FwdRing<T, R>;
     const int threads = threads_for(a.dim, 1);
-    const size_t smem = (size_t)S::STAGES * S::WORDS * threads * sizeof(float4) + 2 * 16 * sizeof(float);
+    const size_t smem = (size_t)S::STAGES * S::WORDS * threads * sizeof(float4) + 2 * 32 * sizeof(float);
     auto kernel = a.gate_kind == SF_GATE_NONE     ? norm_fwd_ring_kernel<T, R, SF_GATE_NONE>
                   : a.gate_kind == SF_GATE_LINEAR ? norm_fwd_ring_kernel<T, R, SF_GATE_LINEAR>
                   : a.gate_kind == SF_GATE_SILU   ? norm_fwd_ring_kernel<T, R, SF_GATE_SILU>
