@@ -65,10 +65,10 @@ class _BlockNorm(torch.autograd.Function):
         y, residual, gate, post_weight, pre_weight, scale, rstd = ctx.saved_tensors
 
         def like(t):
-            return None if t is None else _empty(t.shape, t.dtype, t.device)
+            return None if t is None else t.new_empty(t.shape)
 
-        dr = None if dr is None else dr.contiguous()
-        dx = None if dx is None else dx.contiguous()
+        dr = dense(dr)
+        dx = dense(dx)
         dy, dres, dgate, dpost, dpre, dscale = (like(t) for t in (y, residual, gate, post_weight, pre_weight, scale))
         nbytes = _lib.load().sf_block_norm_backward_workspace_size(ctx.desc)
         ws = _empty(max(nbytes, 1), torch.uint8, y.device)

@@ -52,9 +52,9 @@ class _CausalConv1d(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy, dfinal):
         x, weight, bias, initial_state, seq_offsets = ctx.saved_tensors
-        dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else dy.contiguous()
-        dfinal = None if dfinal is None else dfinal.contiguous()
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else dense(dy)
+        dfinal = dense(dfinal)
+        dx = x.new_empty(x.shape)
         dweight = torch.empty_like(weight)
         dbias = None if bias is None else torch.empty_like(bias)
         dinit = torch.empty_like(initial_state) if initial_state is not None and ctx.needs_input_grad[3] else None

@@ -74,10 +74,10 @@ def _forward(x, dt, A, B, C, D, z, dt_bias, initial_state, seq_offsets, softplus
     desc = _lib.selective_scan_desc(length, strides, n_seq, dim, state, groups, softplus, x.dtype, packed)
     lib = _lib.load()
     y = x.new_empty(x.shape)
-    final = torch.empty(n_seq, dim, state, dtype=torch.float32, device=x.device) if want_final else None
+    final = A.new_empty((n_seq, dim, state)) if want_final else None
     ck = None
     if want_checkpoints:
-        ck = torch.empty(lib.sf_selective_scan_checkpoint_bytes(desc) // 4, dtype=torch.float32, device=x.device)
+        ck = A.new_empty(lib.sf_selective_scan_checkpoint_bytes(desc) // 4)
     nbytes = lib.sf_selective_scan_workspace_size(desc)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device) if nbytes else None
     call_on(x.get_device(), "sf_selective_scan", ptr(x), ptr(dt), ptr(A), ptr(B), ptr(C), ptr(D), ptr(z), ptr(dt_bias),
@@ -101,14 +101,14 @@ class _SelectiveScan(torch.autograd.Function):
         x, dt, A, B, C, D, z, dt_bias, seq_offsets, ck = ctx.saved_tensors
 
         def like(t):
-            return None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
+            return None if t is None else t.new_empty(t.shape)
 
-        dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else dy.contiguous()
-        dfinal = None if dfinal is None else dfinal.contiguous()
+        dy = torch.zeros(x.shape, dtype=x.dtype, device=x.device) if dy is None else dense(dy)
+        dfinal = dense(dfinal)
         dx, ddt, dA, dB, dC, dD, dz, dbias = (like(t) for t in (x, dt, A, B, C, D, z, dt_bias))
         dinit = None
         if ctx.state_shape is not None and ctx.needs_input_grad[8]:
-            dinit = torch.empty(ctx.state_shape, dtype=torch.float32, device=x.device)
+            dinit = A.new_empty(ctx.state_shape)
         nbytes = _lib.load().sf_selective_scan_backward_workspace_size(ctx.desc)
         ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=x.device)
         call_on(x.get_device(), "sf_selective_scan_backward", ptr(x), ptr(dt), ptr(A), ptr(B), ptr(C), ptr(D), ptr(z),

@@ -639,13 +639,20 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long 
 }
 
 // out[g][i] = factor[i] sum over j < blocks of part[g][j][stride] at i, to at most two outputs (a null output is left
-// out, a null factor is 1). A warp has 32 values and each of the block's 8 warps every eighth block: a fixed order.
+// out, a null factor is 1); where blockIdx.z is 1, out2[i] = the sum over j of the n values after those.
+// A warp has 32 values and each of the block's 8 warps every eighth block: a fixed order.
 __global__ void __launch_bounds__(256) norm_reduce_kernel(const float* part, long long blocks, long long stride, int n,
                                                           int dtype, void* out0, const void* factor0, void* out1,
-                                                          const void* factor1, int factor_dtype) {
+                                                          const void* factor1, int factor_dtype, void* out2) {
   __shared__ float sums[8][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
   const float* p = part + (long long)blockIdx.y * blocks * stride + i;
+  if (blockIdx.z == 1) {
+    p += n;
+    out0 = out2;
+    factor0 = nullptr;
+    out1 = nullptr;
+  }
   float s = 0.f;
   if (i < n) {
 #pragma unroll 8
@@ -853,14 +860,11 @@ extern "C" sf_status sf_block_norm_backward(const void* y, const void* residual,
     if (status != SF_OK) return status;
   }
   const unsigned grid = (d->dim + 31) / 32;
-  if (d_post_weight || d_scale)
-    norm_reduce_kernel<<<grid, 256, 0, st>>>(part, blocks, 2ll * d->dim, d->dim, d->w_dtype, d_post_weight, scale, d_scale,
-                                             post_weight, d->w_dtype);
-  if (d_pre_weight)
-    norm_reduce_kernel<<<grid, 256, 0, st>>>(part + d->dim, blocks, 2ll * d->dim, d->dim, d->w_dtype, d_pre_weight,
-                                             nullptr, nullptr, nullptr, d->w_dtype);
+  if (d_post_weight || d_scale || d_pre_weight)
+    norm_reduce_kernel<<<dim3(grid, 1, 2), 256, 0, st>>>(part, blocks, 2ll * d->dim, d->dim, d->w_dtype, d_post_weight,
+                                                         scale, d_scale, post_weight, d->w_dtype, d_pre_weight);
   if (p.shared_gate && d_gate && d->rows > 0)
     norm_reduce_kernel<<<dim3(grid, (unsigned)p.groups), 256, 0, st>>>(a.part_gate, p.blocks, d->dim, d->dim, d->dtype,
-                                                                       d_gate, nullptr, nullptr, nullptr, d->w_dtype);
+                                                                       d_gate, nullptr, nullptr, nullptr, d->w_dtype, nullptr);
   return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
 }

@@ -25,13 +25,30 @@ __global__ void scan_bc_reduce_kernel(const float* part, long long rows, int til
   if (m < state) (i / NP % 2 ? dC : dB)[i / (2 * NP) * state + m] = DT<T>::from_f(v);
 }
 
-// out[i] = sum over j < count of part[j * n + i], in order.
-__global__ void scan_sum_kernel(const float* part, long long count, long long n, float* out) {
-  const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= n) return;
+// dA [na], dD and dbias [nd] (each may be null): sums over `count` segments of part_a [count][na] and part_d [2][count][nd],
+// in order.
+__global__ void scan_sum_kernel(const float* part_a, const float* part_d, long long count, long long na, long long nd,
+                                float* dA, float* dD, float* dbias) {
+  long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
+  const float* p = part_a;
+  float* out = dA;
+  long long n = na;
+  if (i >= na) {
+    i -= na;
+    n = nd;
+    p = part_d;
+    out = dD;
+    if (i >= nd) {
+      i -= nd;
+      p += count * nd;
+      out = dbias;
+    }
+    if (i >= nd) return;
+  }
+  if (!out) return;
   float v = 0.f;
 #pragma unroll 8
-  for (long long j = 0; j < count; ++j) v += part[j * n + i];
+  for (long long j = 0; j < count; ++j) v += p[j * n + i];
   out[i] = v;
 }
 
@@ -380,10 +397,8 @@ extern "C" sf_status sf_selective_scan_backward(const void* x, const void* dt, c
     }
   }
   const long long na = (long long)d->dim * d->state, nd = d->dim, count = some ? slots : 0;
-  scan_sum_kernel<<<(unsigned)((na + 127) / 128), 128, 0, st>>>(a.part_a, count, na, dA);
-  const unsigned gd = (unsigned)((nd + 127) / 128);
-  if (dD) scan_sum_kernel<<<gd, 128, 0, st>>>(a.part_d, count, nd, dD);
-  if (d_dt_bias) scan_sum_kernel<<<gd, 128, 0, st>>>(some ? a.part_d + slots * nd : nullptr, count, nd, d_dt_bias);
+  scan_sum_kernel<<<(unsigned)((na + 2 * nd + 127) / 128), 128, 0, st>>>(a.part_a, a.part_d, count, na, nd, dA, dD,
+                                                                         d_dt_bias);
   return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
 }
 
