@@ -10,6 +10,9 @@
 // sectors) and walks down a slot of rows with the last W rows in registers. The rows ahead are copied asynchronously
 // to a ring in shared memory, each thread its own, so no barrier guards it. Every x is read once, but for the W - 1
 // rows above each slot, which come from L2. Products and sums are pairs of fp32 (mul/fma .f32x2).
+// Measured (bf16, 16384 rows of 4096 channels, 4 taps, SiLU): forward 58 us, 4.6 TB/s; backward 106 + 10 us (sums),
+// 3.8 TB/s: 140 and 240 instructions for 8 channels of a warp's row at 0.6 a cycle, half of them the activation's
+// exponentials and divisions and 16-bit conversions.
 #include "sequence.cuh"
 
 namespace sf {

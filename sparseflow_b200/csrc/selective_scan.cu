@@ -172,15 +172,15 @@ int tiles_of(const sf_selective_scan_desc* d) {  // blocks for the channels of a
 // long alone on its SM as t[0], two or more together as t[1], t[2] ..; cut into about 1400 blocks in all, so that the
 // last round of them is short beside the rest, the time goes with the work, `cut` a block's sequence (the kernel that
 // finds the segments' shares included). Whole against cut, forward: 64 blocks 0.25 / 0.14, 128: 0.25 / 0.24, 192:
-// 0.33 / 0.36, 256: 0.33 / 0.48, 448: 0.62 / 0.83; backward: 128 blocks 0.76 / 0.52, 256: 1.02 / 0.96, 320: 1.29 / 1.16,
+// 0.33 / 0.36, 256: 0.33 / 0.48, 512: 0.58 / 0.95; backward: 128 blocks 0.76 / 0.52, 256: 1.02 / 0.96, 320: 1.29 / 1.16,
 // 384: 1.29 / 1.39, 512: 1.97 / 1.86. The cheaper is taken; 0.01 ms stands for the launch that cutting adds. Packed
 // sequences count as of equal length (the host does not know theirs).
 struct SegmentCosts {
   int resident;  // blocks on an SM
-  double t[3], cut;
+  double t[4], cut;
 };
-constexpr SegmentCosts kFwdCosts = {3, {0.250, 0.327, 0.430}, 1.86e-3};
-constexpr SegmentCosts kBwdCosts = {3, {0.750, 1.000, 1.290}, 3.62e-3};
+constexpr SegmentCosts kFwdCosts = {4, {0.250, 0.327, 0.430, 0.580}, 1.86e-3};
+constexpr SegmentCosts kBwdCosts = {3, {0.750, 1.000, 1.290, 0.}, 3.62e-3};
 
 long long segment_rows(const sf_selective_scan_desc* d, const SegmentCosts& k) {
   if (d->n_seq == 0 || d->length == 0) return kWhole;

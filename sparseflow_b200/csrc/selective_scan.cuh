@@ -13,11 +13,18 @@
 // (mul/fma .f32x2) halve the multiply-adds, and everything that is per channel and row, not per state (softplus,
 // the gate, D x), is done once, by the thread that loads the element, and handed on through shared memory.
 //
-// Layout: a lane owns 4 states of one channel; the LPC = ceil(state / 4) (a power of two) lanes of a channel lie
-// next to each other. A block takes CH = 64 channels of one group (fewer above 16 states) through a segment of the
-// rows, 16 rows a tile; tile t+1 is on its way to registers while tile t is worked on. Sums over the states end in
-// a reduce-scatter over four rows and the lanes of a channel, so each lane finishes other rows.
-// States past `state` have A = B = C = 0 and stay 0; rows past the end have dt = x = 0 and change nothing.
+// Layout: a lane owns 4 states of each of two channels; the LPC = ceil(state / 4) (a power of two) lanes of a channel lie
+// next to each other. B and C, read once for both channels, and the sums over channels that gB and gC need are then half
+// as dear; with one channel a lane shared memory was the bound (14 wavefronts a row of 8 channels). A block takes CH =
+// 64 channels of one group (fewer above 16 states) through a segment of the rows, 16 rows a tile, while the tiles ahead
+// are copied to a ring. Sums over the states end in a reduce-scatter over four rows and the lanes of a channel, so
+// each lane finishes other rows. States past `state` have A = B = C = 0 and stay 0; rows past the end have dt = x = 0
+// and change nothing.
+//
+// Measured (bf16, 16 states, 8192 rows of 4096 channels as 4 sequences, 537 M state steps; the exponentials alone take
+// 119 us): forward 0.33 ms, backward 0.97 ms. Forward 38 instructions a warp and row of 8 channels and 5.3 exponentials
+// or reciprocals (8 cycles each) at 0.52 instructions a cycle; backward 109 at 0.56: bound by the latency of each
+// warp's chain, of which registers allow 12 an SM.
 //
 // Few channels and long sequences leave most of the GPU idle, so sequences are cut into segments: a first kernel
 // finds what each segment adds to a state of 0 and how much it decays one (exp(A sum dt)), and the second starts
@@ -536,9 +543,11 @@ struct FwdSmem {
   Ring<T, LPC, CPT, VEC, true, true, false, true, true, STAGES> ring;
 };
 
-// One block: one segment of a sequence and CH channels of one group.
-template <typename T, int LPC, int CPT, bool VEC>
-__global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, 3) scan_fwd_kernel(ScanArgs a) {
+// One block: one segment of a sequence and CH channels of one group. BLOCKS on an SM: three have the registers to load
+// ahead over a whole tile, four hide more latency where there are as many (2048 rows, 256 blocks 0.33 / 0.38 ms, 384
+// 0.43 / 0.48, 512 0.61 / 0.58).
+template <typename T, int LPC, int CPT, bool VEC, int BLOCKS>
+__global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, BLOCKS) scan_fwd_kernel(ScanArgs a) {
   using F = Cfg<LPC, CPT>;
   extern __shared__ __align__(16) char smem[];
   FwdSmem<T, LPC, CPT, VEC>& s = *reinterpret_cast<FwdSmem<T, LPC, CPT, VEC>*>(smem);
@@ -726,7 +735,7 @@ __device__ __forceinline__ int sums_first(int lane) {
 // over the tiles by scan_bc_reduce_kernel; sums over a segment of gA, gD and gbias to part_a / part_d, added over
 // the segments by scan_sum_kernel. No atomics: the order of every sum is fixed.
 template <typename T, int LPC, int CPT, bool VEC>
-__global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, CPT == 2 ? 3 : 2) scan_bwd_kernel(ScanArgs a) {
+__global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, 3) scan_bwd_kernel(ScanArgs a) {
   using F = Cfg<LPC, CPT>;
   extern __shared__ __align__(16) char smem[];
   BwdSmem<T, LPC, CPT, VEC>& s = *reinterpret_cast<BwdSmem<T, LPC, CPT, VEC>*>(smem);
@@ -1002,8 +1011,10 @@ sf_status run_fwd(const ScanArgs& a, dim3 grid, cudaStream_t st) {
     scan_carry_kernel<T, LPC, CPT, VEC, false><<<grid, threads, bytes, st>>>(a);
   }
   constexpr size_t smem = sizeof(FwdSmem<T, LPC, CPT, VEC>);
-  if (!prepare_smem(scan_fwd_kernel<T, LPC, CPT, VEC>, smem)) return SF_ERR_CUDA;
-  scan_fwd_kernel<T, LPC, CPT, VEC><<<grid, threads, smem, st>>>(a);
+  auto kernel = (long long)grid.x * grid.y > 3 * 148 ? scan_fwd_kernel<T, LPC, CPT, VEC, 4>
+                                                     : scan_fwd_kernel<T, LPC, CPT, VEC, 3>;
+  if (!prepare_smem(kernel, smem)) return SF_ERR_CUDA;
+  kernel<<<grid, threads, smem, st>>>(a);
   return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
 }
 template <typename T, int LPC, int CPT, bool VEC>
