@@ -21,8 +21,10 @@
 // registers, while the rows ahead are copied asynchronously to a ring in shared memory, each thread its own channels
 // (no barrier guards the ring). Measured (bf16, fp32 residual, 8192 rows of 4096 channels, SiLU gate): forward 93 us, 4.9
 // TB/s; backward 178 us, 4.1 TB/s: one block of 512 threads fills an SM's registers, so nothing covers the sum over
-// the block between the two halves of a row. Rows of more than kRingDim channels, or that 16-byte copies do not fit, take the
-// kernels without a ring, which read them twice where registers do not hold them.
+// the block between the two halves of a row. Rows of more than kRingDim channels are shared backward by a cluster of two
+// or four blocks, which add up through each other's shared memory. Rows that 16-byte copies do not fit, and wider rows
+// forward, take the kernels without a ring.
+#include <cooperative_groups.h>
 #include "sequence.cuh"
 
 namespace sf {
@@ -36,7 +38,7 @@ using seq::u64;
 using seq::unpack2;
 
 constexpr int kV = 8;             // channels per vector: 16 bytes of a 16-bit type
-constexpr int kRingDim = 4096;    // 512 threads
+constexpr int kRingDim = 4096;    // channels of a row in a block of 512 threads
 constexpr int kMaxDim = 16384;    // 1024 threads, two vectors each
 
 struct NormArgs {
@@ -50,6 +52,7 @@ struct NormArgs {
   int dim, w_dtype, gate_kind;
   float alpha, eps;
   int vec;  // whether every row of every tensor takes vector accesses
+  int cluster, slice;  // kernels with a ring: blocks that share a row, channels of it in each
 };
 
 // 8 channels from column c on as floats; past dim: 0.
@@ -150,6 +153,7 @@ __global__ void __launch_bounds__(1024) norm_fwd_kernel(NormArgs a) {
   const float inv = 1.f / (float)a.dim;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const T* yp = static_cast<const T*>(a.y) + row * a.y_row;
+    const long long gate_row = a.rows_per_gate == 1 ? row : row / a.rows_per_gate;
     float r[K][kV];
     float s1[1] = {0.f};
 #pragma unroll
@@ -179,8 +183,9 @@ __global__ void __launch_bounds__(1024) norm_fwd_kernel(NormArgs a) {
 #pragma unroll
         for (int i = 0; i < kV; ++i) r[k][i] *= t[i];
       }
+      // Loaded only now: with gate and residual in registers one block of 1024 threads fills an SM (0.28 against 0.20 ms).
       if (a.gate_kind != SF_GATE_NONE) {
-        load8<T>(t, static_cast<const T*>(a.gate) + row / a.rows_per_gate * a.gate_row, c, a.dim, a.vec);
+        load8<T>(t, static_cast<const T*>(a.gate) + gate_row * a.gate_row, c, a.dim, a.vec);
 #pragma unroll
         for (int i = 0; i < kV; ++i) r[k][i] *= gate_act(t[i], a.gate_kind);
       }
@@ -387,27 +392,56 @@ __device__ __forceinline__ u64 dact2(u64 g, u64 sig) {
   return KIND == SF_GATE_SILU ? mul2(sig, fma2(g, rest, both(1.f))) : mul2(sig, rest);
 }
 
-// Sums over the block with one barrier: `buf` alternates between two halves, so the sum before may still be read.
+// Sums over the block, or over the cluster's blocks that share a row, with one barrier: every warp writes its sums to
+// all blocks of the cluster. `buf` alternates between two halves, so the sum before may still be read.
+constexpr int kMaxCluster = 4;
 template <int N>
-__device__ __forceinline__ void ring_sum(float (&v)[N], float (*buf)[16 * N], int& half) {
+using SumBuf = float[16 * kMaxCluster * N];
+template <int N>
+__device__ __forceinline__ void ring_sum(float (&v)[N], SumBuf<N>* buf, int& half, int cluster) {
 #pragma unroll
   for (int n = 0; n < N; ++n)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
   const int warps = blockDim.x >> 5, w = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (warps == 1) return;
-  if (lane == 0)
+  float s[N];
+  if (cluster == 1) {
+    if (warps == 1) return;
+    if (lane == 0)
 #pragma unroll
-    for (int n = 0; n < N; ++n) buf[half][w * N + n] = v[n];
-  __syncthreads();
+      for (int n = 0; n < N; ++n) buf[half][w * N + n] = v[n];
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < N; ++n) s[n] = lane < warps ? buf[half][lane * N + n] : 0.f;
+  } else {
+    const auto g = cooperative_groups::this_cluster();
+    if (lane < cluster) {
+      float* to = g.map_shared_rank(&buf[half][0], lane) + (g.block_rank() * warps + w) * N;
+#pragma unroll
+      for (int n = 0; n < N; ++n) to[n] = v[n];
+    }
+    g.sync();
+#pragma unroll
+    for (int n = 0; n < N; ++n) s[n] = 0.f;
+    for (int i = lane; i < cluster * warps; i += 32)
+#pragma unroll
+      for (int n = 0; n < N; ++n) s[n] += buf[half][i * N + n];
+  }
 #pragma unroll
   for (int n = 0; n < N; ++n) {
-    float s = lane < warps ? buf[half][lane * N + n] : 0.f;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    v[n] = __shfl_sync(0xffffffffu, s, 0);
+    for (int o = 16; o > 0; o >>= 1) s[n] += __shfl_xor_sync(0xffffffffu, s[n], o);
+    v[n] = s[n];
   }
   half ^= 1;
+}
+// This block's channels: the first of the thread's eight, and whether they lie in the row. In a cluster, waits until
+// all its blocks run, whose shared memory the sums are written to.
+__device__ __forceinline__ int ring_channel(const NormArgs& a, bool& own) {
+  const int local = threadIdx.x * kV, c = (int)(blockIdx.x % a.cluster) * a.slice + local;
+  own = local < a.slice && c < a.dim;
+  if (a.cluster > 1) cooperative_groups::this_cluster().sync();
+  return c;
 }
 
 template <typename T, typename R>
@@ -420,8 +454,8 @@ __global__ void __launch_bounds__(512, 2) norm_fwd_ring_kernel(NormArgs a) {
   using S = FwdRing<T, R>;
   extern __shared__ __align__(16) float4 ring[];
   const int c = threadIdx.x * kV, n = blockDim.x;
-  float(*buf)[32] = reinterpret_cast<float(*)[32]>(ring + S::STAGES * S::WORDS * n);
   const bool own = c < a.dim;
+  SumBuf<2>* buf = reinterpret_cast<SumBuf<2>*>(ring + S::STAGES * S::WORDS * n);
   const float inv = 1.f / (float)a.dim;
   constexpr bool gated = KIND != SF_GATE_NONE, curved = KIND == SF_GATE_SILU || KIND == SF_GATE_SIGMOID;
   long long ahead = blockIdx.x;
@@ -463,7 +497,7 @@ __global__ void __launch_bounds__(512, 2) norm_fwd_ring_kernel(NormArgs a) {
     get8<T>(y, ring + S::Y * n);
     sum[1] = squares(y);
   }
-  if (a.w_post) ring_sum<2>(sum, buf, half);
+  if (a.w_post) ring_sum<2>(sum, buf, half, 1);
   float rstd1 = a.w_post ? rsqrtf(sum[1] * inv + a.eps) : 1.f;
   for (long long row = blockIdx.x; row < a.rows; row += gridDim.x) {
     const float4* s = ring + get * S::WORDS * n;
@@ -496,7 +530,7 @@ __global__ void __launch_bounds__(512, 2) norm_fwd_ring_kernel(NormArgs a) {
       get8<T>(y, ring + (get * S::WORDS + S::Y) * n);
       sum[1] = squares(y);
     }
-    if (a.w_post || a.w_pre) ring_sum<2>(sum, buf, half);
+    if (a.w_post || a.w_pre) ring_sum<2>(sum, buf, half, 1);
     const float rstd2 = a.w_pre ? rsqrtf(sum[0] * inv + a.eps) : 1.f;
     if (a.w_pre && own) {
       const u64 k = both(rstd2);
@@ -523,14 +557,14 @@ template <typename T, typename R, int KIND>
 __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long long group_rows, long long per) {
   using S = BwdRing<T, R>;
   extern __shared__ __align__(16) float4 ring[];
-  const int c = threadIdx.x * kV, n = blockDim.x;
-  float(*buf)[48] = reinterpret_cast<float(*)[48]>(ring + S::STAGES * S::WORDS * n);
-  const bool own = c < a.dim;
+  bool own;
+  const int c = ring_channel(a, own), n = blockDim.x;
+  SumBuf<3>* buf = reinterpret_cast<SumBuf<3>*>(ring + S::STAGES * S::WORDS * n);
   const float inv = 1.f / (float)a.dim;
   constexpr bool gated = KIND != SF_GATE_NONE, curved = KIND == SF_GATE_SILU || KIND == SF_GATE_SIGMOID;
   const bool shared_gate = a.part_gate != nullptr, pre = a.w_pre && a.dx;
   const long long first = (long long)blockIdx.y * group_rows;
-  const long long begin = first + blockIdx.x * per, end = min(begin + per, first + group_rows);
+  const long long begin = first + blockIdx.x / a.cluster * per, end = min(begin + per, first + group_rows);
   long long ahead = begin;
   int put = 0, get = 0, half = 0;
   float next1 = 1.f, next2 = 0.f;
@@ -597,7 +631,7 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long 
       }
       sum[0] = seq::sum2(s0), sum[1] = seq::sum2(s1), sum[2] = seq::sum2(s2);
     }
-    ring_sum<3>(sum, buf, half);
+    ring_sum<3>(sum, buf, half, a.cluster);
     const float c2 = sum[0] * inv * rstd2, c1 = a.w_post ? (sum[1] - c2 * sum[2]) * inv : 0.f;
     if (own) {
       const u64 m2 = both(-c2), m1 = both(-c1 * rstd1);
@@ -634,7 +668,7 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long 
     load();
   }
   if (!own) return;
-  const long long block = (long long)blockIdx.y * gridDim.x + blockIdx.x;
+  const long long block = ((long long)blockIdx.y * gridDim.x + blockIdx.x) / a.cluster;
   put8<float>(a.part_w, block * 2 * a.dim + c, Q);
   put8<float>(a.part_w, (block * 2 + 1) * a.dim + c, gpre);
   if (shared_gate) put8<float>(a.part_gate, block * a.dim + c, ggate);
@@ -693,9 +727,17 @@ int threads_for(int dim, int K) {
   return (t + 31) / 32 * 32;
 }
 
-// Blocks that fill the GPU: rows of up to kRingDim channels, 512 threads an SM backward (about 110 registers each) and
-// 1024 forward; wider ones, one row in 1024 threads.
-long long bwd_blocks(int dim) { return dim <= kRingDim ? 148ll * (512 / threads_for(dim, 1)) : 296; }
+// Blocks that share a row in the kernels with a ring, as a cluster, and the channels of each.
+int cluster_of(int dim) { return dim <= kRingDim ? 1 : dim <= 2 * kRingDim ? 2 : kMaxCluster; }
+int slice_of(int dim) {
+  const int cl = cluster_of(dim);
+  return (dim + cl * kV - 1) / (cl * kV) * kV;
+}
+// Rows at work at a time that fill the GPU: 512 threads an SM backward (about 126 registers each), 1024 forward.
+long long rows_at_work(int dim, int threads_per_sm) {
+  const long long rows = 148ll * (threads_per_sm / threads_for(slice_of(dim), 1)) / cluster_of(dim);
+  return rows < 1 ? 1 : rows;
+}
 
 struct BwdPlan {
   long long groups, group_rows, blocks, per;
@@ -706,7 +748,8 @@ BwdPlan bwd_plan(const sf_block_norm_desc* d) {
   p.shared_gate = d->gate_kind != SF_GATE_NONE && d->rows_per_gate > 1;
   p.groups = p.shared_gate ? d->rows / d->rows_per_gate : 1;
   p.group_rows = p.shared_gate ? d->rows_per_gate : d->rows;
-  const long long want = bwd_blocks(d->dim);
+  // Wide rows that no ring takes: blocks of up to 1024 threads, two an SM.
+  const long long want = d->dim % kV && d->dim > kRingDim ? 296 : rows_at_work(d->dim, 512);
   long long blocks = (want + p.groups - 1) / p.groups;
   if (blocks > p.group_rows) blocks = p.group_rows;
   if (blocks < 1) blocks = 1;
@@ -732,27 +775,51 @@ NormArgs base_args(const void* y, const void* residual, const void* gate, const 
   a.dim = d->dim;
   a.w_dtype = d->w_dtype;
   a.gate_kind = d->gate_kind;
+  a.cluster = cluster_of(d->dim);
+  a.slice = slice_of(d->dim);
   a.alpha = d->residual_scale;
   a.eps = d->eps;
   return a;
 }
 
-bool ring_fits(const NormArgs& a) { return a.vec && a.dim <= kRingDim; }
+// Launches a kernel with a ring on a grid of rows at work (and groups), a cluster for each row of several blocks.
+template <typename K, typename... Args>
+sf_status launch_ring(K kernel, const NormArgs& a, long long rows, long long groups, size_t words, int sums,
+                      cudaStream_t st, Args... args) {
+  const int threads = threads_for(a.slice, 1);
+  const size_t smem = words * threads * sizeof(float4) + 2 * 16 * kMaxCluster * sums * sizeof(float);
+  if (smem > 48 * 1024 && !allow_max_smem(reinterpret_cast<const void*>(kernel))) return SF_ERR_CUDA;
+  const dim3 grid((unsigned)(rows * a.cluster), (unsigned)groups);
+  if (a.cluster == 1) {
+    kernel<<<grid, threads, smem, st>>>(a, args...);
+    return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
+  }
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = a.cluster;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, a, args...) == cudaSuccess ? SF_OK : SF_ERR_CUDA;
+}
 
 template <typename T, typename R>
 sf_status run_fwd(const NormArgs& a, cudaStream_t st) {
-  if (ring_fits(a)) {
+  // Wider rows: the barrier of a cluster costs more than the ring gives (8192 rows of 8192 channels: 0.24 ms in
+  // clusters of two, 0.20 ms without a ring; backward 0.44 against 0.68 ms).
+  if (a.vec && a.cluster == 1) {
     using S = FwdRing<T, R>;
-    const int threads = threads_for(a.dim, 1);
-    const size_t smem = (size_t)S::STAGES * S::WORDS * threads * sizeof(float4) + 2 * 32 * sizeof(float);
     auto kernel = a.gate_kind == SF_GATE_NONE     ? norm_fwd_ring_kernel<T, R, SF_GATE_NONE>
                   : a.gate_kind == SF_GATE_LINEAR ? norm_fwd_ring_kernel<T, R, SF_GATE_LINEAR>
                   : a.gate_kind == SF_GATE_SILU   ? norm_fwd_ring_kernel<T, R, SF_GATE_SILU>
                                                   : norm_fwd_ring_kernel<T, R, SF_GATE_SIGMOID>;
-    if (smem > 48 * 1024 && !allow_max_smem(reinterpret_cast<const void*>(kernel))) return SF_ERR_CUDA;
-    const long long most = 148ll * (1024 / threads);
-    kernel<<<(unsigned)(a.rows < most ? a.rows : most), threads, smem, st>>>(a);
-    return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
+    const long long most = rows_at_work(a.dim, 1024);
+    return launch_ring(kernel, a, a.rows < most ? a.rows : most, 1, S::STAGES * S::WORDS, 2, st);
   }
   const int K = vectors_per_thread(a.dim), threads = threads_for(a.dim, K);
   const unsigned grid = (unsigned)(a.rows < INT32_MAX ? a.rows : INT32_MAX);
@@ -762,17 +829,13 @@ sf_status run_fwd(const NormArgs& a, cudaStream_t st) {
 }
 template <typename T, typename R>
 sf_status run_bwd(const NormArgs& a, const BwdPlan& p, cudaStream_t st) {
-  if (ring_fits(a)) {
+  if (a.vec) {
     using S = BwdRing<T, R>;
-    const int threads = threads_for(a.dim, 1);
-    const size_t smem = (size_t)S::STAGES * S::WORDS * threads * sizeof(float4) + 2 * 48 * sizeof(float);
     auto kernel = a.gate_kind == SF_GATE_NONE     ? norm_bwd_ring_kernel<T, R, SF_GATE_NONE>
                   : a.gate_kind == SF_GATE_LINEAR ? norm_bwd_ring_kernel<T, R, SF_GATE_LINEAR>
                   : a.gate_kind == SF_GATE_SILU   ? norm_bwd_ring_kernel<T, R, SF_GATE_SILU>
                                                   : norm_bwd_ring_kernel<T, R, SF_GATE_SIGMOID>;
-    if (smem > 48 * 1024 && !allow_max_smem(reinterpret_cast<const void*>(kernel))) return SF_ERR_CUDA;
-    kernel<<<dim3((unsigned)p.blocks, (unsigned)p.groups), threads, smem, st>>>(a, p.group_rows, p.per);
-    return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
+    return launch_ring(kernel, a, p.blocks, p.groups, S::STAGES * S::WORDS, 3, st, p.group_rows, p.per);
   }
   // The kernel wants about 90 registers with one vector a thread and 160 with two.
   const int K = a.dim > 512 * kV ? 2 : 1, threads = threads_for(a.dim, K);
