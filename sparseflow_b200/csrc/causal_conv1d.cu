@@ -700,7 +700,7 @@ extern "C" sf_status sf_causal_conv1d_update(const void* x, void* state_pool, co
                                              const sf_causal_conv1d_desc* d, void* stream) {
   if (!valid(d) || !weight || n_slots < 0) return SF_ERR_INVALID_ARG;
   if (d->n_seq == 0 || d->dim == 0) return SF_OK;
-  if (!x || !y || !state_pool) return SF_ERR_INVALID_ARG;
+  if (!x || !y || (!state_pool && n_slots > 0)) return SF_ERR_INVALID_ARG;
   ConvArgs a = base_args(x, weight, bias, nullptr, nullptr, d);
   a.y = y;
   const bool fit = vectors_fit(bwd_vec(d), d, false, {x, state_pool, y});

@@ -76,7 +76,6 @@ __global__ void __launch_bounds__(kThreads, 8) scan_update_kernel(ScanArgs a, fl
 #pragma unroll
   for (int r = 0; r < 4; ++r) {
     const long long row = min(row0 + r, rows - 1);
-    load4(h[r], pool + ((long long)max(slot[r], 0) * a.dim + d) * a.state, n, a.state);
     const T* Bp = static_cast<const T*>(a.B) + row * a.b_row + (long long)g * a.state;
     const T* Cp = static_cast<const T*>(a.C) + row * a.c_row + (long long)g * a.state;
     if (VEC) {  // the state is a multiple of 4; lanes past it have h = 0
@@ -100,6 +99,10 @@ __global__ void __launch_bounds__(kThreads, 8) scan_update_kernel(ScanArgs a, fl
   }
   load4(A, a.A + (long long)d * a.state, n, a.state);
   const float bias = a.dt_bias ? a.dt_bias[d] : 0.f, D = a.D ? a.D[d] : 0.f;
+  // The states last: their addresses wait for the slots.
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    load4(h[r], pool + ((long long)max(slot[r], 0) * a.dim + d) * a.state, n, a.state);
 #pragma unroll
   for (int i = 0; i < kS; ++i) A[i] *= kLog2e;
   float u[RPL], y[4];
@@ -409,7 +412,12 @@ extern "C" sf_status sf_selective_scan_update(const void* x, const void* dt, con
   if (!valid(d) || !A || n_slots < 0) return SF_ERR_INVALID_ARG;
   if (d->state > kMaxState) return SF_ERR_UNSUPPORTED;
   if (d->n_seq == 0 || d->dim == 0) return SF_OK;
-  if (!x || !dt || !B || !C || !y || !state_pool || n_slots == 0) return SF_ERR_INVALID_ARG;
+  if (!x || !dt || !B || !C || !y || (!state_pool && n_slots > 0)) return SF_ERR_INVALID_ARG;
+  if (n_slots == 0)  // every row is padding
+    return cudaMemsetAsync(y, 0, (size_t)d->n_seq * d->dim * dtype_size(d->dtype), static_cast<cudaStream_t>(stream)) ==
+                   cudaSuccess
+               ? SF_OK
+               : SF_ERR_CUDA;
   ScanArgs a = base_args(x, dt, A, B, C, D, z, dt_bias, nullptr, d);
   a.y = y;
   if (!aligned16(A) || !aligned16(state_pool)) return SF_ERR_ALIGNMENT;

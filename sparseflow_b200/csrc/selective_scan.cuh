@@ -180,13 +180,13 @@ __device__ __forceinline__ int entry(int c) { return c ^ ((c >> 3) & 2); }
 
 template <bool VEC, typename T>
 __device__ __forceinline__ void store_unit(T* p, const seq::Vec<T, 4>& v, int valid) {
-  if (VEC) {
+  if constexpr (VEC) {
     if (valid > 0) *reinterpret_cast<seq::Vec<T, 4>*>(p) = v;
-    return;
-  }
+  } else {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (i < valid) p[i] = v.v[i];
+    for (int i = 0; i < 4; ++i)
+      if (i < valid) p[i] = v.v[i];
+  }
 }
 
 // The block's place: its group and channels; the lane's CPT channels, CH / CPT apart.

@@ -299,3 +299,16 @@ def test_c_entry_refuses():
     assert call(desc(state=129)) == _lib.SF_ERR_UNSUPPORTED
     assert lib.sf_selective_scan_backward(*([p] * 5), None, None, None, None, p, p, None, p, p, p, p, p, None, None, None,
                                           None, desc(), None, 0, None) == _lib.SF_ERR_WORKSPACE
+
+
+def test_pool_without_slots_is_all_padding():
+    from sparseflow_b200.Kernels.causal_conv1d import causal_conv1d_update
+    from sparseflow_b200.Kernels.selective_scan import selective_scan_update
+    m = _make(torch.bfloat16, [1] * 3, 24, 16, 1, False)
+    idx = torch.tensor([0, -1, 5], dtype=torch.int32, device="cuda")
+    y = selective_scan_update(m["x"][:, 0], m["dt"][:, 0], m["A"], m["B"][:, 0], m["C"][:, 0],
+                              torch.zeros(0, 24, 16, device="cuda"), m["D"], state_indices=idx)
+    assert y.shape == (3, 24) and (y == 0).all()
+    x = m["x"][:, 0].contiguous()
+    y = causal_conv1d_update(x, x.new_zeros(0, 3, 24), x.new_ones(24, 4), state_indices=idx)
+    assert y.shape == (3, 24) and (y == 0).all()
