@@ -376,14 +376,15 @@ __global__ void __launch_bounds__(kConvThreads, WT <= 4 ? 4 : 2) conv_bwd_kernel
         }
     }
     if (t + G <= r1) {  // the slot's own rows, without conditions, so that the moving windows cost no moves
-      const bool above = t > p.r0;
+      const int above = (int)(t - p.r0);  // rows of the slot before this group
 #pragma unroll
       for (int u = 0; u < G; ++u) {
         u64 o[P];
         row(u);
         add_sums();
         dx_row(o);
-        if (above || u >= W - 1) store_raw<T, V>(po + (long long)u * a.dim, from_pairs<T, V>(o));
+        // The first W - 1 gradients complete rows of the slot before, which its own block stores.
+        if (above + u >= W - 1) store_raw<T, V>(po + (long long)u * a.dim, from_pairs<T, V>(o));
       }
     } else {
 #pragma unroll

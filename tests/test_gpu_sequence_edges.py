@@ -1,0 +1,89 @@
+"""The sequence operators where a call is most easily wrong: many taps, memory beside the outputs, empty and unaligned
+tensors, batches past a grid's limits."""
+import ctypes
+
+import pytest
+import torch
+
+import sequence_reference as ref
+
+pytestmark = pytest.mark.gpu
+
+TYPES = [torch.float32, torch.float16, torch.bfloat16]
+CONV_FWD = 8 + 12  # fp32 roundings of a convolution's output: taps, bias and activation
+
+
+def _offsets(lengths):
+    return torch.tensor([0] + torch.tensor(lengths).cumsum(0).tolist(), dtype=torch.int32, device="cuda")
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# causal_conv1d
+# ----------------------------------------------------------------------------------------------------------------------
+
+def _conv_gradients(dtype, lengths, dim, width, packed):
+    """Every output and gradient of a convolution with a SiLU, initial and final state, against 64 bits."""
+    from sparseflow_b200.Kernels.causal_conv1d import causal_conv1d
+    g = torch.Generator(device="cuda").manual_seed(width)
+
+    def r(*s):
+        return torch.randn(*s, device="cuda", generator=g).to(dtype)
+    n = len(lengths)
+    shape = (sum(lengths), dim) if packed else (n, lengths[0], dim)
+    off = _offsets(lengths) if packed else None
+    x, w, b, init, dy, df = r(*shape), r(dim, width), r(dim), r(n, width - 1, dim), r(*shape), r(n, width - 1, dim)
+    leaves = [t.requires_grad_() for t in (x, w, b, init)]
+    outs = causal_conv1d(x, w, b, "silu", init, off, True)
+    grads = torch.autograd.grad(outs, leaves, (dy, df))
+    args = (*ref.f64(x, w, b), True, ref.f64(init), None if off is None else off.tolist(), *ref.f64(dy, df))
+    val, mag = ref.conv(*args), ref.conv(*args, mag=True)
+    ref.close(outs[0], val[0], mag[0], CONV_FWD, "y")
+    for i, (name, got) in enumerate(zip(("dx", "dweight", "dbias", "dinit"), grads)):
+        ref.close(got, val[2 + i], mag[2 + i], 2 * CONV_FWD + sum(lengths), name)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [5, 6, 7, 8])
+def test_many_taps_over_many_slots(dtype, width):
+    """More slots, and sequences that begin inside the packed rows, than run on the GPU at a time: a gradient's row is
+    stored by its own slot alone."""
+    _conv_gradients(dtype, [9 + 7 * i % 13 for i in range(5000)], 16, width, True)
+    _conv_gradients(dtype, [21] * 2500, 9, width, False)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("width", [5, 6, 7, 8])
+@pytest.mark.parametrize("length", [8, 12, 130, 1029])
+def test_many_taps_long_sequences(dtype, width, length):
+    _conv_gradients(dtype, [length] * 2, 136, width, False)
+    _conv_gradients(dtype, [length, 1, length + 3], 136, width, True)
+
+
+@pytest.mark.parametrize("width", range(2, 9))
+@pytest.mark.parametrize("length", [1, 4, 8, 131])
+def test_conv_writes_its_outputs_alone(width, length):
+    """Outputs in the middle of larger buffers given to the C entries: what lies before and after stays."""
+    from sparseflow_b200 import _lib
+    lib, dim, n, pad = _lib.load(), 24, 3, 8 * 24
+    sizes = {"y": n * length * dim, "final": n * (width - 1) * dim, "dx": n * length * dim, "dw": dim * width, "db": dim,
+             "dinit": n * (width - 1) * dim}
+    buffers = {k: torch.full((pad + s + pad,), -77.0, device="cuda") for k, s in sizes.items()}
+    at = {k: b.data_ptr() + 4 * pad for k, b in buffers.items()}
+    x, dy = (torch.randn(n, length, dim, device="cuda") for _ in range(2))
+    w, b = torch.randn(dim, width, device="cuda"), torch.randn(dim, device="cuda")
+    init, df = (torch.randn(n, width - 1, dim, device="cuda") for _ in range(2))
+    d = ctypes.byref(_lib.CausalConv1dDesc(length, length * dim, dim, n, dim, width, 1, 0, 0, 0))
+    stream = torch.cuda.current_stream().cuda_stream
+    assert lib.sf_causal_conv1d(x.data_ptr(), w.data_ptr(), b.data_ptr(), init.data_ptr(), None, at["y"], at["final"], d,
+                                stream) == _lib.SF_OK
+    nbytes = lib.sf_causal_conv1d_backward_workspace_size(d)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    assert lib.sf_causal_conv1d_backward(x.data_ptr(), w.data_ptr(), b.data_ptr(), init.data_ptr(), None, dy.data_ptr(),
+                                         df.data_ptr(), at["dx"], at["dw"], at["db"], at["dinit"], d, ws.data_ptr(),
+                                         nbytes, stream) == _lib.SF_OK
+    for k, buf in buffers.items():
+        assert (buf[:pad] == -77).all() and (buf[-pad:] == -77).all(), k
+    val = ref.conv(*ref.f64(x, w, b), True, ref.f64(init), None, *ref.f64(dy, df))
+    mag = ref.conv(*ref.f64(x, w, b), True, ref.f64(init), None, *ref.f64(dy, df), mag=True)
+    dx = buffers["dx"][pad:-pad].view(n, length, dim)
+    ref.close(dx, val[2], mag[2], 2 * CONV_FWD + n * length, "dx")
