@@ -745,7 +745,7 @@ struct BwdPlan {
 };
 BwdPlan bwd_plan(const sf_block_norm_desc* d) {
   BwdPlan p;
-  p.shared_gate = d->gate_kind != SF_GATE_NONE && d->rows_per_gate > 1;
+  p.shared_gate = d->gate_kind != SF_GATE_NONE && d->rows_per_gate > 1 && d->rows > 0;
   p.groups = p.shared_gate ? d->rows / d->rows_per_gate : 1;
   p.group_rows = p.shared_gate ? d->rows_per_gate : d->rows;
   // Wide rows that no ring takes: blocks of up to 1024 threads, two an SM.
@@ -885,7 +885,7 @@ extern "C" sf_status sf_block_norm(const void* y, const void* residual, const vo
 }
 
 extern "C" size_t sf_block_norm_backward_workspace_size(const sf_block_norm_desc* d) {
-  if (!valid(d)) return 0;
+  if (!valid(d) || d->dim > kMaxDim) return 0;
   const BwdPlan p = bwd_plan(d);
   return (size_t)(p.blocks * p.groups) * d->dim * (p.shared_gate ? 3 : 2) * sizeof(float);
 }

@@ -87,3 +87,23 @@ def test_conv_writes_its_outputs_alone(width, length):
     mag = ref.conv(*ref.f64(x, w, b), True, ref.f64(init), None, *ref.f64(dy, df), mag=True)
     dx = buffers["dx"][pad:-pad].view(n, length, dim)
     ref.close(dx, val[2], mag[2], 2 * CONV_FWD + n * length, "dx")
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# block_norm
+# ----------------------------------------------------------------------------------------------------------------------
+
+def _norm_leaves(shape, gate_shape):
+    def r(*s):
+        return torch.randn(*s, device="cuda").requires_grad_()
+    dim = shape[-1]
+    return dict(y=r(*shape), residual=r(*shape), gate=r(*gate_shape), post_weight=r(dim), pre_weight=r(dim), scale=r(dim))
+
+
+def test_norm_of_no_sequences_with_a_gate_each():
+    """No sequences of five rows: no gate rows either, and the weights' gradients are 0."""
+    from sparseflow_b200.Kernels.block_norm import block_norm
+    leaves = _norm_leaves((0, 5, 32), (0, 1, 32))
+    r, x = block_norm(**leaves, gate_activation="silu")
+    grads = torch.autograd.grad((r, x), list(leaves.values()), (torch.ones_like(r), torch.ones_like(x)))
+    assert all(g.shape == t.shape and (g == 0).all() for g, t in zip(grads, leaves.values()))

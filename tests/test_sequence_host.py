@@ -1,0 +1,29 @@
+"""The host side of the sequence operators, without a GPU."""
+import ctypes
+import itertools
+import subprocess
+import sys
+from pathlib import Path
+
+import pytest
+import torch
+
+ROOT = Path(__file__).resolve().parent.parent
+
+
+def _in_a_process(code):
+    """Runs code that would end the process where the host arithmetic faults."""
+    r = subprocess.run([sys.executable, "-c", "import ctypes, itertools\nfrom sparseflow_b200 import _lib\nlib = _lib.load()\n" + code],
+                       cwd=ROOT, capture_output=True, text=True)
+    assert r.returncode == 0, (r.returncode, r.stderr[-500:])
+
+
+def test_block_norm_workspace_of_any_shape():
+    """Every count of rows, rows per gate and channels has a workspace size, what the entries refuse has 0; none divides
+    by zero."""
+    _in_a_process("""
+for rows, per, dim, gate in itertools.product((0, 1, 6, 1 << 40), (1, 2, 6), (1, 7, 4096, 16384, 20000, 1 << 30), (0, 2)):
+    d = _lib.BlockNormDesc(rows, dim, dim, dim, per, dim, 0, 0, 0, gate, 1.0, 1e-6)
+    n = lib.sf_block_norm_backward_workspace_size(ctypes.byref(d))
+    assert (n > 0) == (rows % per == 0 and dim <= 16384), (rows, per, dim, gate, n)
+""")
