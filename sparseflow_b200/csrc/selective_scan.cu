@@ -160,6 +160,8 @@ bool valid(const sf_selective_scan_desc* d) {
   return d && d->length >= 0 && d->n_seq >= 0 && d->dim >= 0 && d->state >= 1 && d->groups >= 1 &&
          d->dim % d->groups == 0 && dtype_size(d->dtype) != 0;
 }
+// Whether buffers can be sized: blocks have channels up to kMaxState states.
+bool sized(const sf_selective_scan_desc* d) { return valid(d) && d->state <= kMaxState; }
 int lanes(int state) {
   int l = 1;
   while (l * kS < state) l *= 2;
@@ -299,12 +301,12 @@ using namespace sf;
   }
 
 extern "C" size_t sf_selective_scan_checkpoint_bytes(const sf_selective_scan_desc* d) {
-  if (!valid(d)) return 0;
+  if (!sized(d)) return 0;
   return (size_t)seq::total_slots(d->length, d->n_seq, d->packed, kRows) * d->dim * d->state * sizeof(float);
 }
 
 extern "C" size_t sf_selective_scan_workspace_size(const sf_selective_scan_desc* d) {
-  if (!valid(d) || d->n_seq == 0) return 0;
+  if (!sized(d) || d->n_seq == 0) return 0;
   return (size_t)carry_floats(d, segment_rows(d, kFwdCosts)) * sizeof(float);
 }
 
@@ -341,7 +343,7 @@ extern "C" sf_status sf_selective_scan(const void* x, const void* dt, const floa
 }
 
 extern "C" size_t sf_selective_scan_backward_workspace_size(const sf_selective_scan_desc* d) {
-  if (!valid(d)) return 0;
+  if (!sized(d)) return 0;
   return (size_t)bwd_layout(d, segment_rows(d, kBwdCosts)).total * sizeof(float);
 }
 

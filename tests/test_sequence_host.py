@@ -27,3 +27,16 @@ for rows, per, dim, gate in itertools.product((0, 1, 6, 1 << 40), (1, 2, 6), (1,
     n = lib.sf_block_norm_backward_workspace_size(ctypes.byref(d))
     assert (n > 0) == (rows % per == 0 and dim <= 16384), (rows, per, dim, gate, n)
 """)
+
+
+def test_selective_scan_workspace_of_any_shape():
+    """Sizes of every shape that the entries take, and 0 for states that they refuse."""
+    _in_a_process("""
+for length, n, dim, state, groups, packed in itertools.product((0, 1, 17, 1 << 33), (0, 1, 3), (0, 8, 1 << 20),
+                                                               (1, 16, 128, 129, 1025, 5000, 2 ** 31 - 1), (1, 8), (0, 1)):
+    d = ctypes.byref(_lib.SelectiveScanDesc(length, *[0] * 10, n, dim, state, groups, 1, 0, packed))
+    sizes = [lib.sf_selective_scan_checkpoint_bytes(d), lib.sf_selective_scan_workspace_size(d),
+             lib.sf_selective_scan_backward_workspace_size(d)]
+    assert state <= 128 or not any(sizes), sizes
+    assert state > 128 or n == 0 or dim == 0 or (sizes[0] > 0 and sizes[2] > 0), sizes
+""")
