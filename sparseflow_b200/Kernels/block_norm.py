@@ -70,6 +70,8 @@ class _BlockNorm(torch.autograd.Function):
         dr = dense(dr)
         dx = dense(dx)
         dy, dres, dgate, dpost, dpre, dscale = (like(t) for t in (y, residual, gate, post_weight, pre_weight, scale))
+        if dgate is not None and not y.numel():  # gates of sequences without rows, which no kernel meets
+            dgate.zero_()
         nbytes = _lib.load().sf_block_norm_backward_workspace_size(ctx.desc)
         ws = _empty(max(nbytes, 1), torch.uint8, y.device)
         call_on(y.get_device(), "sf_block_norm_backward", ptr(y), ptr(residual), ptr(gate), ptr(post_weight), ptr(pre_weight),

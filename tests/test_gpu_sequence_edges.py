@@ -107,3 +107,14 @@ def test_norm_of_no_sequences_with_a_gate_each():
     r, x = block_norm(**leaves, gate_activation="silu")
     grads = torch.autograd.grad((r, x), list(leaves.values()), (torch.ones_like(r), torch.ones_like(x)))
     assert all(g.shape == t.shape and (g == 0).all() for g, t in zip(grads, leaves.values()))
+
+
+def test_norm_gates_of_empty_sequences():
+    """Sequences without rows: their gates' gradient is 0, whatever the memory held before."""
+    from sparseflow_b200.Kernels.block_norm import block_norm
+    leaves = _norm_leaves((3, 0, 64), (3, 1, 64))
+    r, x = block_norm(**leaves, gate_activation="sigmoid")
+    used = [torch.full((3, 1, 64), float("nan"), device="cuda") for _ in range(8)]
+    del used  # the allocator gives such a block next
+    grads = torch.autograd.grad((r, x), list(leaves.values()), (torch.ones_like(r), torch.ones_like(x)))
+    assert all(g.shape == t.shape and (g == 0).all() for g, t in zip(grads, leaves.values()))
