@@ -54,6 +54,9 @@ def rows_of(t: torch.Tensor, inner: int = 1):
     width = 1
     for k in range(1, inner + 1):
         if stride[-k] != width and shape[-k] != 1:
+            if not t.numel():  # counts as contiguous whatever its strides are
+                t = t.new_empty(shape)
+                return t, t.stride(0), t.stride(-inner - 1)
             return rows_of(t.contiguous(), inner)
         width *= shape[-k]
     row = stride[-inner - 1] if shape[-inner - 1] > 1 else width

@@ -118,3 +118,24 @@ def test_norm_gates_of_empty_sequences():
     del used  # the allocator gives such a block next
     grads = torch.autograd.grad((r, x), list(leaves.values()), (torch.ones_like(r), torch.ones_like(x)))
     assert all(g.shape == t.shape and (g == 0).all() for g, t in zip(grads, leaves.values()))
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# All of them
+# ----------------------------------------------------------------------------------------------------------------------
+
+def test_empty_views_of_other_orders():
+    """An empty chunk of channels-first activations is an empty call, with gradients."""
+    from sparseflow_b200.Kernels.causal_conv1d import causal_conv1d
+    from sparseflow_b200.Kernels.selective_scan import selective_scan
+    x = torch.randn(2, 8, 5, device="cuda", requires_grad=True)
+    bc = torch.randn(2, 4, 5, device="cuda", requires_grad=True)
+    part, part_bc = x.transpose(1, 2)[:, :0], bc.transpose(1, 2)[:, :0]
+    w = torch.randn(8, 4, device="cuda", requires_grad=True)
+    A = -torch.rand(8, 4, device="cuda")
+    y, f = causal_conv1d(part, w, return_final_state=True)
+    assert y.shape == (2, 0, 8) and (f == 0).all()
+    assert (torch.autograd.grad((y, f), (x, w), (y, f), allow_unused=True)[1] == 0).all()
+    y, f = selective_scan(part, part, A, part_bc, part_bc, z=part, return_final_state=True)
+    assert y.shape == (2, 0, 8) and (f == 0).all()
+    assert all((g == 0).all() for g in torch.autograd.grad((y, f), (x, bc), (y, f)))

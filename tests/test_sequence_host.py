@@ -40,3 +40,14 @@ for length, n, dim, state, groups, packed in itertools.product((0, 1, 17, 1 << 3
     assert state <= 128 or not any(sizes), sizes
     assert state > 128 or n == 0 or dim == 0 or (sizes[0] > 0 and sizes[2] > 0), sizes
 """)
+
+
+@pytest.mark.parametrize("inner", [1, 2])
+@pytest.mark.parametrize("empty", [lambda t: t.transpose(1, 3)[:, :0], lambda t: t.transpose(1, 3)[:0],
+                                   lambda t: t[:, :0].permute(0, 3, 2, 1), lambda t: t.permute(3, 2, 1, 0)[..., :0]])
+def test_rows_of_empty_views(empty, inner):
+    """Views without elements in any order of dimensions: strides of a contiguous tensor, and no endless recursion."""
+    from sparseflow_b200.Kernels._sequence import rows_of
+    t = empty(torch.zeros(2, 8, 5, 7))
+    got, batch, row = rows_of(t, inner)
+    assert got.shape == t.shape and row >= 0 and batch >= 0
