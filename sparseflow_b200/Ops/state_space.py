@@ -89,7 +89,14 @@ class StateSpaceMixer(nn.Module):
         return out if state is None else (out, (conv_state, scan_state))
 
     def step(self, u: torch.Tensor, state, state_indices: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """One token for each row of u [rows, dim]; the states (pools, where indices are given) are updated in place."""
+        """One token for each row of u [rows, dim]; the states (pools, where indices are given) are updated in place.
+        A spiking mixer takes the same rows in the same order at every step, as its membranes go by row."""
+        if self.lif is not None:
+            if state_indices is not None:
+                raise ValueError("state_indices need spiking=False: the LIF neuron's membranes go by row, not by slot")
+            if self.lif.v is not None and self.lif.v.shape[0] != u.shape[0]:
+                raise ValueError(f"{u.shape[0]} rows, but membranes of {self.lif.v.shape[0]}: reset_net() before "
+                                 "another batch")
         x, z = self.in_proj(u).split(self.inner, -1)
         x = causal_conv1d_update(x, state[0], self.conv_weight, self.conv_bias, "silu", state_indices)
         dt, B, C = self._selection(x)

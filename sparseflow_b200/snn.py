@@ -206,5 +206,6 @@ class SpikingStateSpaceLM(nn.Module):
         return self._run(tokens, mix), states
 
     def step(self, tokens: torch.Tensor, states, state_indices: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """Logits [rows, vocab] of one more token [rows] for each sequence."""
+        """Logits [rows, vocab] of one more token [rows] for each sequence; with ``state_indices`` (not if spiking) row i
+        uses the states' slot state_indices[i]."""
         return self._run(tokens, lambda i, x: self.mixers[i].step(x, states[i], state_indices))

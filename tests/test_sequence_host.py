@@ -51,3 +51,17 @@ def test_rows_of_empty_views(empty, inner):
     t = empty(torch.zeros(2, 8, 5, 7))
     got, batch, row = rows_of(t, inner)
     assert got.shape == t.shape and row >= 0 and batch >= 0
+
+
+def test_spiking_steps_refuse_slots_and_other_rows():
+    """The membranes of a spiking mixer go by row: a pool's slots, or another number of rows, would mix requests."""
+    from sparseflow_b200.Ops.state_space import StateSpaceMixer
+    m = StateSpaceMixer(8, spiking=True).eval()
+    state = m.new_state(4)
+    before = [s.clone() for s in state]
+    with pytest.raises(ValueError, match="spiking"):
+        m.step(torch.zeros(2, 8), state, torch.tensor([3, 0], dtype=torch.int32))
+    m.lif.v = torch.zeros(4, m.inner)
+    with pytest.raises(ValueError, match="reset_net"):
+        m.step(torch.zeros(2, 8), state)
+    assert all(torch.equal(a, b) for a, b in zip(state, before))
