@@ -7,12 +7,15 @@ from __future__ import annotations
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _lib
 
 
 def require_cuda(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
-    """All given tensors on one CUDA device."""
+    """All given tensors on one CUDA device, and none with a tangent: the kernels would drop it."""
+    if forward_ad._current_level >= 0:
+        _refuse_tangents(first, *others)
     if not first.is_cuda:
         raise RuntimeError("the sequence operators need CUDA tensors (there is no CPU path)")
     index = first.get_device()
@@ -21,6 +24,11 @@ def require_cuda(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
             if not t.is_cuda:
                 raise RuntimeError("the sequence operators need CUDA tensors (there is no CPU path)")
             raise ValueError(f"a tensor is on {t.device}, another on {first.device}")
+
+
+def _refuse_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("the sequence operators have no forward-mode derivative")
 
 
 def check_shape(name: str, t: torch.Tensor, shape) -> None:

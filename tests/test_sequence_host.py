@@ -65,3 +65,31 @@ def test_spiking_steps_refuse_slots_and_other_rows():
     with pytest.raises(ValueError, match="reset_net"):
         m.step(torch.zeros(2, 8), state)
     assert all(torch.equal(a, b) for a, b in zip(state, before))
+
+
+def _calls():
+    """A call of each operator on CPU tensors, by the names of its tensors."""
+    from sparseflow_b200.Kernels.block_norm import block_norm
+    from sparseflow_b200.Kernels.causal_conv1d import causal_conv1d, causal_conv1d_update
+    from sparseflow_b200.Kernels.selective_scan import selective_scan, selective_scan_update
+    x, w, A, b = torch.ones(1, 2, 4), torch.ones(4, 3), -torch.ones(4, 2), torch.ones(1, 2, 2)
+    return [(causal_conv1d, dict(x=x, weight=w, bias=w[:, 0], initial_state=torch.ones(1, 2, 4))),
+            (causal_conv1d_update, dict(x=x[0], state=torch.ones(2, 2, 4), weight=w, bias=w[:, 0])),
+            (selective_scan, dict(x=x, dt=x, A=A, B=b, C=b, D=w[:, 0], z=x, dt_bias=w[:, 0],
+                                  initial_state=torch.ones(1, 4, 2))),
+            (selective_scan_update, dict(x=x[0], dt=x[0], A=A, B=b[0], C=b[0], state=torch.ones(2, 4, 2), D=w[:, 0],
+                                         z=x[0], dt_bias=w[:, 0])),
+            (block_norm, dict(y=x, residual=x, post_weight=w[:, 0], pre_weight=w[:, 0], gate=x, scale=w[:, 0]))]
+
+
+@pytest.mark.parametrize("which", range(5))
+def test_tangents_are_refused(which):
+    """No operator has a forward-mode derivative: a dual tensor in any place raises, and plain ones do not."""
+    fn, tensors = _calls()[which]
+    with torch.autograd.forward_ad.dual_level():
+        for name, t in tensors.items():
+            dual = torch.autograd.forward_ad.make_dual(t, torch.ones_like(t))
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                fn(**{**tensors, name: dual})
+        with pytest.raises(RuntimeError, match="CUDA"):
+            fn(**tensors)
