@@ -86,6 +86,11 @@ def needs_grad(*tensors: Optional[torch.Tensor]) -> bool:
     return False
 
 
+def written(t: torch.Tensor) -> None:
+    """What a kernel has written in place counts as changed, so that a backward pass that had saved it raises."""
+    torch._C._increment_version((t,))
+
+
 def layout(t: Optional[torch.Tensor]):
     """What the checks of a call depend on, as a key of calls that have passed them."""
     return None if t is None else (t.shape, t.stride(), t.dtype)

@@ -11,7 +11,7 @@ import torch
 
 from .. import _lib
 from ._sequence import (call_on, check_dtype, check_offsets, check_shape, check_state_indices, dense, layout, needs_grad, ptr,
-                        require_cuda, rows_of)
+                        require_cuda, rows_of, written)
 
 _ACTIVATIONS = {None: False, "silu": True}
 
@@ -109,6 +109,7 @@ def causal_conv1d_update(x: torch.Tensor, state: torch.Tensor, weight: torch.Ten
     y = x.new_empty(x.shape)
     call_on(x.get_device(), "sf_causal_conv1d_update", x.data_ptr(), state.data_ptr(), weight.data_ptr(), ptr(bias),
             ptr(state_indices), y.data_ptr(), state.shape[0], desc)
+    written(state)
     return y
 
 

@@ -12,7 +12,7 @@ import torch
 
 from .. import _lib
 from ._sequence import (call_on, check_dtype, check_offsets, check_shape, check_state_indices, dense, layout, needs_grad, ptr,
-                        require_cuda, rows_of)
+                        require_cuda, rows_of, written)
 
 _MAX_STATE = 128
 
@@ -169,6 +169,7 @@ def selective_scan_update(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B:
     call_on(x.get_device(), "sf_selective_scan_update", x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(),
             C.data_ptr(), ptr(D), ptr(z), ptr(dt_bias), state.data_ptr(), ptr(state_indices), y.data_ptr(),
             state.shape[0], desc)
+    written(state)
     return y
 
 

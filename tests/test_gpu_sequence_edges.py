@@ -139,3 +139,22 @@ def test_empty_views_of_other_orders():
     y, f = selective_scan(part, part, A, part_bc, part_bc, z=part, return_final_state=True)
     assert y.shape == (2, 0, 8) and (f == 0).all()
     assert all((g == 0).all() for g in torch.autograd.grad((y, f), (x, bc), (y, f)))
+
+
+def test_pools_count_as_written():
+    """A state that a backward pass has saved and a token has moved since: autograd's error, not a wrong gradient."""
+    from sparseflow_b200.Kernels.causal_conv1d import causal_conv1d, causal_conv1d_update
+    from sparseflow_b200.Kernels.selective_scan import selective_scan_update
+    x, w = torch.randn(2, 5, 8, device="cuda"), torch.randn(8, 4, device="cuda", requires_grad=True)
+    state = torch.randn(2, 3, 8, device="cuda")
+    y = causal_conv1d(x, w, initial_state=state)
+    with torch.no_grad():
+        causal_conv1d_update(x[:, 0], state, w)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    pool, A, b = torch.randn(2, 8, 4, device="cuda"), -torch.rand(8, 4, device="cuda"), torch.randn(2, 4, device="cuda")
+    before = pool._version
+    selective_scan_update(x[:, 0], x[:, 0], A, b, b, pool)
+    assert pool._version > before
+    with torch.inference_mode():
+        selective_scan_update(x[:, 0], x[:, 0], A, b, b, pool.clone())
