@@ -86,9 +86,25 @@ def needs_grad(*tensors: Optional[torch.Tensor]) -> bool:
     return False
 
 
-def written(t: torch.Tensor) -> None:
-    """What a kernel has written in place counts as changed, so that a backward pass that had saved it raises."""
-    torch._C._increment_version((t,))
+class _NoGradient(torch.autograd.Function):
+    """The result of a function without a gradient as a part of the graph, so that a backward pass that comes to it
+    raises instead of passing over it."""
+
+    @staticmethod
+    def forward(ctx, fn, *args):
+        ctx.name = fn.__name__
+        return fn(*args)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise RuntimeError(f"{ctx.name} has no gradient: run sequences through the prompt's function to train")
+
+
+without_gradient = _NoGradient.apply
+
+
+# Tensors that a kernel has written in place count as changed, so that a backward pass that had saved one raises.
+written = torch._C._increment_version
 
 
 def layout(t: Optional[torch.Tensor]):

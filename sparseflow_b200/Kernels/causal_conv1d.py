@@ -11,7 +11,7 @@ import torch
 
 from .. import _lib
 from ._sequence import (call_on, check_dtype, check_offsets, check_shape, check_state_indices, dense, layout, needs_grad, ptr,
-                        require_cuda, rows_of, written)
+                        require_cuda, rows_of, without_gradient, written)
 
 _ACTIVATIONS = {None: False, "silu": True}
 
@@ -99,17 +99,22 @@ def causal_conv1d_update(x: torch.Tensor, state: torch.Tensor, weight: torch.Ten
     """One more token: x [rows, dim] -> y [rows, dim]; ``state`` [slots, width - 1, dim] is shifted in place.
 
     Row i uses slot ``state_indices[i]`` (int32 on the device, distinct), or slot i without indices. A row whose
-    index is no slot (-1, say) is padding: its y is 0 and no state changes. Not differentiable.
+    index is no slot (-1, say) is padding: its y is 0 and no state changes. Not differentiable: where an input asks
+    for a gradient, a backward pass through y raises.
     """
     require_cuda(x, state, weight, bias, state_indices)
-    key = (layout(x), layout(state), layout(weight), layout(bias), layout(state_indices), activation)
+    if torch.is_grad_enabled() and (x.requires_grad or state.requires_grad or weight.requires_grad
+                                    or (bias is not None and bias.requires_grad)):
+        return without_gradient(causal_conv1d_update, x, state, weight, bias, activation, state_indices)
+    key = (x.shape, x.stride(), x.dtype, state.shape, state.stride(), state.dtype, weight.shape, weight.stride(),
+           weight.dtype, layout(bias), layout(state_indices), activation)
     desc = _update_plans.get(key)
     if desc is None:
         x, weight, bias, desc = _update_plan(x, state, weight, bias, activation, state_indices, key)
     y = x.new_empty(x.shape)
     call_on(x.get_device(), "sf_causal_conv1d_update", x.data_ptr(), state.data_ptr(), weight.data_ptr(), ptr(bias),
             ptr(state_indices), y.data_ptr(), state.shape[0], desc)
-    written(state)
+    written((state,))
     return y
 
 

@@ -12,7 +12,7 @@ import torch
 
 from .. import _lib
 from ._sequence import (call_on, check_dtype, check_offsets, check_shape, check_state_indices, dense, layout, needs_grad, ptr,
-                        require_cuda, rows_of, written)
+                        require_cuda, rows_of, without_gradient, written)
 
 _MAX_STATE = 128
 
@@ -155,12 +155,16 @@ def selective_scan_update(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B:
 
     ``state`` [slots, dim, state] fp32 is updated in place. Row i uses slot ``state_indices[i]`` (int32 on the
     device, distinct), or slot i without indices; a row whose index is no slot is padding: its y is 0 and no state
-    changes. Not differentiable.
+    changes. Not differentiable: where an input asks for a gradient, a backward pass through y raises.
     """
     require_cuda(x, dt, A, B, C, state, D, z, dt_bias, state_indices)
+    if torch.is_grad_enabled() and (x.requires_grad or dt.requires_grad or A.requires_grad or B.requires_grad
+                                    or C.requires_grad or state.requires_grad or needs_grad(D, z, dt_bias)):
+        return without_gradient(selective_scan_update, x, dt, A, B, C, state, D, z, dt_bias, dt_softplus,
+                                state_indices)
     key = (x.shape, x.stride(), x.dtype, dt.shape, dt.stride(), dt.dtype, B.shape, B.stride(), B.dtype, C.shape,
-           C.stride(), C.dtype, layout(A), layout(state), layout(D), layout(z), layout(dt_bias), layout(state_indices),
-           dt_softplus)
+           C.stride(), C.dtype, A.shape, A.stride(), A.dtype, state.shape, state.stride(), state.dtype, layout(D),
+           layout(z), layout(dt_bias), layout(state_indices), dt_softplus)
     desc = _update_plans.get(key)
     if desc is None:
         x, dt, A, B, C, D, z, dt_bias, desc = _update_plan(x, dt, A, B, C, state, D, z, dt_bias, dt_softplus,
@@ -169,7 +173,7 @@ def selective_scan_update(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B:
     call_on(x.get_device(), "sf_selective_scan_update", x.data_ptr(), dt.data_ptr(), A.data_ptr(), B.data_ptr(),
             C.data_ptr(), ptr(D), ptr(z), ptr(dt_bias), state.data_ptr(), ptr(state_indices), y.data_ptr(),
             state.shape[0], desc)
-    written(state)
+    written((state,))
     return y
 
 

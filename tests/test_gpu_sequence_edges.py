@@ -158,3 +158,28 @@ def test_pools_count_as_written():
     assert pool._version > before
     with torch.inference_mode():
         selective_scan_update(x[:, 0], x[:, 0], A, b, b, pool.clone())
+
+
+def test_backward_through_tokens_raises():
+    """Tokens have no gradient: their results say so where a backward pass comes to them, and are the same."""
+    from sparseflow_b200.Kernels.causal_conv1d import causal_conv1d_update
+    from sparseflow_b200.Kernels.selective_scan import selective_scan_update
+    from sparseflow_b200.Ops.state_space import StateSpaceMixer
+    x, w, state = torch.randn(2, 8, device="cuda"), torch.randn(8, 4, device="cuda"), torch.randn(2, 3, 8, device="cuda")
+    want, moved = causal_conv1d_update(x, before := state.clone(), w), before
+    y = causal_conv1d_update(x, state, w.requires_grad_())
+    assert torch.equal(y, want) and torch.equal(state, moved)
+    with pytest.raises(RuntimeError, match="causal_conv1d_update has no gradient"):
+        y.sum().backward()
+    A, b = -torch.rand(8, 4, device="cuda"), torch.randn(2, 4, device="cuda")
+    pool, same = torch.zeros(2, 8, 4, device="cuda"), torch.zeros(2, 8, 4, device="cuda")
+    want = selective_scan_update(x, x, A, b, b, same)
+    y = selective_scan_update(x.requires_grad_(), x, A, b, b, pool)
+    assert torch.equal(y, want) and torch.equal(pool, same)
+    with pytest.raises(RuntimeError, match="selective_scan_update has no gradient"):
+        (y * 2).sum().backward()
+    with torch.no_grad():
+        assert not selective_scan_update(x, x, A, b, b, pool).requires_grad
+    m = StateSpaceMixer(16).cuda()
+    with pytest.raises(RuntimeError, match="has no gradient"):
+        m.step(torch.randn(2, 16, device="cuda"), m.new_state(2)).sum().backward()
