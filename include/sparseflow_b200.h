@@ -321,7 +321,9 @@ typedef struct sf_selective_scan_desc {
  * NULL) fp32; z may be NULL (no gate); states [n_seq, dim, state] fp32,
  * initial_state NULL means 0, final_state may be NULL. checkpoints (NULL
  * unless the backward pass will run; sf_selective_scan_checkpoint_bytes, 16-byte
- * aligned) receives the states that the backward pass starts from. */
+ * aligned like the workspace) receives the states that the backward pass starts
+ * from. A and the states may begin anywhere; four states are moved as one word
+ * where their number is a multiple of 4 and all begin at 16 bytes. */
 size_t sf_selective_scan_checkpoint_bytes(const sf_selective_scan_desc* d);
 size_t sf_selective_scan_workspace_size(const sf_selective_scan_desc* d);
 sf_status sf_selective_scan(const void* x, const void* dt, const float* A, const void* B, const void* C,

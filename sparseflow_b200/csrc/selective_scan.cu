@@ -97,12 +97,12 @@ __global__ void __launch_bounds__(kThreads, 8) scan_update_kernel(ScanArgs a, fl
     x[l] = DT<T>::to_f(static_cast<const T*>(a.x)[row * a.x_row + d]);
     z[l] = a.z ? DT<T>::to_f(static_cast<const T*>(a.z)[row * a.z_row + d]) : 0.f;
   }
-  load4(A, a.A + (long long)d * a.state, n, a.state);
+  load4(A, a.A + (long long)d * a.state, n, a);
   const float bias = a.dt_bias ? a.dt_bias[d] : 0.f, D = a.D ? a.D[d] : 0.f;
   // The states last: their addresses wait for the slots.
 #pragma unroll
   for (int r = 0; r < 4; ++r)
-    load4(h[r], pool + ((long long)max(slot[r], 0) * a.dim + d) * a.state, n, a.state);
+    load4(h[r], pool + ((long long)max(slot[r], 0) * a.dim + d) * a.state, n, a);
 #pragma unroll
   for (int i = 0; i < kS; ++i) A[i] *= kLog2e;
   float u[RPL], y[4];
@@ -132,7 +132,7 @@ __global__ void __launch_bounds__(kThreads, 8) scan_update_kernel(ScanArgs a, fl
       h[r][i] = fmaf(ex2(step * A[i]), h[r][i], w * b);
       y[r] = fmaf(Cv[r][i], h[r][i], y[r]);
     }
-    if (slot[r] >= 0) store4(pool + ((long long)slot[r] * a.dim + d) * a.state, h[r], n, a.state);
+    if (slot[r] >= 0) store4(pool + ((long long)slot[r] * a.dim + d) * a.state, h[r], n, a);
   }
   float o[RPL];
   scatter4<LPC>(o, y, q);
@@ -256,6 +256,14 @@ BwdLayout bwd_layout(const sf_selective_scan_desc* d, long long seg) {
   return l;
 }
 
+// Whether rows of states can be read and written as words of four, in every tensor that has them.
+bool states_fit(const sf_selective_scan_desc* d, std::initializer_list<const void*> ptrs) {
+  if (d->state % kS) return false;
+  for (const void* p : ptrs)
+    if (!aligned16(p)) return false;
+  return true;
+}
+
 // Whether four channels can be read and written as one word: every row of every group begins at a multiple.
 bool vectors_fit(const sf_selective_scan_desc* d, std::initializer_list<const void*> ptrs) {
   if ((d->dim / d->groups) % 4) return false;
@@ -328,10 +336,8 @@ extern "C" sf_status sf_selective_scan(const void* x, const void* dt, const floa
   a.seg_rows = segment_rows(d, kFwdCosts);
   const long long carry = carry_floats(d, a.seg_rows), slots = slots_of(d, a.seg_rows);
   if (carry && (!workspace || workspace_bytes < (size_t)carry * sizeof(float))) return SF_ERR_WORKSPACE;
-  for (const void* p : {static_cast<const void*>(A), static_cast<const void*>(initial_state),
-                        static_cast<const void*>(final_state), static_cast<const void*>(checkpoints),
-                        static_cast<const void*>(carry ? workspace : nullptr)})
-    if (!aligned16(p)) return SF_ERR_ALIGNMENT;
+  if (!aligned16(checkpoints) || (carry && !aligned16(workspace))) return SF_ERR_ALIGNMENT;
+  a.wide = states_fit(d, {A, initial_state, final_state});
   if (slots > 65535) return SF_ERR_UNSUPPORTED;
   a.seg_state = static_cast<float*>(workspace);
   a.seg_dt = a.seg_state + slots * d->dim * d->state;
@@ -366,10 +372,7 @@ extern "C" sf_status sf_selective_scan_backward(const void* x, const void* dt, c
   const long long seg = segment_rows(d, kBwdCosts), slots = slots_of(d, seg);
   const BwdLayout l = bwd_layout(d, seg);
   if (some && (!workspace || workspace_bytes < (size_t)l.total * sizeof(float))) return SF_ERR_WORKSPACE;
-  if (some && !aligned16(workspace)) return SF_ERR_ALIGNMENT;
-  for (const void* p : {static_cast<const void*>(A), checkpoints, static_cast<const void*>(d_final_state),
-                        static_cast<const void*>(d_initial_state)})
-    if (!aligned16(p)) return SF_ERR_ALIGNMENT;
+  if (some && (!aligned16(workspace) || !aligned16(checkpoints))) return SF_ERR_ALIGNMENT;
   if (slots > 65535) return SF_ERR_UNSUPPORTED;
   float* ws = static_cast<float*>(workspace);
   ScanArgs a = base_args(x, dt, A, B, C, D, z, dt_bias, seq_offsets, d);
@@ -380,6 +383,7 @@ extern "C" sf_status sf_selective_scan_backward(const void* x, const void* dt, c
   a.ddt = ddt;
   a.dz = z ? dz : nullptr;
   a.dinit = d_initial_state;
+  a.wide = states_fit(d, {A, d_final_state, d_initial_state});
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (some) {
     a.part_bc = ws + l.bc;
@@ -422,7 +426,7 @@ extern "C" sf_status sf_selective_scan_update(const void* x, const void* dt, con
                : SF_ERR_CUDA;
   ScanArgs a = base_args(x, dt, A, B, C, D, z, dt_bias, nullptr, d);
   a.y = y;
-  if (!aligned16(A) || !aligned16(state_pool)) return SF_ERR_ALIGNMENT;
+  a.wide = states_fit(d, {A, state_pool});
   if (d->n_seq > 65535) return SF_ERR_UNSUPPORTED;
   const bool vec = d->state % 4 == 0 && d->b_row_stride % 4 == 0 && d->c_row_stride % 4 == 0 &&
                    reinterpret_cast<uintptr_t>(B) % (4 * dtype_size(d->dtype)) == 0 &&

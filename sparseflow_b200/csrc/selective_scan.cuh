@@ -61,6 +61,7 @@ struct ScanArgs {
   long long seg_rows;                // rows per segment, a multiple of kRows
   long long x_batch, x_row, dt_batch, dt_row, z_batch, z_row, b_batch, b_row, c_batch, c_row;
   int dim, state, groups, softplus;
+  int wide;  // whether rows of states (A, states, their gradients) begin at 16 bytes, four of them a word
 };
 
 constexpr long long kWhole = 1ll << 40;  // seg_rows of segments that take any sequence whole
@@ -92,9 +93,9 @@ __device__ __forceinline__ long long row0(const ScanArgs& a, const Span& s) {
 }
 
 // Four values of a [.., state] row of floats from state n on, 0 past the end.
-__device__ __forceinline__ void load4(float (&o)[kS], const float* p, int n, int state) {
-  if ((state & 3) == 0) {
-    if (n < state) {
+__device__ __forceinline__ void load4(float (&o)[kS], const float* p, int n, const ScanArgs& a) {
+  if (a.wide) {
+    if (n < a.state) {
       const float4 v = *reinterpret_cast<const float4*>(p + n);
       o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w;
     } else {
@@ -103,28 +104,28 @@ __device__ __forceinline__ void load4(float (&o)[kS], const float* p, int n, int
     return;
   }
 #pragma unroll
-  for (int i = 0; i < kS; ++i) o[i] = n + i < state ? p[n + i] : 0.f;
+  for (int i = 0; i < kS; ++i) o[i] = n + i < a.state ? p[n + i] : 0.f;
 }
-__device__ __forceinline__ void store4(float* p, const float (&v)[kS], int n, int state) {
-  if ((state & 3) == 0) {
-    if (n < state) *reinterpret_cast<float4*>(p + n) = make_float4(v[0], v[1], v[2], v[3]);
+__device__ __forceinline__ void store4(float* p, const float (&v)[kS], int n, const ScanArgs& a) {
+  if (a.wide) {
+    if (n < a.state) *reinterpret_cast<float4*>(p + n) = make_float4(v[0], v[1], v[2], v[3]);
     return;
   }
 #pragma unroll
   for (int i = 0; i < kS; ++i)
-    if (n + i < state) p[n + i] = v[i];
+    if (n + i < a.state) p[n + i] = v[i];
 }
-__device__ __forceinline__ void load4(u64 (&o)[2], const float* p, int n, int state) {
+__device__ __forceinline__ void load4(u64 (&o)[2], const float* p, int n, const ScanArgs& a) {
   float v[kS];
-  load4(v, p, n, state);
+  load4(v, p, n, a);
   o[0] = pack2(v[0], v[1]);
   o[1] = pack2(v[2], v[3]);
 }
-__device__ __forceinline__ void store4(float* p, const u64 (&v)[2], int n, int state) {
+__device__ __forceinline__ void store4(float* p, const u64 (&v)[2], int n, const ScanArgs& a) {
   float f[kS];
   unpack2(f[0], f[1], v[0]);
   unpack2(f[2], f[3], v[1]);
-  store4(p, f, n, state);
+  store4(p, f, n, a);
 }
 
 template <int LPC>
@@ -400,7 +401,7 @@ __device__ __forceinline__ void segment_start(u64 (&h)[2], const ScanArgs& a, co
   for (int i = 0; i < j; ++i) {
     const long long slot = p.slot0 + (REV ? p.n_slots - 1 - i : i);
     u64 e[2];
-    load4(e, a.seg_state + (slot * a.dim + d) * a.state, n, a.state);
+    load4(e, a.seg_state + (slot * a.dim + d) * a.state, n, a);
     const float s = a.seg_dt[slot * a.dim + d];
     const u64 s2 = pack2(s, s);
     h[0] = fma2(ex2x2(mul2(s2, A2[0])), h[0], e[0]);
@@ -412,7 +413,7 @@ __device__ __forceinline__ void segment_start(u64 (&h)[2], const ScanArgs& a, co
 template <int LPC, int CPT>
 __device__ __forceinline__ void load_decay(u64 (&A2)[2], const ScanArgs& a, const Place<LPC, CPT>& k, int j) {
   float v[kS] = {};
-  if (k.own(j)) load4(v, a.A + (long long)k.d(j) * a.state, k.n, a.state);
+  if (k.own(j)) load4(v, a.A + (long long)k.d(j) * a.state, k.n, a);
   A2[0] = pack2(v[0] * kLog2e, v[1] * kLog2e);
   A2[1] = pack2(v[2] * kLog2e, v[3] * kLog2e);
 }
@@ -527,7 +528,7 @@ __global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS) scan_carry_kernel(Scan
   for (int j = 0; j < CPT; ++j)
     if (k.own(j)) {
       const long long o = (long long)blockIdx.y * a.dim + k.d(j);
-      store4(a.seg_state + o * a.state, E[j], k.n, a.state);
+      store4(a.seg_state + o * a.state, E[j], k.n, a);
       if (k.q == 0) a.seg_dt[o] = sum[j];
     }
 }
@@ -580,7 +581,7 @@ __global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, BLOCKS) scan_fwd_kerne
   for (int j = 0; j < CPT; ++j) {
     load_decay(A2[j], a, k, j);
     if (!k.own(j)) continue;
-    if (a.init) load4(h[j], a.init + ((long long)p.s * a.dim + k.d(j)) * a.state, k.n, a.state);
+    if (a.init) load4(h[j], a.init + ((long long)p.s * a.dim + k.d(j)) * a.state, k.n, a);
     if (seg > 0) segment_start<false>(h[j], a, p, A2[j], seg, k.d(j), k.n);
     if (a.ck_out)
       ck[j] = a.ck_out + ((seq::seq_slot0(a.rows, p.s, kRows) + p.r0 / kRows) * a.dim + k.d(j)) * a.state;
@@ -590,7 +591,7 @@ __global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, BLOCKS) scan_fwd_kerne
 #pragma unroll
     for (int j = 0; j < CPT; ++j)
       if (ck[j]) {
-        store4(ck[j], h[j], k.n, a.state);
+        store4(ck[j], h[j], k.n, a);
         ck[j] += (long long)a.dim * a.state;
       }
     f.wait();
@@ -678,7 +679,7 @@ __global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, BLOCKS) scan_fwd_kerne
   if (a.final_state && seg == p.n_slots - 1)
 #pragma unroll
     for (int j = 0; j < CPT; ++j)
-      if (k.own(j)) store4(a.final_state + ((long long)p.s * a.dim + k.d(j)) * a.state, h[j], k.n, a.state);
+      if (k.own(j)) store4(a.final_state + ((long long)p.s * a.dim + k.d(j)) * a.state, h[j], k.n, a);
 }
 
 template <typename T, int LPC, int CPT, bool VEC>
@@ -748,7 +749,7 @@ __global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, 3) scan_bwd_kernel(Sca
     for (int j = 0; j < CPT; ++j)
       if (k.own(j)) {
         const long long sd = sd0 + k.d(j);
-        store4(a.part_a + sd * a.state, zero, k.n, a.state);
+        store4(a.part_a + sd * a.state, zero, k.n, a);
         if (k.q == 0) a.part_d[sd] = a.part_d[(long long)gridDim.y * a.dim + sd] = 0.f;
       }
     return;
@@ -791,11 +792,11 @@ __global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, 3) scan_bwd_kernel(Sca
     for (int j = 0; j < CPT; ++j) {
       float4* dst = &s.ck[i & 1][j][threadIdx.x];
       const float* src = ck + (long long)k.chan(j) * a.state;
-      if ((a.state & 3) == 0) {
+      if (a.wide) {
         cp_async(dst, k.own(j) && k.n < a.state ? src + k.n : a.ck, 16, k.own(j) && k.n < a.state);
       } else {
         float v[kS] = {};
-        if (k.own(j)) load4(v, src, k.n, a.state);
+        if (k.own(j)) load4(v, src, k.n, a);
         *dst = make_float4(v[0], v[1], v[2], v[3]);
       }
     }
@@ -812,7 +813,7 @@ __global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, 3) scan_bwd_kernel(Sca
     load_decay(A2[j], a, k, j);
     D[j] = a.D && k.own(j) ? a.D[k.d(j)] : 0.f;
     if (!k.own(j)) continue;
-    if (a.dfinal) load4(gh[j], a.dfinal + ((long long)p.s * a.dim + k.d(j)) * a.state, k.n, a.state);
+    if (a.dfinal) load4(gh[j], a.dfinal + ((long long)p.s * a.dim + k.d(j)) * a.state, k.n, a);
     if (seg < p.n_slots - 1) segment_start<true>(gh[j], a, p, A2[j], p.n_slots - 1 - seg, k.d(j), k.n);
   }
   const int first = sums_first<LPC>(lane);
@@ -988,8 +989,8 @@ __global__ void __launch_bounds__(Cfg<LPC, CPT>::THREADS, 3) scan_bwd_kernel(Sca
     const float d = lanes_sum<(LPC < 4 ? LPC : 4)>(gD[j]), bias = lanes_sum<(LPC < 4 ? LPC : 4)>(gbias[j]);
     if (!k.own(j)) continue;
     const long long sd = sd0 + k.d(j);
-    if (a.dinit && seg == 0) store4(a.dinit + ((long long)p.s * a.dim + k.d(j)) * a.state, gh[j], k.n, a.state);
-    store4(a.part_a + sd * a.state, gA[j], k.n, a.state);
+    if (a.dinit && seg == 0) store4(a.dinit + ((long long)p.s * a.dim + k.d(j)) * a.state, gh[j], k.n, a);
+    store4(a.part_a + sd * a.state, gA[j], k.n, a);
     if (k.q == 0) {
       a.part_d[sd] = d;
       a.part_d[(long long)gridDim.y * a.dim + sd] = bias;

@@ -121,6 +121,83 @@ def test_norm_gates_of_empty_sequences():
 
 
 # ----------------------------------------------------------------------------------------------------------------------
+# selective_scan
+# ----------------------------------------------------------------------------------------------------------------------
+
+def _shifted(t, by=1):
+    """The same values, contiguous, `by` elements into a buffer: not at a multiple of 16 bytes."""
+    buf = torch.empty(t.numel() + 4, dtype=t.dtype, device=t.device)
+    out = buf[by:by + t.numel()].view(t.shape)
+    out.copy_(t)
+    assert out.is_contiguous() and out.data_ptr() % 16
+    return out
+
+
+def _scan_inputs(lead, dim, n, groups=1, dtype=torch.float32, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+
+    def r(*s, dt=dtype):
+        return torch.randn(*s, device="cuda", generator=g).to(dt)
+    f = torch.float32
+    return dict(x=r(*lead, dim), dt=r(*lead, dim), A=-torch.exp(0.5 * r(dim, n, dt=f)), B=r(*lead, groups, n),
+                C=r(*lead, groups, n), D=r(dim, dt=f), z=r(*lead, dim), dt_bias=r(dim, dt=f) - 1)
+
+
+@pytest.mark.parametrize("n", [3, 4, 13, 16, 64])
+@pytest.mark.parametrize("length", [7, 700])
+def test_scan_of_unaligned_states(n, length):
+    """A, initial states and the gradient of the final states that begin between words of 16 bytes: the same bits."""
+    from sparseflow_b200.Kernels.selective_scan import selective_scan
+    m = _scan_inputs((2, length), 22, n)
+    init, df = torch.randn(2, 22, n, device="cuda"), torch.randn(2, 22, n, device="cuda")
+    dy = torch.randn_like(m["x"])
+
+    def run(A, init, df):
+        leaves = [A.detach().requires_grad_(), init.detach().requires_grad_(), m["x"].detach().requires_grad_()]
+        y, f = selective_scan(**{**m, "A": leaves[0], "x": leaves[2]}, initial_state=leaves[1], return_final_state=True)
+        return y, f, *torch.autograd.grad((y, f), leaves, (dy, df))
+    want = run(m["A"], init, df)
+    for k in range(8):
+        got = run(_shifted(m["A"]) if k & 1 else m["A"], _shifted(init, 3) if k & 2 else init,
+                  _shifted(df, 2) if k & 4 else df)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), k
+
+
+@pytest.mark.parametrize("n", [13, 16])
+def test_scan_of_a_layer_of_stacked_states(n):
+    """Layers of one pool and of stacked parameters, and final states that are joined: ordinary views."""
+    from sparseflow_b200.Kernels.selective_scan import selective_scan, selective_scan_update
+    m = _scan_inputs((3, 9), 770, n, groups=2)
+    stack = torch.stack([m["A"], 2 * m["A"], m["A"]])
+    states = torch.randn(4, 3, 770, n, device="cuda")
+    one = {k: v if k in ("A", "D", "dt_bias") else v[:, 0] for k, v in m.items()}
+    for layer in range(3):
+        want_state = states[layer + 1].clone()
+        want = selective_scan_update(**{**one, "A": stack[layer].clone()}, state=want_state)
+        before = states.clone()
+        got = selective_scan_update(**{**one, "A": stack[layer]}, state=states[layer + 1])
+        assert torch.equal(got, want) and torch.equal(states[layer + 1], want_state)
+        rest = [i for i in range(4) if i != layer + 1]
+        assert torch.equal(states[rest], before[rest])
+    x = m["x"].requires_grad_()
+    finals = [selective_scan(**m, initial_state=s, return_final_state=True)[1] for s in states[1:3]]
+    assert torch.autograd.grad(torch.cat([finals[0][:1], finals[1]]).square().sum(), x)[0].isfinite().all()
+
+
+@pytest.mark.parametrize("n", [3, 13, 16])
+def test_tokens_of_unaligned_pools(n):
+    from sparseflow_b200.Kernels.selective_scan import selective_scan_update
+    m = {k: v if k in ("A", "D", "dt_bias") else v[:, 0] for k, v in _scan_inputs((5, 1), 38, n).items()}
+    pool = torch.randn(7, 38, n, device="cuda")
+    idx = torch.tensor([6, 0, -1, 3, 2], dtype=torch.int32, device="cuda")
+    there = _shifted(pool)
+    want = selective_scan_update(**m, state=pool, state_indices=idx)
+    assert torch.equal(selective_scan_update(**m, state=there, state_indices=idx), want) and torch.equal(there, pool)
+    assert torch.equal(selective_scan_update(**{**m, "A": _shifted(m["A"], 3)}, state=there.clone(), state_indices=idx),
+                       selective_scan_update(**m, state=pool, state_indices=idx))
+
+
+# ----------------------------------------------------------------------------------------------------------------------
 # All of them
 # ----------------------------------------------------------------------------------------------------------------------
 
