@@ -308,7 +308,7 @@ typedef struct sf_selective_scan_desc {
   int64_t length; /* rows per sequence; packed: rows in all */
   int64_t x_batch_stride, x_row_stride, dt_batch_stride, dt_row_stride, z_batch_stride, z_row_stride;
   int64_t b_batch_stride, b_row_stride, c_batch_stride, c_row_stride; /* a row of B or C is [groups, state] */
-  int32_t n_seq, dim;
+  int32_t n_seq, dim;  /* up to 65535 sequences; of single tokens up to 262140 rows */
   int32_t state;       /* states per channel, 1 .. 128 */
   int32_t groups;      /* divides dim: channel d reads group d / (dim / groups) of B and C */
   int32_t dt_softplus; /* nonzero: dt = softplus(dt + dt_bias), else dt + dt_bias */

@@ -125,7 +125,7 @@ def selective_scan(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.
     """h_t = exp(dt_t A) h_(t-1) + dt_t x_t B_t, y_t = (C_t . h_t + D x_t) silu(z_t), channel by channel.
 
     x, dt, z: [batch, length, dim], or [total, dim] of packed sequences with ``seq_offsets`` (int32 [n_seq + 1] on
-    the device, from 0 to total; sequences may be empty); B, C: the same leading dimensions and [state] or
+    the device, from 0 to total; sequences may be empty; up to 65535 of them either way); B, C: the same leading dimensions and [state] or
     [groups, state] (channel d reads group d // (dim / groups)), all of x's type. Rows may be slices of wider rows.
     A [dim, state], D, dt_bias [dim] are read in 32 bits. dt is softplus(dt + dt_bias), or dt + dt_bias without
     ``dt_softplus``. States are fp32 [n_seq, dim, state]; the initial one is 0 if None. Returns y, or
@@ -155,7 +155,8 @@ def selective_scan_update(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B:
 
     ``state`` [slots, dim, state] fp32 is updated in place. Row i uses slot ``state_indices[i]`` (int32 on the
     device, distinct), or slot i without indices; a row whose index is no slot is padding: its y is 0 and no state
-    changes. Not differentiable: where an input asks for a gradient, a backward pass through y raises.
+    changes. Up to 262140 rows. Not differentiable: where an input asks for a gradient, a backward pass through y
+    raises.
     """
     require_cuda(x, dt, A, B, C, state, D, z, dt_bias, state_indices)
     if torch.is_grad_enabled() and (x.requires_grad or dt.requires_grad or A.requires_grad or B.requires_grad

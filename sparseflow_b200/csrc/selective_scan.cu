@@ -424,10 +424,10 @@ extern "C" sf_status sf_selective_scan_update(const void* x, const void* dt, con
                    cudaSuccess
                ? SF_OK
                : SF_ERR_CUDA;
+  if (d->n_seq > 4 * 65535) return SF_ERR_UNSUPPORTED;  // a block has four rows
   ScanArgs a = base_args(x, dt, A, B, C, D, z, dt_bias, nullptr, d);
   a.y = y;
   a.wide = states_fit(d, {A, state_pool});
-  if (d->n_seq > 65535) return SF_ERR_UNSUPPORTED;
   const bool vec = d->state % 4 == 0 && d->b_row_stride % 4 == 0 && d->c_row_stride % 4 == 0 &&
                    reinterpret_cast<uintptr_t>(B) % (4 * dtype_size(d->dtype)) == 0 &&
                    reinterpret_cast<uintptr_t>(C) % (4 * dtype_size(d->dtype)) == 0;

@@ -197,6 +197,26 @@ def test_tokens_of_unaligned_pools(n):
                        selective_scan_update(**m, state=pool, state_indices=idx))
 
 
+def test_many_rows_of_tokens():
+    """More rows than a grid has blocks in its second dimension; past the limit a clear refusal."""
+    from sparseflow_b200._lib import SparseFlowError
+    from sparseflow_b200.Kernels.selective_scan import selective_scan, selective_scan_update
+    m = {k: v if k in ("A", "D", "dt_bias") else v[:, 0] for k, v in _scan_inputs((70001, 1), 5, 3).items()}
+    pool = torch.randn(70001, 5, 3, device="cuda")
+    parts = pool.clone()
+    y = selective_scan_update(**m, state=pool)
+    for a, b in ((0, 40000), (40000, 70001)):
+        rows = {k: v if k in ("A", "D", "dt_bias") else v[a:b] for k, v in m.items()}
+        assert torch.equal(selective_scan_update(**rows, state=parts[a:b]), y[a:b])
+    assert torch.equal(pool, parts)
+    m = {k: v if k in ("A", "D", "dt_bias") else v[:1].expand(262141, *v.shape[1:]) for k, v in m.items()}
+    with pytest.raises(SparseFlowError):
+        selective_scan_update(**m, state=torch.zeros(262141, 5, 3, device="cuda"))
+    m = _scan_inputs((65536, 1), 2, 1)
+    with pytest.raises(SparseFlowError):
+        selective_scan(**m)
+
+
 # ----------------------------------------------------------------------------------------------------------------------
 # All of them
 # ----------------------------------------------------------------------------------------------------------------------
