@@ -220,14 +220,15 @@ __global__ void __launch_bounds__(1024) norm_fwd_kernel(NormArgs a) {
   }
 }
 
-// Block b of gate group g: rows g * group_rows + [b * per, (b + 1) * per) of the group. The sums over rows of the
-// weights' gradients (and, where one gate row serves many rows, of the gate's) stay in registers.
+// Block b of gate group g (block g * blocks + b of the grid): rows g * group_rows + [b * per, (b + 1) * per) of the group.
+// The sums over rows of the weights' gradients (and, where one gate row serves many rows, of the gate's) stay in registers.
 template <typename T, typename R, int K, int MAXT>
-__global__ void __launch_bounds__(MAXT) norm_bwd_kernel(NormArgs a, long long group_rows, long long per) {
+__global__ void __launch_bounds__(MAXT) norm_bwd_kernel(NormArgs a, long long group_rows, long long per,
+                                                        unsigned blocks) {
   __shared__ float buf[96];
   const float inv = 1.f / (float)a.dim;
-  const long long first = (long long)blockIdx.y * group_rows;
-  const long long begin = first + blockIdx.x * per, end = min(begin + per, first + group_rows);
+  const long long first = blockIdx.x / blocks * group_rows;
+  const long long begin = first + blockIdx.x % blocks * per, end = min(begin + per, first + group_rows);
   const bool shared_gate = a.part_gate != nullptr;
   float Q[K][kV] = {}, gpre[K][kV] = {}, ggate[K][kV] = {};
   for (long long row = begin; row < end; ++row) {
@@ -317,7 +318,7 @@ __global__ void __launch_bounds__(MAXT) norm_bwd_kernel(NormArgs a, long long gr
       }
     }
   }
-  const long long block = (long long)blockIdx.y * gridDim.x + blockIdx.x;
+  const long long block = blockIdx.x;
   float* pw = a.part_w + block * 2 * a.dim;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
@@ -554,7 +555,8 @@ struct BwdRing {
 };
 // Rows as in norm_bwd_kernel; part_w[block][0]: Q, [1]: dw_pre.
 template <typename T, typename R, int KIND>
-__global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long long group_rows, long long per) {
+__global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long long group_rows, long long per,
+                                                              unsigned blocks) {
   using S = BwdRing<T, R>;
   extern __shared__ __align__(16) float4 ring[];
   bool own;
@@ -563,8 +565,9 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long 
   const float inv = 1.f / (float)a.dim;
   constexpr bool gated = KIND != SF_GATE_NONE, curved = KIND == SF_GATE_SILU || KIND == SF_GATE_SIGMOID;
   const bool shared_gate = a.part_gate != nullptr, pre = a.w_pre && a.dx;
-  const long long first = (long long)blockIdx.y * group_rows;
-  const long long begin = first + blockIdx.x / a.cluster * per, end = min(begin + per, first + group_rows);
+  const unsigned block = blockIdx.x / a.cluster, group = block / blocks;
+  const long long first = group * group_rows;
+  const long long begin = first + block % blocks * per, end = min(begin + per, first + group_rows);
   long long ahead = begin;
   int put = 0, get = 0, half = 0;
   float next1 = 1.f, next2 = 0.f;
@@ -573,7 +576,7 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long 
       float4* s = ring + put * S::WORDS * n;
       copy8<T>(s + S::Y * n, a.y, ahead * a.y_row + c);
       // a gate row for many rows: one for the block's group
-      if (gated) copy8<T>(s + S::GATE * n, a.gate, (shared_gate ? (long long)blockIdx.y : ahead) * a.gate_row + c);
+      if (gated) copy8<T>(s + S::GATE * n, a.gate, (shared_gate ? (long long)group : ahead) * a.gate_row + c);
       if (a.res) copy8<R>(s + S::RES * n, a.res, ahead * a.res_row + c);
       const long long at = ahead * a.dim + c;
       if (pre) copy8<T>(s + S::DX * n, a.dx, at);
@@ -668,22 +671,22 @@ __global__ void __launch_bounds__(512, 1) norm_bwd_ring_kernel(NormArgs a, long 
     load();
   }
   if (!own) return;
-  const long long block = ((long long)blockIdx.y * gridDim.x + blockIdx.x) / a.cluster;
-  put8<float>(a.part_w, block * 2 * a.dim + c, Q);
-  put8<float>(a.part_w, (block * 2 + 1) * a.dim + c, gpre);
-  if (shared_gate) put8<float>(a.part_gate, block * a.dim + c, ggate);
+  put8<float>(a.part_w, 2ll * block * a.dim + c, Q);
+  put8<float>(a.part_w, (2ll * block + 1) * a.dim + c, gpre);
+  if (shared_gate) put8<float>(a.part_gate, (long long)block * a.dim + c, ggate);
 }
 
 // out[g][i] = factor[i] sum over j < blocks of part[g][j][stride] at i, to at most two outputs (a null output is left
-// out, a null factor is 1); where blockIdx.z is 1, out2[i] = the sum over j of the n values after those.
-// A warp has 32 values and each of the block's 8 warps every eighth block: a fixed order.
+// out, a null factor is 1); where blockIdx.y is 1, out2[i] = the sum over j of the n values after those. A block has 32 of
+// a group's n values, and each of its 8 warps every eighth j: a fixed order.
 __global__ void __launch_bounds__(256) norm_reduce_kernel(const float* part, long long blocks, long long stride, int n,
                                                           int dtype, void* out0, const void* factor0, void* out1,
                                                           const void* factor1, int factor_dtype, void* out2) {
   __shared__ float sums[8][32];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = blockIdx.x * 32 + lane;
-  const float* p = part + (long long)blockIdx.y * blocks * stride + i;
-  if (blockIdx.z == 1) {
+  const unsigned tiles = (n + 31) / 32, g = blockIdx.x / tiles;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, i = (int)(blockIdx.x % tiles) * 32 + lane;
+  const float* p = part + g * blocks * stride + i;
+  if (blockIdx.y == 1) {
     p += n;
     out0 = out2;
     factor0 = nullptr;
@@ -699,7 +702,7 @@ __global__ void __launch_bounds__(256) norm_reduce_kernel(const float* part, lon
   if (warp != 0 || i >= n) return;
 #pragma unroll
   for (int w = 1; w < 8; ++w) s += sums[w][lane];
-  const long long o = (long long)blockIdx.y * n + i;
+  const long long o = (long long)g * n + i;
   if (out0) seq::store_param(out0, o, dtype, factor0 ? s * seq::load_param(factor0, i, factor_dtype) : s);
   if (out1) seq::store_param(out1, o, dtype, factor1 ? s * seq::load_param(factor1, i, factor_dtype) : s);
 }
@@ -782,14 +785,14 @@ NormArgs base_args(const void* y, const void* residual, const void* gate, const 
   return a;
 }
 
-// Launches a kernel with a ring on a grid of rows at work (and groups), a cluster for each row of several blocks.
+// Launches a kernel with a ring on a grid of rows at work, a cluster for each row of several blocks.
 template <typename K, typename... Args>
-sf_status launch_ring(K kernel, const NormArgs& a, long long rows, long long groups, size_t words, int sums,
-                      cudaStream_t st, Args... args) {
+sf_status launch_ring(K kernel, const NormArgs& a, long long rows, size_t words, int sums, cudaStream_t st,
+                      Args... args) {
   const int threads = threads_for(a.slice, 1);
   const size_t smem = words * threads * sizeof(float4) + 2 * 16 * kMaxCluster * sums * sizeof(float);
   if (smem > 48 * 1024 && !allow_max_smem(reinterpret_cast<const void*>(kernel))) return SF_ERR_CUDA;
-  const dim3 grid((unsigned)(rows * a.cluster), (unsigned)groups);
+  const dim3 grid((unsigned)(rows * a.cluster));
   if (a.cluster == 1) {
     kernel<<<grid, threads, smem, st>>>(a, args...);
     return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
@@ -819,7 +822,7 @@ sf_status run_fwd(const NormArgs& a, cudaStream_t st) {
                   : a.gate_kind == SF_GATE_SILU   ? norm_fwd_ring_kernel<T, R, SF_GATE_SILU>
                                                   : norm_fwd_ring_kernel<T, R, SF_GATE_SIGMOID>;
     const long long most = rows_at_work(a.dim, 1024);
-    return launch_ring(kernel, a, a.rows < most ? a.rows : most, 1, S::STAGES * S::WORDS, 2, st);
+    return launch_ring(kernel, a, a.rows < most ? a.rows : most, S::STAGES * S::WORDS, 2, st);
   }
   const int K = vectors_per_thread(a.dim), threads = threads_for(a.dim, K);
   const unsigned grid = (unsigned)(a.rows < INT32_MAX ? a.rows : INT32_MAX);
@@ -829,20 +832,21 @@ sf_status run_fwd(const NormArgs& a, cudaStream_t st) {
 }
 template <typename T, typename R>
 sf_status run_bwd(const NormArgs& a, const BwdPlan& p, cudaStream_t st) {
+  const unsigned blocks = (unsigned)p.blocks;
   if (a.vec) {
     using S = BwdRing<T, R>;
     auto kernel = a.gate_kind == SF_GATE_NONE     ? norm_bwd_ring_kernel<T, R, SF_GATE_NONE>
                   : a.gate_kind == SF_GATE_LINEAR ? norm_bwd_ring_kernel<T, R, SF_GATE_LINEAR>
                   : a.gate_kind == SF_GATE_SILU   ? norm_bwd_ring_kernel<T, R, SF_GATE_SILU>
                                                   : norm_bwd_ring_kernel<T, R, SF_GATE_SIGMOID>;
-    return launch_ring(kernel, a, p.blocks, p.groups, S::STAGES * S::WORDS, 3, st, p.group_rows, p.per);
+    return launch_ring(kernel, a, p.blocks * p.groups, S::STAGES * S::WORDS, 3, st, p.group_rows, p.per, blocks);
   }
   // The kernel wants about 90 registers with one vector a thread and 160 with two.
   const int K = a.dim > 512 * kV ? 2 : 1, threads = threads_for(a.dim, K);
-  const dim3 grid((unsigned)p.blocks, (unsigned)p.groups);
-  if (K == 1) norm_bwd_kernel<T, R, 1, 512><<<grid, threads, 0, st>>>(a, p.group_rows, p.per);
-  else if (threads <= 512) norm_bwd_kernel<T, R, 2, 512><<<grid, threads, 0, st>>>(a, p.group_rows, p.per);
-  else norm_bwd_kernel<T, R, 2, 1024><<<grid, threads, 0, st>>>(a, p.group_rows, p.per);
+  const unsigned grid = (unsigned)(p.blocks * p.groups);
+  if (K == 1) norm_bwd_kernel<T, R, 1, 512><<<grid, threads, 0, st>>>(a, p.group_rows, p.per, blocks);
+  else if (threads <= 512) norm_bwd_kernel<T, R, 2, 512><<<grid, threads, 0, st>>>(a, p.group_rows, p.per, blocks);
+  else norm_bwd_kernel<T, R, 2, 1024><<<grid, threads, 0, st>>>(a, p.group_rows, p.per, blocks);
   return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
 }
 
@@ -904,7 +908,8 @@ extern "C" sf_status sf_block_norm_backward(const void* y, const void* residual,
     return SF_ERR_WORKSPACE;
   if (d->rows > 0 && !aligned16(workspace)) return SF_ERR_ALIGNMENT;
   const BwdPlan p = bwd_plan(d);
-  if (p.groups > 65535) return SF_ERR_UNSUPPORTED;
+  const unsigned tiles = (d->dim + 31) / 32;  // of the sums over blocks
+  if (p.blocks * p.groups > INT32_MAX / kMaxCluster || p.groups > INT32_MAX / tiles) return SF_ERR_UNSUPPORTED;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const long long blocks = d->rows > 0 ? p.blocks * p.groups : 0;
   float* part = static_cast<float*>(workspace);
@@ -924,12 +929,11 @@ extern "C" sf_status sf_block_norm_backward(const void* y, const void* residual,
     SF_NORM_DISPATCH(d, (run_bwd<T, R>(a, p, st)));
     if (status != SF_OK) return status;
   }
-  const unsigned grid = (d->dim + 31) / 32;
   if (d_post_weight || d_scale || d_pre_weight)
-    norm_reduce_kernel<<<dim3(grid, 1, 2), 256, 0, st>>>(part, blocks, 2ll * d->dim, d->dim, d->w_dtype, d_post_weight,
+    norm_reduce_kernel<<<dim3(tiles, 2), 256, 0, st>>>(part, blocks, 2ll * d->dim, d->dim, d->w_dtype, d_post_weight,
                                                          scale, d_scale, post_weight, d->w_dtype, d_pre_weight);
   if (p.shared_gate && d_gate && d->rows > 0)
-    norm_reduce_kernel<<<dim3(grid, (unsigned)p.groups), 256, 0, st>>>(a.part_gate, p.blocks, d->dim, d->dim, d->dtype,
+    norm_reduce_kernel<<<tiles * (unsigned)p.groups, 256, 0, st>>>(a.part_gate, p.blocks, d->dim, d->dim, d->dtype,
                                                                        d_gate, nullptr, nullptr, nullptr, d->w_dtype, nullptr);
   return cudaGetLastError() == cudaSuccess ? SF_OK : SF_ERR_CUDA;
 }

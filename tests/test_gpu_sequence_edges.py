@@ -120,6 +120,23 @@ def test_norm_gates_of_empty_sequences():
     assert all(g.shape == t.shape and (g == 0).all() for g, t in zip(grads, leaves.values()))
 
 
+@pytest.mark.parametrize("dim", [16, 9])
+def test_norm_gates_of_many_sequences(dim):
+    """More gates than a grid has blocks in its second dimension, forward and backward."""
+    from sparseflow_b200.Kernels.block_norm import block_norm
+    torch.manual_seed(1)
+    leaves = _norm_leaves((70000, 2, dim), (70000, 1, dim))
+    dr, dx = torch.randn(70000, 2, dim, device="cuda"), torch.randn(70000, 2, dim, device="cuda")
+    r, x = block_norm(**leaves, gate_activation="silu", eps=1e-5)
+    grads = torch.autograd.grad((r, x), list(leaves.values()), (dr, dx))
+    args = (*ref.f64(*(leaves[k] for k in ("y", "residual", "gate"))), "silu",
+            *ref.f64(*(leaves[k] for k in ("post_weight", "pre_weight", "scale"))), 1.0, 1e-5, *ref.f64(dr, dx))
+    val, mag = ref.norm(*args), ref.norm(*args, mag=True)
+    ref.close(x, val["x"], mag["x"], 64, "normed")
+    for name, got, k in zip(leaves, grads, ("dy", "dres", "dgate", "dpost", "dpre", "dscale")):
+        ref.close(got, val[k], mag[k], 4 * 64 + (140000 if k in ("dpost", "dpre", "dscale") else 2), name)
+
+
 # ----------------------------------------------------------------------------------------------------------------------
 # selective_scan
 # ----------------------------------------------------------------------------------------------------------------------
