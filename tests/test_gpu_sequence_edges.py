@@ -234,6 +234,51 @@ def test_many_rows_of_tokens():
         selective_scan(**m)
 
 
+def _scan_against_64_bits(m, softplus, init, dy, df, length):
+    """Outputs and gradients; 64 roundings a row and twice that for gradients (|dt A| <= 8)."""
+    from sparseflow_b200.Kernels.selective_scan import selective_scan
+    names = ("x", "dt", "A", "B", "C", "D", "z", "dt_bias")
+    leaves = {k: m[k].detach().requires_grad_() for k in names if m[k] is not None}
+    init = init.requires_grad_()
+    outs = selective_scan(**{**m, **leaves}, dt_softplus=softplus, initial_state=init, return_final_state=True)
+    grads = torch.autograd.grad(outs, [*leaves.values(), init], (dy, df))
+    args = (*ref.f64(*(m[k] for k in names)), softplus, ref.f64(init), None, *ref.f64(dy, df))
+    val, mag = ref.scan(*args), ref.scan(*args, mag=True)
+    k = 64 * (length + 8)
+    ref.close(outs[0], val["y"], mag["y"], k, "y")
+    ref.close(outs[1], val["final"], mag["final"], k, "final")
+    for name, got in zip([*leaves, "init"], grads):
+        name = "bias" if name == "dt_bias" else name
+        ref.close(got, val["d" + name], mag["d" + name], 2 * k, name)
+
+
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("length", [20, 51, 1100])
+def test_scan_of_states_that_grow(sign, length):
+    """exp(dt A) = exp(7) a row, by A or by dt: a tile's or a segment's product is past fp32, but the states before the
+    first x and the gradients after the last dy are 0, and stay it."""
+    m = _scan_inputs((2, length), 10, 16)
+    m.update(A=torch.full((10, 16), float(sign), device="cuda"), dt=torch.full_like(m["x"], 7.0 * sign), dt_bias=None)
+    m["x"][:, :-3] = 0
+    dy = torch.randn_like(m["x"])
+    dy[:, 3:] = 0
+    _scan_against_64_bits(m, False, torch.zeros(2, 10, 16, device="cuda"), dy, torch.zeros(2, 10, 16, device="cuda"),
+                          length)
+
+
+def test_scan_of_a_small_state_that_grows():
+    """16 rows of exp(7) each: the product of a tile is past fp32, a state of 1e-30 after it is not."""
+    from sparseflow_b200.Kernels.selective_scan import selective_scan
+    m = _scan_inputs((2, 16), 10, 16)
+    m.update(A=torch.ones(10, 16, device="cuda"), dt=torch.full_like(m["x"], 7.0), x=torch.zeros_like(m["x"]), dt_bias=None)
+    init = 1e-30 * torch.randn(2, 10, 16, device="cuda")
+    y, f = selective_scan(**m, dt_softplus=False, initial_state=init, return_final_state=True)
+    args = (*ref.f64(*(m[k] for k in ("x", "dt", "A", "B", "C", "D", "z"))), None, False, ref.f64(init), None)
+    val, mag = ref.scan(*args), ref.scan(*args, mag=True)
+    ref.close(y, val["y"], mag["y"], 64 * 24, "y")
+    ref.close(f, val["final"], mag["final"], 64 * 24, "final")
+
+
 # ----------------------------------------------------------------------------------------------------------------------
 # All of them
 # ----------------------------------------------------------------------------------------------------------------------
