@@ -27,6 +27,8 @@ class StateSpaceMixer(nn.Module):
     ``spiking``: the scan's output passes a LIF neuron over the tokens and the projection back is a ``SparseLinear`` of
     its spikes (the membrane is kept between calls like any ``LIFNode``'s, see ``reset_net``). Without it the
     projection is dense and the layer is differentiable; the LIF neuron and the SparseLinear are inference operators.
+    ``A_log``, ``dt_bias`` and ``D`` stay fp32 when the layer is cast to another type: 16 bits would hold a step of 1e-3,
+    whose bias is near -6.9, to 1.6 %, and the scan reads them in 32 bits.
     """
 
     def __init__(self, dim: int, state: int = 16, width: int = 4, expand: int = 2, dt_rank: Optional[int] = None,
@@ -47,6 +49,14 @@ class StateSpaceMixer(nn.Module):
         self.D = nn.Parameter(torch.ones(inner))
         self.lif = LIFNode(tau=tau, v_threshold=v_threshold) if spiking else None
         self.out_proj = SparseLinear(inner, dim) if spiking else nn.Linear(inner, dim)
+
+    def _apply(self, fn, recurse=True):
+        fp32 = [t for p in (self.A_log, self.dt_bias, self.D) for t in (p, p.grad) if t is not None]
+
+        def keep(t):
+            out = fn(t)
+            return t.to(out.device) if out.dtype != t.dtype and any(t is p for p in fp32) else out
+        return super()._apply(keep, recurse)
 
     def new_state(self, batch: int):
         """(convolution state, scan state) of `batch` sequences that have not begun."""

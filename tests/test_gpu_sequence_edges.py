@@ -342,3 +342,20 @@ def test_backward_through_tokens_raises():
     m = StateSpaceMixer(16).cuda()
     with pytest.raises(RuntimeError, match="has no gradient"):
         m.step(torch.randn(2, 16, device="cuda"), m.new_state(2)).sum().backward()
+
+
+def test_model_in_16_bits():
+    """A model cast as a whole trains and serves, and its steps equal its prompt."""
+    from sparseflow_b200.snn import SpikingStateSpaceLM
+    torch.manual_seed(0)
+    m = SpikingStateSpaceLM(vocab=40, dim=64, layers=2).cuda().bfloat16()
+    tokens = torch.randint(0, 40, (3, 20), device="cuda")
+    torch.nn.functional.cross_entropy(m(tokens[:, :-1]).flatten(0, 1).float(), tokens[:, 1:].flatten()).backward()
+    assert all(p.grad.dtype == p.dtype and torch.isfinite(p.grad).all() for p in m.parameters())
+    assert m.mixers[0].dt_bias.grad.dtype == torch.float32
+    with torch.no_grad():
+        whole = m(tokens).float()
+        logits, states = m.prefill(tokens[:, :12])
+        parts = [logits] + [m.step(tokens[:, t], states)[:, None] for t in range(12, 20)]
+    # Matrix products of one row and of many may round bf16 values to the one or the other neighbour.
+    assert (torch.cat(parts, 1).float() - whole).norm() <= 0.03 * whole.norm()

@@ -93,3 +93,22 @@ def test_tangents_are_refused(which):
                 fn(**{**tensors, name: dual})
         with pytest.raises(RuntimeError, match="CUDA"):
             fn(**tensors)
+
+
+@pytest.mark.parametrize("cast", [lambda m: m.bfloat16(), lambda m: m.half(), lambda m: m.to(torch.bfloat16),
+                                  lambda m: m.to("cpu", torch.float16)])
+def test_scan_parameters_stay_in_32_bits(cast):
+    """Casting a model leaves the parameters that the scan reads in 32 bits as they are, and their gradients."""
+    from sparseflow_b200.snn import SpikingStateSpaceLM
+    m = SpikingStateSpaceLM(10, 16, 2)
+    m.mixers[0].D.grad = torch.full_like(m.mixers[0].D, 1.001)
+    before = [(p.A_log.clone(), p.dt_bias.clone(), p.D.clone()) for p in m.mixers]
+    cast(m)
+    for mixer, want in zip(m.mixers, before):
+        for got, value in zip((mixer.A_log, mixer.dt_bias, mixer.D), want):
+            assert isinstance(got, torch.nn.Parameter) and got.dtype == torch.float32 and torch.equal(got, value)
+        assert mixer.in_proj.weight.dtype == mixer.conv_weight.dtype == m.embedding.weight.dtype != torch.float32
+    assert m.mixers[0].D.grad.dtype == torch.float32 and (m.mixers[0].D.grad == torch.tensor(1.001)).all()
+    m.float()
+    assert all(p.dtype == torch.float32 for p in m.parameters())
+    assert m.to("meta").mixers[1].A_log.is_meta
