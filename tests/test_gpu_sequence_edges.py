@@ -359,3 +359,125 @@ def test_model_in_16_bits():
         parts = [logits] + [m.step(tokens[:, t], states)[:, None] for t in range(12, 20)]
     # Matrix products of one row and of many may round bf16 values to the one or the other neighbour.
     assert (torch.cat(parts, 1).float() - whole).norm() <= 0.03 * whole.norm()
+
+
+# ----------------------------------------------------------------------------------------------------------------------
+# Bounds that follow the errors, and memory beside outputs
+# ----------------------------------------------------------------------------------------------------------------------
+
+ULP = 2.0 ** -24
+
+
+def _scan_with_bounds(x, dt, A, B, C, D, z):
+    """y and the final states in 64 bits [length, dim(, state)], and what fp32 can be off by, row after row.
+
+    A row's decay is off by the roundings of its exponent (A log2 e, the product, the sums of dt over the 16 rows of a
+    tile and the up to 24 tiles of a segment: 44 |dt A|) and by 8 (the exponential to 2^-22, products, slack), its input
+    dt x B by 4, its sum by 2; y by 20 for 16 products and their sum, and by the gate's exponential and reciprocal."""
+    h = E = H = torch.zeros(A.shape, dtype=A.dtype, device=A.device)
+    ys, offs = [], []
+    gate = z * torch.sigmoid(z)
+    for t in range(x.shape[0]):
+        v = dt[t][:, None] * A
+        a, w = torch.exp(v), (dt[t] * x[t])[:, None] * B[t]
+        h, size = a * h + w, a * H + w.abs()
+        E = a * (E + (44 * v.abs() + 8) * ULP * H) + 4 * ULP * w.abs() + 2 * ULP * size
+        H = size
+        p = (h * C[t]).sum(-1) + D * x[t]
+        m = (H * C[t].abs()).sum(-1) + (D * x[t]).abs()
+        e = (E * C[t].abs()).sum(-1) + 20 * ULP * m
+        ys.append(p * gate[t])
+        offs.append((e + (2 * z[t].abs() + 10) * ULP * m) * gate[t].abs())
+    return torch.stack(ys), torch.stack(offs), h, E
+
+
+@pytest.mark.parametrize("length", [60, 1100, 16384])
+def test_scan_within_the_bounds_of_32_bits(length):
+    """Whole and cut sequences in fp32, up to a prompt of 16384 rows."""
+    from sparseflow_b200.Kernels.selective_scan import selective_scan
+    m = _scan_inputs((1, length), 64, 16, seed=length)
+    m["dt"], m["dt_bias"] = m["dt"].abs() * 0.1, None
+    y, f = selective_scan(**m, dt_softplus=False, return_final_state=True)
+    rows = [m[k][0].double() for k in ("x", "dt", "B", "C", "z")]
+    want, off, h, E = _scan_with_bounds(rows[0], rows[1], m["A"].double(), rows[2], rows[3], m["D"].double(), rows[4])
+    assert ((y[0].double() - want).abs() <= off + ULP * want.abs()).all()
+    assert ((f[0].double() - h).abs() <= E).all()
+
+
+def test_scan_gradients_within_the_norm_of_32_bits():
+    """Gradients of a cut sequence in fp32: a state remembers about 1 / |dt A| <= 20 rows here, so that each of the two
+    chains that a gradient multiplies is off by at most 44 + 8 * 20 roundings."""
+    from sparseflow_b200.Kernels.selective_scan import selective_scan
+    m = _scan_inputs((1, 1100), 24, 16, seed=3)
+    m["dt"], m["dt_bias"], m["A"] = 0.1 + m["dt"].abs() * 0.1, None, -0.5 - torch.rand(24, 16, device="cuda")
+    names = ("x", "dt", "A", "B", "C", "D", "z")
+    leaves = [m[k].requires_grad_() for k in names]
+    dy = torch.randn_like(m["x"])
+    got = torch.autograd.grad(selective_scan(**m, dt_softplus=False), leaves, dy)
+    want = ref.scan(*ref.f64(*leaves), None, False, None, None, ref.f64(dy))
+    for k, g in zip(names, got):
+        off = (g.double().cpu() - want["d" + k]).norm() / want["d" + k].norm()
+        assert off <= 2 * (44 + 8 * 20) * ULP, (k, off)
+
+
+class _Guarded:
+    """Buffers whose middle is handed out, to see afterwards that what lies around it has stayed."""
+
+    def __init__(self):
+        self.buffers = []
+
+    def __call__(self, numel, dtype=torch.float32, pad=512):
+        buf = torch.full((numel + 2 * pad,), -77.0, device="cuda").to(dtype)
+        self.buffers.append((buf, pad))
+        return buf.data_ptr() + pad * buf.element_size()
+
+    def check(self):
+        for i, (buf, pad) in enumerate(self.buffers):
+            assert (buf[:pad] == -77).all() and (buf[-pad:] == -77).all(), i
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("length, dim, n, groups", [(1, 5, 3, 1), (17, 70, 13, 2), (700, 66, 16, 1), (33, 64, 40, 4)])
+def test_scan_writes_its_outputs_alone(dtype, length, dim, n, groups):
+    from sparseflow_b200 import _lib
+    lib, s, give = _lib.load(), 2, _Guarded()
+    m = _scan_inputs((s, length), dim, n, groups, dtype)
+    init, df, dy = torch.randn(s, dim, n, device="cuda"), torch.randn(s, dim, n, device="cuda"), torch.randn_like(m["x"])
+    p = {k: t.data_ptr() for k, t in m.items()}
+    row, bc = (length * dim, dim), (length * groups * n, groups * n)
+    d = ctypes.byref(_lib.SelectiveScanDesc(length, *row * 3, *bc * 2, s, dim, n, groups, 1, _lib.sf_dtype(dtype), 0))
+    stream = torch.cuda.current_stream().cuda_stream
+    ck = give(lib.sf_selective_scan_checkpoint_bytes(d) // 4)
+    size = lib.sf_selective_scan_workspace_size(d)
+    assert lib.sf_selective_scan(p["x"], p["dt"], p["A"], p["B"], p["C"], p["D"], p["z"], p["dt_bias"], init.data_ptr(),
+                                 None, give(s * length * dim, dtype), give(s * dim * n), ck, d, give(size // 4), size,
+                                 stream) == _lib.SF_OK
+    size = lib.sf_selective_scan_backward_workspace_size(d)
+    x, bc = s * length * dim, s * length * groups * n
+    assert lib.sf_selective_scan_backward(
+        p["x"], p["dt"], p["A"], p["B"], p["C"], p["D"], p["z"], p["dt_bias"], None, ck, dy.data_ptr(), df.data_ptr(),
+        give(x, dtype), give(x, dtype), give(dim * n), give(bc, dtype), give(bc, dtype), give(dim), give(x, dtype),
+        give(dim), give(s * dim * n), d, give(size // 4), size, stream) == _lib.SF_OK
+    give.check()
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows, per, dim", [(1, 1, 7), (6, 3, 96), (40, 20, 4104), (300, 1, 1000)])
+def test_norm_writes_its_outputs_alone(dtype, rows, per, dim):
+    from sparseflow_b200 import _lib
+    lib, give, k = _lib.load(), _Guarded(), _lib.sf_dtype(dtype)
+    y, res, dr, dx = (torch.randn(rows, dim, device="cuda").to(dtype) for _ in range(4))
+    gate = torch.randn(rows // per, dim, device="cuda").to(dtype)
+    w = [torch.randn(dim, device="cuda").to(dtype) for _ in range(3)]
+    d = ctypes.byref(_lib.BlockNormDesc(rows, dim, dim, dim, per, dim, k, k, k, _lib.SF_GATE_SILU, 1.0, 1e-6))
+    stream = torch.cuda.current_stream().cuda_stream
+    inputs = [t.data_ptr() for t in (y, res, gate, *w)]
+    rstd = torch.zeros(2 * rows, device="cuda")
+    assert lib.sf_block_norm(*inputs, give(rows * dim, dtype), give(rows * dim, dtype), rstd.data_ptr(), d,
+                             stream) == _lib.SF_OK
+    size = lib.sf_block_norm_backward_workspace_size(d)
+    assert lib.sf_block_norm_backward(*inputs, rstd.data_ptr(), dr.data_ptr(), dx.data_ptr(), give(rows * dim, dtype),
+                                      give(rows * dim, dtype), give(rows // per * dim, dtype),
+                                      *(give(dim, dtype) for _ in range(3)), d, give(size // 4), size,
+                                      stream) == _lib.SF_OK
+    give.check()
