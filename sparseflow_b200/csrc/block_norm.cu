@@ -738,7 +738,7 @@ int slice_of(int dim) {
 }
 // Rows at work at a time that fill the GPU: 512 threads an SM backward (about 126 registers each), 1024 forward.
 long long rows_at_work(int dim, int threads_per_sm) {
-  const long long rows = 148ll * (threads_per_sm / threads_for(slice_of(dim), 1)) / cluster_of(dim);
+  const long long rows = (long long)seq::kSms * (threads_per_sm / threads_for(slice_of(dim), 1)) / cluster_of(dim);
   return rows < 1 ? 1 : rows;
 }
 
@@ -752,7 +752,7 @@ BwdPlan bwd_plan(const sf_block_norm_desc* d) {
   p.groups = p.shared_gate ? d->rows / d->rows_per_gate : 1;
   p.group_rows = p.shared_gate ? d->rows_per_gate : d->rows;
   // Wide rows that no ring takes: blocks of up to 1024 threads, two an SM.
-  const long long want = d->dim % kV && d->dim > kRingDim ? 296 : rows_at_work(d->dim, 512);
+  const long long want = d->dim % kV && d->dim > kRingDim ? 2 * seq::kSms : rows_at_work(d->dim, 512);
   long long blocks = (want + p.groups - 1) / p.groups;
   if (blocks > p.group_rows) blocks = p.group_rows;
   if (blocks < 1) blocks = 1;

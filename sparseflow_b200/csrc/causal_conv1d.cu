@@ -6,10 +6,10 @@
 //   dw[k] = sum_t g[t] x[t - (W-1) + k];  dbias = sum_t g[t]
 //
 // About W + 9 instructions an element forward against 2 |x| bytes, 3 W + 15 backward against 3 |x|: HBM-bound, if
-// enough bytes are on their way. A thread owns V neighbouring channels (8 or 16 bytes of a row, so a warp reads whole
-// sectors) and walks down a slot of rows with the last W rows in registers. The rows ahead are copied asynchronously
-// to a ring in shared memory, each thread its own, so no barrier guards it. Every x is read once, but for the W - 1
-// rows above each slot, which come from L2. Products and sums are pairs of fp32 (mul/fma .f32x2).
+// enough bytes are on their way. A thread owns V neighbouring channels (8 bytes of a row, so a warp reads whole sectors)
+// and walks down a slot of rows with the last W rows in registers. The rows ahead are copied asynchronously to a ring in
+// shared memory, each thread its own, so no barrier guards it. Every x is read once, but for the W - 1 rows above each
+// slot, which come from L2. Products and sums are pairs of fp32 (mul/fma .f32x2).
 // Measured (bf16, 16384 rows of 4096 channels, 4 taps, SiLU): forward 58 us, 4.6 TB/s; backward 106 + 10 us (sums),
 // 3.8 TB/s: 140 and 240 instructions for 8 channels of a warp's row at 0.6 a cycle, half of them the activation's
 // exponentials and divisions and 16-bit conversions.
@@ -576,11 +576,12 @@ long long slot_rows(const sf_causal_conv1d_desc* d, int V, long long want, long 
   while (rows > 8 && seq::total_slots(d->length, d->n_seq, d->packed, rows) * across < want) rows /= 2;
   return rows;
 }
-// Vector widths (bytes): 16 forward; 8 backward and above 4 taps, whose windows would not fit the registers.
-int fwd_vec(const sf_causal_conv1d_desc* d) { return 8 / (int)dtype_size(d->dtype); }
-int bwd_vec(const sf_causal_conv1d_desc* d) { return 8 / (int)dtype_size(d->dtype); }
-long long fwd_rows(const sf_causal_conv1d_desc* d) { return slot_rows(d, fwd_vec(d), 148 * 3, 64); }
-long long bwd_rows(const sf_causal_conv1d_desc* d) { return slot_rows(d, bwd_vec(d), 148 * 6, 128); }
+// Channels a thread: 8 bytes. With 16 there are half as many warps (forward, ragged prompts of 5003 rows: 38 us against
+// 29), and the windows of the backward pass and of more than 4 taps would not fit the registers.
+constexpr int kVecBytes = 8;
+int vec_of(const sf_causal_conv1d_desc* d) { return kVecBytes / (int)dtype_size(d->dtype); }
+long long fwd_rows(const sf_causal_conv1d_desc* d) { return slot_rows(d, vec_of(d), seq::kSms * 3, 64); }
+long long bwd_rows(const sf_causal_conv1d_desc* d) { return slot_rows(d, vec_of(d), seq::kSms * 6, 128); }
 
 template <typename T, int V, int WT>
 sf_status run_fwd(const ConvArgs& a, dim3 grid, cudaStream_t st) {
@@ -612,23 +613,23 @@ sf_status run_update(const ConvArgs& a, dim3 grid, void* pool, const int32_t* id
 
 using namespace sf;
 
-// CALL<T, V, WT> for the data type, with `BYTES` of channels a thread where `fit` (else one channel), 2, 3, 4 taps or up to 8.
-#define SF_CONV_TYPE(TYPE, BYTES4, BYTES8, CALL, ...)                                        \
-  {                                                                                          \
-    using T = TYPE;                                                                          \
-    constexpr int V4 = BYTES4 / (int)sizeof(T), V8 = BYTES8 / (int)sizeof(T);                \
-    switch (d->width) {                                                                      \
-      case 2: return fit ? CALL<T, V4, 2>(__VA_ARGS__) : CALL<T, 1, 2>(__VA_ARGS__);         \
-      case 3: return fit ? CALL<T, V4, 3>(__VA_ARGS__) : CALL<T, 1, 3>(__VA_ARGS__);         \
-      case 4: return fit ? CALL<T, V4, 4>(__VA_ARGS__) : CALL<T, 1, 4>(__VA_ARGS__);         \
-      default: return fit ? CALL<T, V8, 8>(__VA_ARGS__) : CALL<T, 1, 8>(__VA_ARGS__);        \
-    }                                                                                        \
+// CALL<T, V, WT> for the data type, with V channels a thread where `fit` (else one channel), 2, 3, 4 taps or up to 8.
+#define SF_CONV_TYPE(TYPE, CALL, ...)                                                \
+  {                                                                                  \
+    using T = TYPE;                                                                  \
+    constexpr int V = kVecBytes / (int)sizeof(T);                                    \
+    switch (d->width) {                                                              \
+      case 2: return fit ? CALL<T, V, 2>(__VA_ARGS__) : CALL<T, 1, 2>(__VA_ARGS__);  \
+      case 3: return fit ? CALL<T, V, 3>(__VA_ARGS__) : CALL<T, 1, 3>(__VA_ARGS__);  \
+      case 4: return fit ? CALL<T, V, 4>(__VA_ARGS__) : CALL<T, 1, 4>(__VA_ARGS__);  \
+      default: return fit ? CALL<T, V, 8>(__VA_ARGS__) : CALL<T, 1, 8>(__VA_ARGS__); \
+    }                                                                                \
   }
-#define SF_CONV_DISPATCH(BYTES4, BYTES8, CALL, ...)                                          \
-  switch (d->dtype) {                                                                        \
-    case SF_DTYPE_F32: SF_CONV_TYPE(float, BYTES4, BYTES8, CALL, __VA_ARGS__)                \
-    case SF_DTYPE_F16: SF_CONV_TYPE(__half, BYTES4, BYTES8, CALL, __VA_ARGS__)               \
-    default: SF_CONV_TYPE(__nv_bfloat16, BYTES4, BYTES8, CALL, __VA_ARGS__)                  \
+#define SF_CONV_DISPATCH(CALL, ...)                                 \
+  switch (d->dtype) {                                               \
+    case SF_DTYPE_F32: SF_CONV_TYPE(float, CALL, __VA_ARGS__)       \
+    case SF_DTYPE_F16: SF_CONV_TYPE(__half, CALL, __VA_ARGS__)      \
+    default: SF_CONV_TYPE(__nv_bfloat16, CALL, __VA_ARGS__)         \
   }
 
 extern "C" sf_status sf_causal_conv1d(const void* x, const void* weight, const void* bias, const void* initial_state,
@@ -641,13 +642,13 @@ extern "C" sf_status sf_causal_conv1d(const void* x, const void* weight, const v
   ConvArgs a = base_args(x, weight, bias, initial_state, seq_offsets, d);
   a.y = y;
   a.final_state = final_state;
-  const bool fit = vectors_fit(fwd_vec(d), d, !d->packed, {x, initial_state, y, final_state});
+  const bool fit = vectors_fit(vec_of(d), d, !d->packed, {x, initial_state, y, final_state});
   a.slot_rows = fwd_rows(d);
   const long long slots = seq::total_slots(d->length, d->n_seq, d->packed, a.slot_rows);
   if (slots > INT32_MAX) return SF_ERR_UNSUPPORTED;
   const dim3 grid((unsigned)slots);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  SF_CONV_DISPATCH(8, 8, run_fwd, a, grid, st)
+  SF_CONV_DISPATCH(run_fwd, a, grid, st)
 }
 
 extern "C" size_t sf_causal_conv1d_backward_workspace_size(const sf_causal_conv1d_desc* d) {
@@ -658,7 +659,7 @@ extern "C" size_t sf_causal_conv1d_backward_workspace_size(const sf_causal_conv1
 
 static sf_status conv_backward(const ConvArgs& a, const sf_causal_conv1d_desc* d, bool fit, dim3 grid,
                                cudaStream_t st) {
-  SF_CONV_DISPATCH(8, 8, run_bwd, a, grid, st)
+  SF_CONV_DISPATCH(run_bwd, a, grid, st)
 }
 
 extern "C" sf_status sf_causal_conv1d_backward(const void* x, const void* weight, const void* bias,
@@ -686,7 +687,7 @@ extern "C" sf_status sf_causal_conv1d_backward(const void* x, const void* weight
     a.slot_rows = bwd_rows(d);
     slots = seq::total_slots(d->length, d->n_seq, d->packed, a.slot_rows);
     if (slots > INT32_MAX) return SF_ERR_UNSUPPORTED;
-    const bool fit = vectors_fit(bwd_vec(d), d, !d->packed,
+    const bool fit = vectors_fit(vec_of(d), d, !d->packed,
                                  {x, initial_state, dy, d_final_state, dx, d_initial_state});
     const sf_status s = conv_backward(a, d, fit, dim3((unsigned)slots), st);
     if (s != SF_OK) return s;
@@ -705,8 +706,8 @@ extern "C" sf_status sf_causal_conv1d_update(const void* x, void* state_pool, co
   if (!x || !y || (!state_pool && n_slots > 0)) return SF_ERR_INVALID_ARG;
   ConvArgs a = base_args(x, weight, bias, nullptr, nullptr, d);
   a.y = y;
-  const bool fit = vectors_fit(bwd_vec(d), d, false, {x, state_pool, y});
+  const bool fit = vectors_fit(vec_of(d), d, false, {x, state_pool, y});
   const dim3 grid(d->n_seq);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  SF_CONV_DISPATCH(8, 8, run_update, a, grid, state_pool, state_indices, n_slots, st)
+  SF_CONV_DISPATCH(run_update, a, grid, state_pool, state_indices, n_slots, st)
 }

@@ -179,7 +179,11 @@ int tiles_of(const sf_selective_scan_desc* d) {  // blocks for the channels of a
 // finds the segments' shares included). Whole against cut, forward: 64 blocks 0.25 / 0.14, 128: 0.25 / 0.24, 192:
 // 0.33 / 0.36, 256: 0.33 / 0.48, 512: 0.58 / 0.95; backward: 128 blocks 0.76 / 0.52, 256: 1.02 / 0.96, 320: 1.29 / 1.16,
 // 384: 1.29 / 1.39, 512: 1.97 / 1.86. The cheaper is taken; 0.01 ms stands for the launch that cutting adds. Packed
-// sequences count as of equal length (the host does not know theirs).
+// sequences count as of equal length (the host does not know theirs). The costs of 16 states in bf16 stand for all: of 4
+// to 128 states in bf16 and fp32, 512 to 8192 rows and 64 to 512 blocks, the choice was within 8 % of the better one, but
+// for 128 blocks of 512 rows of up to 8 states, kept whole (0.14 ms, cut 0.07), 256 of 4 states (0.14, cut 0.12) and, cut,
+// the backward pass of 512 blocks of up to 8 states in bf16 (2.05 ms with the forward pass, whole 1.80), of 256 blocks in
+// fp32 (1.48 / 1.35) and of 64 or more states (1.57 / 1.46).
 struct SegmentCosts {
   int resident;  // blocks on an SM
   double t[4], cut;
@@ -192,7 +196,7 @@ long long segment_rows(const sf_selective_scan_desc* d, const SegmentCosts& k) {
   const long long across = (long long)tiles_of(d) * d->groups, blocks = across * d->n_seq;
   const long long total = d->packed ? d->length : d->length * d->n_seq;
   const double length = (double)total / d->n_seq / 2048.;
-  const long long w = (blocks + 147) / 148;
+  const long long w = (blocks + seq::kSms - 1) / seq::kSms;
   double whole = (double)(w / k.resident) * k.t[k.resident - 1];
   if (w % k.resident) whole += k.t[w % k.resident - 1];
   if (whole * length <= k.cut * blocks * length + 0.01) return kWhole;

@@ -766,7 +766,7 @@ __device__ __forceinline__ int sums_first(int lane) {
   return first;
 }
 
-// Tiles from the last to the first: a tile's states again from its checkpoint, half a tile at a time in registers,
+// Tiles from the last to the first: a tile's states again from its checkpoint, a quarter (kPart rows) at a time in registers,
 // then its rows backwards. Sums over a block's channels of gB and gC go to part_bc[tile][row][group][2][NP], added
 // over the tiles by scan_bc_reduce_kernel; sums over a segment of gA, gD and gbias to part_a / part_d, added over
 // the segments by scan_sum_kernel. No atomics: the order of every sum is fixed.
@@ -1047,7 +1047,7 @@ sf_status run_fwd(const ScanArgs& a, dim3 grid, cudaStream_t st) {
     scan_carry_kernel<T, LPC, CPT, VEC, false><<<grid, threads, bytes, st>>>(a);
   }
   constexpr size_t smem = sizeof(FwdSmem<T, LPC, CPT, VEC>);
-  auto kernel = (long long)grid.x * grid.y > 3 * 148 ? scan_fwd_kernel<T, LPC, CPT, VEC, 4>
+  auto kernel = (long long)grid.x * grid.y > 3 * kSms ? scan_fwd_kernel<T, LPC, CPT, VEC, 4>
                                                      : scan_fwd_kernel<T, LPC, CPT, VEC, 3>;
   if (!prepare_smem(kernel, smem)) return SF_ERR_CUDA;
   kernel<<<grid, threads, smem, st>>>(a);

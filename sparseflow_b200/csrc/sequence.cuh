@@ -8,7 +8,11 @@ namespace seq {
 
 typedef unsigned long long u64;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kSms = 148;  // of a B200
 
+// 2^v and 1 / v in one instruction each, good to about two units of the last place; results below 2^-126 are 0. Every
+// decay, gate and softplus takes one or two, and their pipe is what the scan runs against; a full exponential and division
+// would take several instructions more. The scan in fp32 is 7e-7 off the 64-bit result, plain 32-bit operations 4e-7.
 __device__ __forceinline__ float ex2(float v) {
   float r;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
