@@ -160,12 +160,15 @@ def selective_scan_update(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B:
     """
     require_cuda(x, dt, A, B, C, state, D, z, dt_bias, state_indices)
     if torch.is_grad_enabled() and (x.requires_grad or dt.requires_grad or A.requires_grad or B.requires_grad
-                                    or C.requires_grad or state.requires_grad or needs_grad(D, z, dt_bias)):
+                                    or C.requires_grad or state.requires_grad
+                                    or (D is not None and D.requires_grad) or (z is not None and z.requires_grad)
+                                    or (dt_bias is not None and dt_bias.requires_grad)):
         return without_gradient(selective_scan_update, x, dt, A, B, C, state, D, z, dt_bias, dt_softplus,
                                 state_indices)
     key = (x.shape, x.stride(), x.dtype, dt.shape, dt.stride(), dt.dtype, B.shape, B.stride(), B.dtype, C.shape,
-           C.stride(), C.dtype, A.shape, A.stride(), A.dtype, state.shape, state.stride(), state.dtype, layout(D),
-           layout(z), layout(dt_bias), layout(state_indices), dt_softplus)
+           C.stride(), C.dtype, A.shape, A.stride(), A.dtype, state.shape, state.stride(), state.dtype,
+           None if D is None else (D.shape, D.stride(), D.dtype), None if z is None else (z.shape, z.stride(), z.dtype),
+           layout(dt_bias), layout(state_indices), dt_softplus)
     desc = _update_plans.get(key)
     if desc is None:
         x, dt, A, B, C, D, z, dt_bias, desc = _update_plan(x, dt, A, B, C, state, D, z, dt_bias, dt_softplus,

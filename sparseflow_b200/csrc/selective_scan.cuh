@@ -92,9 +92,10 @@ __device__ __forceinline__ long long row0(const ScanArgs& a, const Span& s) {
   return a.rows.offsets ? s.begin : (long long)s.s * a.rows.length;
 }
 
-// Four values of a [.., state] row of floats from state n on, 0 past the end.
+// Four values of a [.., state] row of floats from state n on, 0 past the end. WIDE: as one word without asking.
+template <bool WIDE = false>
 __device__ __forceinline__ void load4(float (&o)[kS], const float* p, int n, const ScanArgs& a) {
-  if (a.wide) {
+  if (WIDE || a.wide) {
     if (n < a.state) {
       const float4 v = *reinterpret_cast<const float4*>(p + n);
       o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w;
@@ -106,8 +107,9 @@ __device__ __forceinline__ void load4(float (&o)[kS], const float* p, int n, con
 #pragma unroll
   for (int i = 0; i < kS; ++i) o[i] = n + i < a.state ? p[n + i] : 0.f;
 }
+template <bool WIDE = false>
 __device__ __forceinline__ void store4(float* p, const float (&v)[kS], int n, const ScanArgs& a) {
-  if (a.wide) {
+  if (WIDE || a.wide) {
     if (n < a.state) *reinterpret_cast<float4*>(p + n) = make_float4(v[0], v[1], v[2], v[3]);
     return;
   }
