@@ -264,9 +264,10 @@ sf_status sf_lif_multistep_events(const void* x, float* v_inout, void* spikes_ou
 /* packed (seq_offsets: n_seq + 1 int32 on the device, ascending from 0;     */
 /* sequence s is rows seq_offsets[s] .. seq_offsets[s+1]-1 of `length` rows  */
 /* in all; offsets are clamped to [0, length], so wrong ones read no other   */
-/* memory); rows of no sequence are not written. A sequence may be empty. Strides are in elements; inputs may be  */
-/* slices of wider rows, outputs are contiguous. Outputs must not overlap    */
-/* inputs. Sums and states are fp32 whatever the data type.                  */
+/* memory); rows of no sequence are not written. A sequence may be empty.    */
+/* Strides are in elements; inputs may be slices of wider rows, outputs are  */
+/* contiguous and must not overlap inputs. Sums and states are fp32 whatever */
+/* the data type.                                                            */
 /* ------------------------------------------------------------------------ */
 typedef struct sf_causal_conv1d_desc {
   int64_t length;                       /* rows per sequence; packed: rows in all */
